@@ -1,10 +1,7 @@
 """Constant tables: generated by nnsp_amd/tables.py from closed-form rules and
-checked word-for-word against the reference (source tables and the CMSIS-DSP
-data sections of evb/libs/libCMSISDSP.a, read as data, never executed)."""
+checked word-for-word against the reference's source tables."""
 import os
 import re
-import subprocess
-import tempfile
 
 import numpy as np
 import pytest
@@ -37,38 +34,6 @@ def _c_table(path, name):
 def test_source_tables_exact(fname, sym, gen):
     ref = _c_table(os.path.join(REFERENCE, "ns-nnsp", "src", fname), sym)
     np.testing.assert_array_equal(gen().astype(np.int64), ref)
-
-
-def _sections(obj):
-    out = {}
-    for line in subprocess.check_output(["readelf", "-S", "-W", obj]).decode().splitlines():
-        m = re.search(r"\]\s+(\S+)\s+PROGBITS\s+\S+\s+([0-9a-f]+)\s+([0-9a-f]+)", line)
-        if m:
-            out[m.group(1)] = (int(m.group(2), 16), int(m.group(3), 16))
-    return out
-
-
-@needs_reference
-def test_cmsis_tables_exact():
-    lib = os.path.join(REFERENCE, "evb", "libs", "libCMSISDSP.a")
-    with tempfile.TemporaryDirectory() as d:
-        subprocess.check_call(["ar", "x", lib, "arm_common_tables.c.obj"], cwd=d)
-        obj = os.path.join(d, "arm_common_tables.c.obj")
-        data = open(obj, "rb").read()
-        secs = _sections(obj)
-
-        def get(name, dt):
-            o, s = secs[".rodata." + name]
-            return np.frombuffer(data[o:o + s], dtype=dt)
-
-        np.testing.assert_array_equal(tables.cfft256_twiddles(), get("twiddleCoef_256_q31", "<i4"))
-        a, b = tables.rfft_split_full()
-        np.testing.assert_array_equal(a, get("realCoefAQ31", "<i4"))
-        np.testing.assert_array_equal(b, get("realCoefBQ31", "<i4"))
-        br = get("armBitRevIndexTable_fixed_256", "<u2").astype(np.int64).reshape(-1, 2) // 8
-        rev = tables.bitrev8()
-        swaps = {tuple(sorted((i, int(rev[i])))) for i in range(256) if i != rev[i]}
-        assert {tuple(sorted(map(int, p))) for p in br} == swaps and len(br) == len(swaps)
 
 
 def test_mel_segments_per_bank_fit_fe_kernel():
