@@ -7,11 +7,14 @@ API and a batched multi-stream API).  This package is its Python host mirror.
 """
 from .nets import SPECS, NetData, NetSpec, synth_net  # noqa: F401
 
-__all__ = ["SPECS", "NetData", "NetSpec", "synth_net", "NNSPBatch"]
+__all__ = ["SPECS", "NetData", "NetSpec", "synth_net", "NNSPBatch", "GatedDelta", "BlockNorm"]
 
 
 def __getattr__(name):
     if name == "NNSPBatch":
         from .engine import NNSPBatch
         return NNSPBatch
+    if name in ("GatedDelta", "BlockNorm"):
+        from . import seq
+        return getattr(seq, name)
     raise AttributeError(name)

@@ -1,5 +1,5 @@
-"""ctypes view of libnnsp_mi355x.so (the C-ABI of include/nnsp_api.h and
-include/nnsp_batch.h).
+"""ctypes view of libnnsp_mi355x.so (the C-ABI of include/nnsp_api.h,
+include/nnsp_batch.h and include/nnsp_seq.h).
 
 The library is built in-tree (``nnsp_amd/libnnsp_mi355x.so``, see
 ``__graft_entry__.build``).  Loading fails loudly when it is missing: there is
@@ -109,6 +109,27 @@ class PostState(C.Structure):
                 ("outputs", C.c_int16 * 3), ("pad1", C.c_int16)]
 
 
+class DeltaArgs(C.Structure):
+    """nnsp_delta_args (include/nnsp_seq.h)."""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "n_streams", "n_frames", "key_heads", "value_heads", "dk", "dv",
+                                          "l2norm")]
+                + [("scale", C.c_float), ("eps", C.c_float)]
+                + [(n + "_stride", C.c_int64 * 3) for n in ("q", "k", "v", "g", "beta", "out")]
+                + [(n, C.c_void_p) for n in ("q", "k", "v", "g", "beta", "lens", "state_in", "out", "state_out",
+                                             "workspace")]
+                + [("workspace_bytes", C.c_size_t)])
+
+
+class NormArgs(C.Structure):
+    """nnsp_norm_args (include/nnsp_seq.h)."""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "res_dtype", "post", "act", "pre", "dim")]
+                + [("rows", C.c_int64), ("groups", C.c_int32), ("pad0", C.c_int32)]
+                + [(n, C.c_float) for n in ("eps_post", "eps_pre", "res_scale", "pad1")]
+                + [(n + "_stride", C.c_int64 * 2) for n in ("x", "gate", "res_in", "res_out", "y")]
+                + [(n, C.c_void_p) for n in ("x", "gate", "res_in", "w_post", "b_post", "col_scale", "w_pre", "b_pre",
+                                             "res_out", "y")])
+
+
 P = C.c_void_p
 I = C.c_int
 # error codes (include/nnsp_batch.h)
@@ -160,6 +181,11 @@ def _declare(L: C.CDLL) -> None:
                                             C.POINTER(C.c_float), C.POINTER(I)]),
         "nnsp_synth_pcm": (I, [P, I, I, C.c_uint64, I, C.c_int64, I, P]),
         "nnsp_synth_pcm_mix": (I, [P, I, I, C.c_uint64, I, C.c_int64, I, P, I, I, I, P]),
+        "nnsp_delta_contiguous": (I, [P]),
+        "nnsp_delta_workspace": (I, [P, C.POINTER(C.c_size_t)]),
+        "nnsp_delta_exec_device": (I, [P, P]),
+        "nnsp_norm_contiguous": (I, [P]),
+        "nnsp_norm_exec_device": (I, [P, P]),
         "nnsp_device_count": (I, [C.POINTER(I)]),
         "nnsp_set_device": (I, [I]),
         "nnsp_device_info": (I, [C.POINTER(I), C.POINTER(I), C.c_char_p, I]),
