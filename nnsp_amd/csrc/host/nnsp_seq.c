@@ -197,6 +197,7 @@ int nnsp_delta_exec_device(const nnsp_delta_args *a, void *stream)
                            {"state_out", a->state_out, a->state_out ? 4 : 0},
                            {"workspace", a->workspace, need ? 16 : 0}};
     TRY(check_ptrs(who, arg, (int)(sizeof arg / sizeof *arg), stream));
+    if (a->n_frames > NNSP_DELTA_STEP_FRAMES && a->dk <= NNSP_DELTA_CHUNK_DK) return nnspk_launch_delta_chunk(a, stream);
     return nnspk_launch_delta_step(a, stream);
 }
 

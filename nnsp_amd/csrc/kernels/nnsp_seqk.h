@@ -11,9 +11,11 @@ extern "C" {
 
 /* largest head width of the delta rule and row length of the norms */
 #define NNSP_DELTA_MAX_D 256
+#define NNSP_DELTA_CHUNK_DK 128
 #define NNSP_NORM_MAX_DIM 16384
 
 int nnspk_launch_delta_step(const nnsp_delta_args *a, void *stream);
+int nnspk_launch_delta_chunk(const nnsp_delta_args *a, void *stream); /* dk <= NNSP_DELTA_CHUNK_DK */
 int nnspk_launch_norm(const nnsp_norm_args *a, void *stream);
 
 /* 1: kernels on device `dev` can use p (its own device memory, pinned host or
