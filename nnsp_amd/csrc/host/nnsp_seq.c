@@ -197,8 +197,10 @@ int nnsp_delta_exec_device(const nnsp_delta_args *a, void *stream)
                            {"state_out", a->state_out, a->state_out ? 4 : 0},
                            {"workspace", a->workspace, need ? 16 : 0}};
     TRY(check_ptrs(who, arg, (int)(sizeof arg / sizeof *arg), stream));
-    if (a->n_frames > NNSP_DELTA_STEP_FRAMES && a->dk <= NNSP_DELTA_CHUNK_DK) return nnspk_launch_delta_chunk(a, stream);
-    return nnspk_launch_delta_step(a, stream);
+    if (a->n_frames <= NNSP_DELTA_STEP_FRAMES || a->dk > NNSP_DELTA_CHUNK_DK) return nnspk_launch_delta_step(a, stream);
+    if (a->dtype == NNSP_BF16) return nnspk_launch_delta_chunk_bf16(a, stream);
+    if (a->dtype == NNSP_F16) return nnspk_launch_delta_chunk_f16(a, stream);
+    return nnspk_launch_delta_chunk_f32(a, stream);
 }
 
 /* ---- norms around a block ---- */
