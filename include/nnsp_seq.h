@@ -75,7 +75,7 @@ extern "C" {
  * time, need one each).
  *
  * Limits: dk, dv 1 .. 256; value_heads a multiple of key_heads;
- * n_streams * value_heads * ceil(dv / 16) below 2^31.
+ * n_frames at most 2^30; n_streams * value_heads * ceil(dv / 16) below 2^31.
  */
 #define NNSP_DELTA_STEP_FRAMES 8
 typedef struct {

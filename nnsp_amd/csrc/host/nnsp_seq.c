@@ -125,6 +125,10 @@ static int delta_sizes(const nnsp_delta_args *a, const char *who)
         nnsp_set_error("%s: dk, dv must be in 1..%d", who, NNSP_DELTA_MAX_D);
         return NNSP_EUNSUPPORTED;
     }
+    if (a->n_frames > 1 << 30) {
+        nnsp_set_error("%s: n_frames must be at most 2^30", who);
+        return NNSP_EUNSUPPORTED;
+    }
     if ((double)a->n_streams * a->value_heads * ((a->dv + 15) / 16) >= 2147483648.0) {
         nnsp_set_error("%s: n_streams * value_heads * ceil(dv / 16) must stay below 2^31", who);
         return NNSP_EUNSUPPORTED;
@@ -151,11 +155,26 @@ int nnsp_delta_contiguous(nnsp_delta_args *a)
     return 0;
 }
 
+/* How a call runs: frame by frame (few frames, or heads too wide for the matrix
+ * kernels' LDS), in chunks, or in chunks in two passes.  */
+enum { DELTA_STEP, DELTA_CHUNK, DELTA_SPLIT };
+
+static int delta_way(const nnsp_delta_args *a)
+{
+    if (a->n_frames <= NNSP_DELTA_STEP_FRAMES || a->dk > NNSP_DELTA_CHUNK_DK) return DELTA_STEP;
+    const long long rows = (long long)a->n_streams * a->value_heads * ((a->dv + 127) / 128);
+    return rows < 1024 && a->n_frames > 64 ? DELTA_SPLIT : DELTA_CHUNK;
+}
+
 int nnsp_delta_workspace(const nnsp_delta_args *a, size_t *bytes)
 {
     if (!bytes) return bad("nnsp_delta_workspace", "NULL arguments");
     *bytes = 0;
     TRY(delta_sizes(a, "nnsp_delta_workspace"));
+    if (delta_way(a) != DELTA_SPLIT || a->n_streams == 0) return 0;
+    *bytes = (size_t)(a->dtype == NNSP_BF16  ? nnspk_delta_split_bytes_bf16(a)
+                      : a->dtype == NNSP_F16 ? nnspk_delta_split_bytes_f16(a)
+                                             : nnspk_delta_split_bytes_f32(a));
     return 0;
 }
 
@@ -197,10 +216,11 @@ int nnsp_delta_exec_device(const nnsp_delta_args *a, void *stream)
                            {"state_out", a->state_out, a->state_out ? 4 : 0},
                            {"workspace", a->workspace, need ? 16 : 0}};
     TRY(check_ptrs(who, arg, (int)(sizeof arg / sizeof *arg), stream));
-    if (a->n_frames <= NNSP_DELTA_STEP_FRAMES || a->dk > NNSP_DELTA_CHUNK_DK) return nnspk_launch_delta_step(a, stream);
-    if (a->dtype == NNSP_BF16) return nnspk_launch_delta_chunk_bf16(a, stream);
-    if (a->dtype == NNSP_F16) return nnspk_launch_delta_chunk_f16(a, stream);
-    return nnspk_launch_delta_chunk_f32(a, stream);
+    const int way = delta_way(a), split = way == DELTA_SPLIT;
+    if (way == DELTA_STEP) return nnspk_launch_delta_step(a, stream);
+    if (a->dtype == NNSP_BF16) return nnspk_launch_delta_chunk_bf16(a, split, stream);
+    if (a->dtype == NNSP_F16) return nnspk_launch_delta_chunk_f16(a, split, stream);
+    return nnspk_launch_delta_chunk_f32(a, split, stream);
 }
 
 /* ---- norms around a block ---- */

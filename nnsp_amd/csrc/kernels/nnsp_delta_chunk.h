@@ -12,14 +12,17 @@
 // triangular inverse.  T and P need no state; the rest is five matrix products.
 //
 // Numbers.  The state, T and U are 32-bit values, and the matrix cores take 16
-// bits: each is scaled by a power of two (its column's or row's largest to
-// 2^14 .. 2^15) and split into an fp16 high and low part, 22 bits in all, and
-// products keep hi hi + hi lo + lo hi, accumulated in 32 bits.  Rows of q and k
-// are scaled the same way, which makes one fp16 part exact for bf16 and fp16
-// (bf16 to 2^-39 of the row's largest); fp32 takes two.  All other factors
-// (norms, decays, beta) multiply in 32 bits outside the products.  For bf16
-// outputs the products that reach only the output (Q S0, P U) use one part of
-// S0, P and U, 11 bits, below the output's own 8.
+// bits: each is scaled by a power of two and split into an fp16 high and low
+// part, 22 bits in all, and products keep hi hi + hi lo + lo hi, accumulated in
+// 32 bits.  The powers come from the largest magnitude among a wave's columns
+// or from a bound; an fp16 pair under a bound of 2^14 is good to 2^-24 in
+// absolute terms, 2^-38 of the bound, so neither a loose bound nor a column much
+// smaller than its neighbours costs precision.  q and k go in with
+// their rows scaled too: fp16 and bf16 in one part (exact down to 2^-19 and
+// 2^-28 of a row's largest, to 2^-30 and 2^-39 of it below), fp32 in two.  All other factors (norms, decays, beta) multiply
+// in 32 bits outside the products.  For bf16 outputs the products that reach
+// only the output (Q S0, P U) use one part of S0, P and U, 11 bits, below the
+// output's own 8.
 //
 // Layout.  A wave owns 16 NB columns of the state and keeps them in registers
 // in the 16x16 accumulator layout (lane: column lane % 16, rows 4 (lane / 16)
@@ -41,6 +44,14 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 constexpr int C = 64;       // frames of a chunk
+constexpr long long DELTA_SLAB_BYTES = 96ll << 20;
+
+// sizes of a call in two passes
+struct DeltaSplit {
+    int chunks, slab;                           // chunks of the call, of a slab
+    long long kq_bytes, tp_bytes, state_bytes;  // images of a chunk; the state between slabs
+    long long bytes() const { return state_bytes + slab * (kq_bytes + tp_bytes); }
+};
 
 __device__ __forceinline__ f32x4 mma(h8 a, h8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -62,9 +73,9 @@ template <int CTRL>
 __device__ __forceinline__ float max_dpp(float x) {
     return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true)));
 }
-// largest over the 16 lanes of a row
-__device__ __forceinline__ float max_row16(float x) {
-    return max_dpp<0x128>(max_dpp<0x141>(max_dpp<0x4e>(max_dpp<0xb1>(x))));
+// largest over the wave
+__device__ __forceinline__ float wave_max(float x) {
+    return max_xor16_32(max_dpp<0x128>(max_dpp<0x141>(max_dpp<0x4e>(max_dpp<0xb1>(x)))));
 }
 __device__ __forceinline__ float amax4(float m, const f32x4& x) {
     return fmaxf(fmaxf(fmaxf(m, fabsf(x[0])), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
@@ -80,21 +91,26 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 
-// two accumulator tiles times s as the high and low B operand of a 32-deep product
-__device__ __forceinline__ void split(const f32x4& a, const f32x4& b, float s, h8& hi, h8& lo) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = i < 4 ? a[i & 3] : b[i & 3];
-        hi[i] = (_Float16)(x * s);
-        lo[i] = (_Float16)fmaf(x, s, -(float)hi[i]);
-    }
+// a s0 and b s1 rounded to fp16
+__device__ __forceinline__ unsigned pack(float a, float s0, float b, float s1) {
+    unsigned d;
+    asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(d) : "v"(a), "v"(s0));
+    asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(d) : "v"(b), "v"(s1));
+    return d;
 }
-__device__ __forceinline__ h8 high(const f32x4& a, const f32x4& b, float s) {
-    h8 r;
+// two accumulator tiles times their rows' factors s as the high and low B
+// operand of a 32-deep product
+template <bool LOW>
+__device__ __forceinline__ void split(const f32x4& a, const f32x4& b, const f32x4& sa, const f32x4& sb, h8& hi, h8& lo) {
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    hi = __builtin_bit_cast(h8, u4{pack(a[0], sa[0], a[1], sa[1]), pack(a[2], sa[2], a[3], sa[3]),
+                                   pack(b[0], sb[0], b[1], sb[1]), pack(b[2], sb[2], b[3], sb[3])});
+    if (LOW)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = (_Float16)((i < 4 ? a[i & 3] : b[i & 3]) * s);
-    return r;
+        for (int i = 0; i < 8; ++i)
+            lo[i] = (_Float16)fmaf(i < 4 ? a[i & 3] : b[i & 3], i < 4 ? sa[i & 3] : sb[i & 3], -(float)hi[i]);
 }
+__device__ __forceinline__ f32x4 all4(float x) { return f32x4{x, x, x, x}; }
 
 // 4 rows x 4 columns per lane group, transposed: lane l of 16 gets column l of rows 0 .. 3
 __device__ __forceinline__ s4 read_tr(const void* p) {
@@ -121,34 +137,41 @@ struct Geo {
     static constexpr bool WIDE = std::is_same<T, float>::value;       // 32-bit input
     static constexpr int KP = WIDE ? 2 : 1;                           // parts of q and k
     static constexpr int OP = std::is_same<T, __bf16>::value ? 1 : 2; // parts of what only the output takes
-    static constexpr int KS = NKT * 32 + 8;                           // row of K and Q, halves
     static constexpr int W = 64 * NB;                                 // columns of a workgroup
     static constexpr int VS = 16 * NB + (WIDE ? 4 : 8);               // row of a wave's V, elements
 };
 
-template <class T, int NKT, int NB>
-struct Lds {
-    using G = Geo<T, NKT, NB>;
-    alignas(16) _Float16 K[G::KP][C][G::KS], Q[G::KP][C][G::KS];
-    union {
-        Tri T_[2];
-        float D[4][16][20];        // transposed inverses of the diagonal blocks, until T is written
-    };
-    Tri P_[G::OP];
-    union {
-        alignas(16) float A[C][C + 4];  // A transposed, until T is done
-        alignas(16) T V[4][C][G::VS];   // from then on: each wave's columns of v, then of out
-    };
-    // factors of a frame; e() is a decay, G the sum of g, s and e the first and last frame of its 16
-    alignas(16) float kx[C], qx[C], kn[C], qn[C];  // norm times 2^-scale, length after the norm
-    alignas(16) float gh[C], gl[C], beta[C];       // log2 of the decay up to the frame (two parts), beta
-    alignas(16) float ab[C], ar[C];                // A rows: beta kx, times e(G - G_s)
-    alignas(16) float pb[C], pr[C], pi[C];         // P rows: qx 2^scale, times e(G - G_s); 2^-scale
-    alignas(16) float kc[C];                       // columns of both: kx e(G_e - G)
-    alignas(16) float fx[C], fk[C], fq[C];         // of K S0, of U into the state, of Q S0
-    float ti[4];                                   // 2^-scale of T's row tiles
-    float all;                                     // decay over the whole chunk
+// q and k of a chunk as the products take them
+template <class T, int NKT>
+struct KQ {
+    static constexpr int KP = std::is_same<T, float>::value ? 2 : 1, KS = NKT * 32 + 8;
+    alignas(16) _Float16 K[KP][C][KS], Q[KP][C][KS];
 };
+// what else a chunk's products take; e() is a decay, G the sum of g
+template <class T>
+struct TP {
+    static constexpr int OP = std::is_same<T, __bf16>::value ? 1 : 2;
+    Tri T_[2], P_[OP];
+    alignas(16) float beta[C], fx[C], fk[C], fq[C];  // factors of v, K S0, U into the state, Q S0
+    alignas(16) float pi[C];                         // 2^-scale of P's rows
+    float ti[4];                                     // 2^-scale of T's row tiles
+    float all, fkmax, pad[2];                        // decay over the whole chunk; largest fk
+};
+// what making T and P takes besides; s and e are the first and last frame of a frame's 16
+struct Make {
+    alignas(16) float kx[C], qx[C], kn[C], qn[C];  // norm times 2^-scale, length after the norm
+    alignas(16) float gh[C], gl[C];                // log2 of the decay up to the frame (two parts)
+    alignas(16) float ab[C], ar[C];                // A rows: beta kx, times e(G - G_s)
+    alignas(16) float pb[C], pr[C];                // P rows: qx 2^scale, times e(G - G_s)
+    alignas(16) float kc[C];                       // columns of both: kx e(G_e - G)
+};
+struct TriA {
+    alignas(16) float A[C][C + 4];  // A transposed
+};
+struct Diag {
+    alignas(16) float D[4][16][20];  // transposed inverses of the diagonal blocks
+};
+static_assert(sizeof(Diag) <= 2 * sizeof(Tri), "the inverses lie where T is written afterwards");
 
 // raw rows of q and k on their way to LDS: thread (row, quarter) holds chunks of
 // 8 elements quarter, quarter + 4, ...
@@ -172,35 +195,54 @@ __device__ __forceinline__ void fetch_rows(RawRows<T, NKT>& r, const T* p, int q
         }
     }
 }
-// scaled fp16 parts to LDS; returns 2^-scale, sets the sum of squares
+// scaled fp16 parts to LDS; returns 2^-scale (0 of a row of zeros), sets the sum of squares
 template <class T, int NKT, int KP, int KS>
 __device__ __forceinline__ float stage_rows(const RawRows<T, NKT>& r, _Float16 (*dst)[C][KS], int row, int quarter, float& ss) {
-    float m = 0.0f;
     ss = 0.0f;
-#pragma unroll
-    for (int i = 0; i < NKT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = (float)r.x[i][j];
-            m = fmaxf(m, fabsf(x));
-            ss = fmaf(x, x, ss);
-        }
-    m = max_dpp<0x4e>(max_dpp<0xb1>(m));
-    ss = add_xor2(add_xor1(ss));
     float inv;
-    const float s = scale_of(m, inv);
+    if constexpr (std::is_same<T, _Float16>::value) {
+        // rows to a length of 2^5 .. 2^6, by the exponent of the sum of squares (which fp16 keeps in fp32's range)
 #pragma unroll
-    for (int i = 0; i < NKT; ++i) {
-        h8 hi, lo;
+        for (int i = 0; i < NKT; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float x = (float)r.x[i][j];
-            hi[j] = (_Float16)(x * s);
-            if (KP == 2) lo[j] = (_Float16)fmaf(x, s, -(float)hi[j]);
+            for (int j = 0; j < 8; j += 2) {
+                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                const h2 x = {r.x[i][j], r.x[i][j + 1]};
+                ss = __builtin_amdgcn_fdot2(x, x, ss, false);
+            }
+        ss = add_xor2(add_xor1(ss));
+        const int e = min(max(5 - (((__float_as_int(ss) >> 23) - 127) >> 1), -14), 15);
+        const _Float16 s = __builtin_bit_cast(_Float16, (unsigned short)((15 + e) << 10));
+        inv = ss > 0.0f ? __int_as_float((127 - e) << 23) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < NKT; ++i) *reinterpret_cast<h8*>(&dst[0][row][(quarter + 4 * i) * 8]) = r.x[i] * s;
+    } else {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NKT; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = (float)r.x[i][j];
+                m = fmaxf(m, fabsf(x));
+                ss = fmaf(x, x, ss);
+            }
+        ss = add_xor2(add_xor1(ss));
+        m = max_dpp<0x4e>(max_dpp<0xb1>(m));
+        const float s = scale_of(m, inv);
+        if (m == 0.0f) inv = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NKT; ++i) {
+            h8 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = (float)r.x[i][j];
+                hi[j] = (_Float16)(x * s);
+                if (KP == 2) lo[j] = (_Float16)fmaf(x, s, -(float)hi[j]);
+            }
+            const int c = (quarter + 4 * i) * 8;
+            *reinterpret_cast<h8*>(&dst[0][row][c]) = hi;
+            if (KP == 2) *reinterpret_cast<h8*>(&dst[KP - 1][row][c]) = lo;
         }
-        const int c = (quarter + 4 * i) * 8;
-        *reinterpret_cast<h8*>(&dst[0][row][c]) = hi;
-        if (KP == 2) *reinterpret_cast<h8*>(&dst[KP - 1][row][c]) = lo;
     }
     return inv;
 }
@@ -232,25 +274,26 @@ __device__ __forceinline__ f32x4 ld4(const float* p) { return *reinterpret_cast<
 // the row's), so it costs two multiplications an element; within a 16 it is an
 // exponential of the difference.  P's row scale comes from a bound (lengths of
 // q and k, the largest decay ratio), which an fp16's exponent has room for.
-template <class T, int NKT, int NB>
-__device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, int nt) {
-    using G = Geo<T, NKT, NB>;
+template <class T, int NKT>
+__device__ __forceinline__ void make_tp(const KQ<T, NKT>& X, TP<T>& Y, Make& M, TriA& A, int wave, int lane, int nt) {
+    constexpr int KP = KQ<T, NKT>::KP, KS = KQ<T, NKT>::KS;
+    Diag& D = *reinterpret_cast<Diag*>(Y.T_);
     const int l15 = lane & 15, g = lane >> 4;
     f32x4 acc[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (j <= wave) acc[j] = dot_tile<NKT, G::KP, G::KS>(L.K, L.K, wave, j, l15, g);
+        if (j <= wave) acc[j] = dot_tile<NKT, KP, KS>(X.K, X.K, wave, j, l15, g);
     {
         const int i = lane, s = i & ~15, e = i | 15;
-        const float h = L.gh[i], l = L.gl[i], kx = L.kx[i];
+        const float h = M.gh[i], l = M.gl[i], kx = M.kx[i];
         if (wave == 0) {
-            const float b = L.beta[i] * kx, r = exp2_fast((h - L.gh[s]) + (l - L.gl[s]));
-            L.ab[i] = b;
-            L.ar[i] = b * r;
-            L.kc[i] = exp2_fast((L.gh[e] - h) + (L.gl[e] - l)) * kx;
+            const float b = Y.beta[i] * kx, r = exp2_fast((h - M.gh[s]) + (l - M.gl[s]));
+            M.ab[i] = b;
+            M.ar[i] = b * r;
+            M.kc[i] = exp2_fast((M.gh[e] - h) + (M.gl[e] - l)) * kx;
         } else if (wave == 1) {
             // largest decay ratio of a row: e(G_i - min over j <= i of G_j); largest length of a key
-            float lo = h, kn = L.kn[i];
+            float lo = h, kn = M.kn[i];
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
                 const float y = __shfl_up(lo, d);
@@ -258,16 +301,18 @@ __device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, 
                 kn = fmaxf(kn, __shfl_xor(kn, d));
             }
             float inv;
-            const float qx = L.qx[i], sc = scale_of(L.qn[i] * kn * exp2_fast(fminf(h - lo, 120.0f)), inv);
-            L.pi[i] = inv;
-            L.pb[i] = qx * sc;
-            L.pr[i] = qx * sc * exp2_fast((h - L.gh[s]) + (l - L.gl[s]));
+            const float qx = M.qx[i], sc = scale_of(M.qn[i] * kn * exp2_fast(fminf(h - lo, 120.0f)), inv);
+            Y.pi[i] = inv;
+            M.pb[i] = qx * sc;
+            M.pr[i] = qx * sc * exp2_fast((h - M.gh[s]) + (l - M.gl[s]));
         } else if (wave == 2) {
             const float up = exp2_fast(h);
-            L.fx[i] = L.beta[i] * up * kx;
-            L.fq[i] = up * L.qx[i];
-            L.fk[i] = exp2_fast((L.gh[C - 1] - h) + (L.gl[C - 1] - l)) * kx;
-            if (i == C - 1) L.all = up;
+            Y.fx[i] = Y.beta[i] * up * kx;
+            Y.fq[i] = up * M.qx[i];
+            const float fk = exp2_fast((M.gh[C - 1] - h) + (M.gl[C - 1] - l)) * kx;
+            Y.fk[i] = fk;
+            const float m = wave_max(fk);
+            if (i == C - 1) Y.all = up, Y.fkmax = m;
         }
     }
     __syncthreads();
@@ -277,15 +322,15 @@ __device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, 
         const int col = 16 * j + l15, row = 16 * wave + 4 * g;
         f32x4 f;
         if (j == wave) {
-            const f32x4 h = ld4(&L.gh[row]), l = ld4(&L.gl[row]), b = ld4(&L.ab[row]);
-            const float hj = L.gh[col], lj = L.gl[col], kj = L.kx[col];
+            const f32x4 h = ld4(&M.gh[row]), l = ld4(&M.gl[row]), b = ld4(&M.ab[row]);
+            const float hj = M.gh[col], lj = M.gl[col], kj = M.kx[col];
 #pragma unroll
             for (int r = 0; r < 4; ++r) f[r] = exp2_fast(fminf((h[r] - hj) + (l[r] - lj), 120.0f)) * (b[r] * kj);
         } else {
-            const float k = L.kc[col] * exp2_fast(L.gh[16 * wave] - L.gh[16 * j + 15]);
-            f = ld4(&L.ar[row]) * k;
+            const float k = M.kc[col] * exp2_fast(M.gh[16 * wave] - M.gh[16 * j + 15]);
+            f = ld4(&M.ar[row]) * k;
         }
-        *reinterpret_cast<f32x4*>(&L.A[col][row]) = acc[j] * f;
+        *reinterpret_cast<f32x4*>(&A.A[col][row]) = acc[j] * f;
     }
     __syncthreads();
     if (wave == 0) {
@@ -298,33 +343,33 @@ __device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, 
         for (int j = 0; j < 15; ++j) {
 #pragma unroll
             for (int q = (j + 1) / 4; q < 4; ++q) {
-                const f32x4 a = ld4(&L.A[b + j][b + 4 * q]);
+                const f32x4 a = ld4(&A.A[b + j][b + 4 * q]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (4 * q + r > j) x[4 * q + r] = fmaf(-a[r], x[j], x[4 * q + r]);
             }
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&L.D[g][l15][4 * q]) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&D.D[g][l15][4 * q]) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
     } else {
         // P meanwhile: rows of tile 3, 2, and 1 with 0; as K Q^T, so that a lane has 4 frames of a row
         const int first = wave == 1 ? 3 : wave == 2 ? 2 : 0, last = wave == 3 ? 1 : first;
         for (int mi = first; mi <= last && mi < nt; ++mi) {
             const int row = 16 * mi + l15;
-            const float pb = L.pb[row], pr = L.pr[row], hi_ = L.gh[row], li = L.gl[row], hs = L.gh[16 * mi];
+            const float pb = M.pb[row], pr = M.pr[row], hi_ = M.gh[row], li = M.gl[row], hs = M.gh[16 * mi];
             for (int j = 0; j <= (mi | 1); ++j) {
                 h4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
                 if (j <= mi) {
-                    const f32x4 p = dot_tile<NKT, G::KP, G::KS>(L.K, L.Q, j, mi, l15, g);
+                    const f32x4 p = dot_tile<NKT, KP, KS>(X.K, X.Q, j, mi, l15, g);
                     const int col = 16 * j + 4 * g;
                     f32x4 f;
                     if (j == mi) {
-                        const f32x4 h = ld4(&L.gh[col]), l = ld4(&L.gl[col]), k = ld4(&L.kx[col]);
+                        const f32x4 h = ld4(&M.gh[col]), l = ld4(&M.gl[col]), k = ld4(&M.kx[col]);
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             f[r] = col + r <= row ? exp2_fast(fminf((hi_ - h[r]) + (li - l[r]), 120.0f)) * (k[r] * pb) : 0.0f;
                     } else {
-                        f = ld4(&L.kc[col]) * (pr * exp2_fast(hs - L.gh[16 * j + 15]));
+                        f = ld4(&M.kc[col]) * (pr * exp2_fast(hs - M.gh[16 * j + 15]));
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
@@ -333,8 +378,8 @@ __device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, 
                         b[r] = (_Float16)(x - (float)a[r]);
                     }
                 }
-                L.P_[0].put(mi, l15, j, g, a);
-                if (G::OP == 2) L.P_[G::OP - 1].put(mi, l15, j, g, b);
+                Y.P_[0].put(mi, l15, j, g, a);
+                if (TP<T>::OP == 2) Y.P_[TP<T>::OP - 1].put(mi, l15, j, g, b);
             }
         }
     }
@@ -348,17 +393,17 @@ __device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, 
         if (j > wave || wave >= nt) continue;
         if (j == wave) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t[j][r] = L.D[j][4 * g + r][l15];
+            for (int r = 0; r < 4; ++r) t[j][r] = D.D[j][4 * g + r][l15];
         } else {
             f32x4 y = {0, 0, 0, 0};
 #pragma unroll
             for (int k = j + 1; k < 4; ++k) {
                 if (k > wave) continue;
-                const f32x4 a = ld4(&L.A[16 * j + l15][16 * k + 4 * g]);
+                const f32x4 a = ld4(&A.A[16 * j + l15][16 * k + 4 * g]);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], t[k][r], y, 0, 0, 0);
             }
-            const f32x4 d = ld4(&L.D[j][l15][4 * g]);
+            const f32x4 d = ld4(&D.D[j][l15][4 * g]);
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(-d[r], y[r], t[j], 0, 0, 0);
         }
@@ -367,8 +412,8 @@ __device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, 
     __syncthreads();
     if (wave < nt) {
         float inv;
-        const float s = scale_of(max_xor16_32(max_row16(m)), inv);
-        if (lane == 0) L.ti[wave] = inv;
+        const float s = scale_of(wave_max(m), inv);
+        if (lane == 0) Y.ti[wave] = inv;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j > (wave | 1)) continue;
@@ -378,59 +423,62 @@ __device__ __forceinline__ void make_tp(Lds<T, NKT, NB>& L, int wave, int lane, 
                 a[r] = (_Float16)(t[j][r] * s);
                 b[r] = (_Float16)fmaf(t[j][r], s, -(float)a[r]);
             }
-            L.T_[0].put(wave, l15, j, g, a);
-            L.T_[1].put(wave, l15, j, g, b);
+            Y.T_[0].put(wave, l15, j, g, a);
+            Y.T_[1].put(wave, l15, j, g, b);
         }
     }
     __syncthreads();
 }
 
 // The products with the state for one chunk of nt live tiles of 16 frames: this
-// wave's columns.  S holds the state times 1 / sinv (a power of two per column);
-// between() runs once the state's 16-bit parts are dead (it holds the next
-// chunk's loads).
+// wave's columns.  S holds the state times 1 / sinv, a power of two; between()
+// runs once the state's 16-bit parts are dead (it holds the next chunk's loads).
 template <class T, int NKT, int NB, class F>
-__device__ __forceinline__ void advance(Lds<T, NKT, NB>& L, f32x4 (&S)[2 * NKT][NB], float (&sinv)[NB], int wave, int lane,
-                                        int nt, const F& between) {
+__device__ __forceinline__ void advance(const KQ<T, NKT>& X, const TP<T>& Y, T (*V)[Geo<T, NKT, NB>::VS],
+                                        f32x4 (&S)[2 * NKT][NB], float& sinv, int lane, int nt, const F& between) {
     using G = Geo<T, NKT, NB>;
+    constexpr bool LOW = G::OP == 2;
     const int l15 = lane & 15, g = lane >> 4;
+    const f32x4 zero = {0, 0, 0, 0};
     f32x4 R[4][NB], O[4][NB];
-    float smax[NB];
+    float smax = 0.0f, rmax = 0.0f;
     {
         h8 hi[NKT][NB], lo[NKT][NB];
-        float inv[NB];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            float m = 0.0f;
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int t = 0; t < 2 * NKT; ++t) m = amax4(m, S[t][n]);
-            smax[n] = max_xor16_32(m);
-            const float s = scale_of(smax[n], inv[n]);
-            inv[n] *= sinv[n];
+            for (int t = 0; t < 2 * NKT; ++t) smax = amax4(smax, S[t][n]);
+        smax = wave_max(smax);
+        float inv;
+        const float s = scale_of(smax, inv);
+        inv *= sinv;
 #pragma unroll
-            for (int t = 0; t < NKT; ++t) split(S[2 * t][n], S[2 * t + 1][n], s, hi[t][n], lo[t][n]);
-        }
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int t = 0; t < NKT; ++t) split<true>(S[2 * t][n], S[2 * t + 1][n], all4(s), all4(s), hi[t][n], lo[t][n]);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            f32x4 x[NB], o[NB];
+            if (m >= nt) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) R[m][n] = O[m][n] = x[n] = o[n] = f32x4{0, 0, 0, 0};
-            if (m >= nt) continue;
+                for (int n = 0; n < NB; ++n) R[m][n] = zero;
+                continue;
+            }
             no_hoist();
+            f32x4 x[NB], o[NB];
 #pragma unroll
             for (int s = 0; s < NKT; ++s) {
                 const int c = 32 * s + 8 * g;
-                const h8 k = *reinterpret_cast<const h8*>(&L.K[0][16 * m + l15][c]);
-                const h8 q = *reinterpret_cast<const h8*>(&L.Q[0][16 * m + l15][c]);
+                const h8 k = *reinterpret_cast<const h8*>(&X.K[0][16 * m + l15][c]);
+                const h8 q = *reinterpret_cast<const h8*>(&X.Q[0][16 * m + l15][c]);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    x[n] = mma(k, lo[s][n], mma(k, hi[s][n], x[n]));
-                    o[n] = mma(q, hi[s][n], o[n]);
-                    if (G::OP == 2) o[n] = mma(q, lo[s][n], o[n]);
+                    x[n] = mma(k, lo[s][n], mma(k, hi[s][n], s ? x[n] : zero));
+                    o[n] = mma(q, hi[s][n], s ? o[n] : zero);
+                    if (LOW) o[n] = mma(q, lo[s][n], o[n]);
                 }
                 if (G::KP == 2) {
-                    const h8 kl = *reinterpret_cast<const h8*>(&L.K[G::KP - 1][16 * m + l15][c]);
-                    const h8 ql = *reinterpret_cast<const h8*>(&L.Q[G::KP - 1][16 * m + l15][c]);
+                    const h8 kl = *reinterpret_cast<const h8*>(&X.K[G::KP - 1][16 * m + l15][c]);
+                    const h8 ql = *reinterpret_cast<const h8*>(&X.Q[G::KP - 1][16 * m + l15][c]);
 #pragma unroll
                     for (int n = 0; n < NB; ++n) {
                         x[n] = mma(kl, hi[s][n], x[n]);
@@ -438,122 +486,113 @@ __device__ __forceinline__ void advance(Lds<T, NKT, NB>& L, f32x4 (&S)[2 * NKT][
                     }
                 }
             }
-            const f32x4 b = ld4(&L.beta[16 * m + 4 * g]), fx = ld4(&L.fx[16 * m + 4 * g]), fq = ld4(&L.fq[16 * m + 4 * g]);
+            const f32x4 b = ld4(&Y.beta[16 * m + 4 * g]);
+            const f32x4 fx = ld4(&Y.fx[16 * m + 4 * g]) * -inv, fq = ld4(&Y.fq[16 * m + 4 * g]) * inv;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                float v[4];
+                f32x4 v;
                 if constexpr (G::WIDE) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = L.V[wave][16 * m + 4 * g + r][16 * n + l15];
+                    for (int r = 0; r < 4; ++r) v[r] = V[16 * m + 4 * g + r][16 * n + l15];
                 } else {
                     const auto t = __builtin_bit_cast(typename Vec<T, 4>::raw,
-                                                      read_tr(&L.V[wave][16 * m + 4 * g + (l15 >> 2)][16 * n + 4 * (l15 & 3)]));
+                                                      read_tr(&V[16 * m + 4 * g + (l15 >> 2)][16 * n + 4 * (l15 & 3)]));
 #pragma unroll
                     for (int r = 0; r < 4; ++r) v[r] = (float)t[r];
                 }
+                v *= b;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    R[m][n][r] = fmaf(-fx[r] * inv[n], x[n][r], b[r] * v[r]);
-                    O[m][n][r] = fq[r] * inv[n] * o[n][r];
-                }
+                for (int r = 0; r < 4; ++r) R[m][n][r] = fmaf(fx[r], x[n][r], v[r]);
+                O[m][n] = o[n] * fq;
+                rmax = amax4(rmax, R[m][n]);
             }
         }
     }
     between();
-    f32x4 U[4][NB];
+    // U = u ti rinv, where |u| is at most 64 products of 2^30
+    f32x4 u[4][NB];
+    float rinv, ti[4], tmax = 0.0f;
     {
         h8 hi[2][NB], lo[2][NB];
-        float inv[NB];
+        const float s = scale_of(wave_max(rmax), rinv);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            float m = 0.0f;
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) m = amax4(m, R[t][n]);
-            const float s = scale_of(max_xor16_32(m), inv[n]);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) split(R[2 * t][n], R[2 * t + 1][n], s, hi[t][n], lo[t][n]);
-        }
+            for (int t = 0; t < 2; ++t) split<true>(R[2 * t][n], R[2 * t + 1][n], all4(s), all4(s), hi[t][n], lo[t][n]);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            f32x4 u[NB];
+            ti[m] = 0.0f;
+            if (m >= nt) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) U[m][n] = u[n] = f32x4{0, 0, 0, 0};
-            if (m >= nt) continue;
+                for (int n = 0; n < NB; ++n) u[m][n] = zero;
+                continue;
+            }
             no_hoist();
+            ti[m] = Y.ti[m];
+            tmax = fmaxf(tmax, ti[m]);
 #pragma unroll
             for (int s = 0; s <= m / 2; ++s) {
-                const h8 th = L.T_[0].operand(m, l15, s, g), tl = L.T_[1].operand(m, l15, s, g);
+                const h8 th = Y.T_[0].operand(m, l15, s, g), tl = Y.T_[1].operand(m, l15, s, g);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) u[n] = mma(tl, hi[s][n], mma(th, lo[s][n], mma(th, hi[s][n], u[n])));
+                for (int n = 0; n < NB; ++n) u[m][n] = mma(tl, hi[s][n], mma(th, lo[s][n], mma(th, hi[s][n], s ? u[m][n] : zero)));
             }
-#pragma unroll
-            for (int n = 0; n < NB; ++n) U[m][n] = u[n] * (L.ti[m] * inv[n]);
         }
     }
+    // to below 2^14: U = (u ti c) rinv / c
+    const float cinv = tmax * 0x1p22f, c = 1.0f / cinv;
     // O += P U
     {
         h8 hi[2][NB], lo[2][NB];
-        float inv[NB];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            float m = 0.0f;
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) m = amax4(m, U[t][n]);
-            const float s = scale_of(max_xor16_32(m), inv[n]);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if (G::OP == 2) split(U[2 * t][n], U[2 * t + 1][n], s, hi[t][n], lo[t][n]);
-                else hi[t][n] = high(U[2 * t][n], U[2 * t + 1][n], s);
-            }
-        }
+            for (int t = 0; t < 2; ++t)
+                split<LOW>(u[2 * t][n], u[2 * t + 1][n], all4(ti[2 * t] * c), all4(ti[2 * t + 1] * c), hi[t][n], lo[t][n]);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             if (m >= nt) continue;
             no_hoist();
             f32x4 o[NB];
 #pragma unroll
-            for (int n = 0; n < NB; ++n) o[n] = f32x4{0, 0, 0, 0};
-#pragma unroll
             for (int s = 0; s <= m / 2; ++s) {
-                const h8 ph = L.P_[0].operand(m, l15, s, g);
+                const h8 ph = Y.P_[0].operand(m, l15, s, g);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) o[n] = mma(ph, hi[s][n], o[n]);
-                if (G::OP == 2) {
-                    const h8 pl = L.P_[G::OP - 1].operand(m, l15, s, g);
+                for (int n = 0; n < NB; ++n) o[n] = mma(ph, hi[s][n], s ? o[n] : zero);
+                if (LOW) {
+                    const h8 pl = Y.P_[G::OP - 1].operand(m, l15, s, g);
 #pragma unroll
                     for (int n = 0; n < NB; ++n) o[n] = mma(pl, hi[s][n], mma(ph, lo[s][n], o[n]));
                 }
             }
-            const f32x4 pi = ld4(&L.pi[16 * m + 4 * g]);
+            const f32x4 pi = ld4(&Y.pi[16 * m + 4 * g]) * (rinv * cinv);
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    L.V[wave][16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r] * inv[n], O[m][n][r]);
+                    V[16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], O[m][n][r]);
         }
     }
-    // S1, accumulated onto the decayed state in U's scale; where U is next to nothing, in 2^13 of the decayed state's
-    // own, so that neither leaves its range (2^100 at most: the state's factor f stays finite)
+    // S1, accumulated onto the decayed state in the scale s of U fk; where U is next to nothing, in 2^13 of the decayed
+    // state's own, so that neither leaves its range (2^100 at most: the state's factor stays finite)
     {
         h8 hi[2][NB], lo[2][NB];
-        const float all = L.all;
+        const float all = Y.all;
+        float zi, li;
+        const float z = scale_of(Y.fkmax, zi) * 0x1p-14f, low = scale_of(fmaxf(smax * sinv * (all * 0x1p-13f), 0x1p-86f), li);
+        const float s = fminf(c * z / rinv, low), k = s * rinv;  // true U fk times s = u ti fk k
+        f32x4 f[4];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            float m = 0.0f;
+        for (int t = 0; t < 4; ++t) f[t] = ld4(&Y.fk[16 * t + 4 * g]) * (ti[t] * k);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                U[t][n] *= ld4(&L.fk[16 * t + 4 * g]);
-                m = amax4(m, U[t][n]);
-            }
-            float inv;
-            const float s = scale_of(fmaxf(fmaxf(max_xor16_32(m), smax[n] * sinv[n] * (all * 0x1p-13f)), 0x1p-86f), inv);
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) split(U[2 * t][n], U[2 * t + 1][n], s, hi[t][n], lo[t][n]);
-            const float f = all * s * sinv[n];
+            for (int t = 0; t < 2; ++t) split<true>(u[2 * t][n], u[2 * t + 1][n], f[2 * t], f[2 * t + 1], hi[t][n], lo[t][n]);
+        const float d = all * s * sinv;
+        sinv = 1.0f / s;
 #pragma unroll
-            for (int t = 0; t < 2 * NKT; ++t) S[t][n] *= f;
-            sinv[n] = inv;
-        }
+        for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int t = 0; t < 2 * NKT; ++t) S[t][n] *= d;
 #pragma unroll
         for (int t = 0; t < 2 * NKT; ++t) {
             if (t & 1) no_hoist();
@@ -562,7 +601,7 @@ __device__ __forceinline__ void advance(Lds<T, NKT, NB>& L, f32x4 (&S)[2 * NKT][
                 if (2 * s >= nt) continue;
                 const int row = 32 * s + 4 * g + (l15 >> 2), col = 32 * (t >> 1) + 8 * (l15 & 3) + 4 * (t & 1);
                 const auto kt = [&](int part) {
-                    const s4 a = read_tr(&L.K[part][row][col]), b = read_tr(&L.K[part][row + 16][col]);
+                    const s4 a = read_tr(&X.K[part][row][col]), b = read_tr(&X.K[part][row + 16][col]);
                     const h4 x = __builtin_bit_cast(h4, a), y = __builtin_bit_cast(h4, b);
                     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
                 };
@@ -579,106 +618,69 @@ __device__ __forceinline__ void advance(Lds<T, NKT, NB>& L, f32x4 (&S)[2 * NKT][
     }
 }
 
-// v of this wave's columns (and out, the other way): 2 NB lanes a row, 8 columns each
-template <class T, int NB>
-struct RawV {
-    static constexpr int LPR = 2 * NB, ROWS = 64 / LPR, N = C / ROWS;
-    typename Vec<T, 8>::raw x[N];
-};
+// f(t, j, r, at, in) for element r of accumulator tile (t, j): its place in the
+// head's state, kept inside it, and whether it is one of it
+template <int NKT, int NB, class F>
+__device__ __forceinline__ void each_state(const nnsp_delta_args& a, int c0, int lane, const F& f) {
+    const int l15 = lane & 15, g = lane >> 4;
+    const bool whole = a.dk == 32 * NKT && c0 + 16 * NB <= a.dv;
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < 2 * NKT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = 32 * (t >> 1) + 4 * (t & 1) + r, col = c0 + 16 * j;  // of lane 0
+                if (whole) f(t, j, r, row * a.dv + col + (8 * g * a.dv + l15), true);
+                else f(t, j, r, min(row + 8 * g, a.dk - 1) * a.dv + min(col + l15, a.dv - 1), row + 8 * g < a.dk && col + l15 < a.dv);
+            }
+}
 
-// FAST: dk and dv are multiples of 8
-template <class T, int NKT, int NB, bool FAST>
-__global__ __launch_bounds__(256, 2) void delta_chunk_kernel(const nnsp_delta_args a) {
-    using G = Geo<T, NKT, NB>;
-    __shared__ Lds<T, NKT, NB> L;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l15 = lane & 15, g = lane >> 4;
-    const int ncb = (a.dv + G::W - 1) / G::W;
-    const int cb = blockIdx.x % ncb, h = (blockIdx.x / ncb) % a.value_heads, s = blockIdx.x / ncb / a.value_heads;
-    const int hk = h / (a.value_heads / a.key_heads);
-    const int n = a.lens ? max(0, min(a.lens[s], a.n_frames)) : a.n_frames;
-    const int c0 = cb * G::W + wave * 16 * NB;  // first column of this wave
-    const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
-
-    f32x4 S[2 * NKT][NB];
-    float sinv[NB];
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-        sinv[j] = 1.0f;
-#pragma unroll
-        for (int t = 0; t < 2 * NKT; ++t) S[t][j] = f32x4{0, 0, 0, 0};
-    }
-    if (a.state_in) {
-        const float* p = a.state_in + so;
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int t = 0; t < 2 * NKT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 32 * (t >> 1) + 8 * g + 4 * (t & 1) + r, col = c0 + 16 * j + l15;
-                    const float x = p[min(row, a.dk - 1) * a.dv + min(col, a.dv - 1)];
-                    S[t][j][r] = row < a.dk && col < a.dv ? x : 0.0f;
-                }
-    }
-
-    using RV = RawV<T, NB>;
-    const int row = tid >> 2, quarter = tid & 3;
-    const int vrow = lane / RV::LPR, vcol = c0 + (lane % RV::LPR) * 8;
-    // this thread's places, moved on by a chunk each time
-    const T* qp = (const T*)a.q + s * a.q_stride[0] + hk * a.q_stride[2] + row * a.q_stride[1] + quarter * 8;
-    const T* kp = (const T*)a.k + s * a.k_stride[0] + hk * a.k_stride[2] + row * a.k_stride[1] + quarter * 8;
-    const T* vp = (const T*)a.v + s * a.v_stride[0] + h * a.v_stride[2] + vrow * a.v_stride[1] + vcol;
-    T* op = (T*)a.out + s * a.out_stride[0] + h * a.out_stride[2] + vrow * a.out_stride[1] + vcol;
-    const float* gp = a.g ? a.g + s * a.g_stride[0] + h * a.g_stride[2] + lane * a.g_stride[1] : nullptr;
-    const float* bp = a.beta + s * a.beta_stride[0] + h * a.beta_stride[2] + lane * a.beta_stride[1];
-    const long long qs = C * a.q_stride[1], ks = C * a.k_stride[1], vs = RV::ROWS * a.v_stride[1], os = RV::ROWS * a.out_stride[1];
-    const long long gs = C * a.g_stride[1], bs = C * a.beta_stride[1];
-    const int vleft = a.dv - vcol;
-
+// A chunk's rows of q, k, g and beta of one stream and head: from global memory to
+// registers, from there to LDS with what make_tp starts from.
+template <class T, int NKT, bool FAST>
+struct Rows {
+    const T *qp, *kp;
+    const float *gp, *bp;
+    long long qs, ks, gs, bs;
     RawRows<T, NKT> rq, rk;
-    RV rv;
-    float rg = 0.0f, rb = 0.0f;
-    const auto fetch = [&](int t0) {
-        const bool live = t0 + row < n;
-        fetch_rows<T, NKT, FAST>(rk, kp, quarter, a.dk, live);
-        fetch_rows<T, NKT, FAST>(rq, qp, quarter, a.dk, live);
-        kp += ks;
-        qp += qs;
-#pragma unroll
-        for (int i = 0; i < RV::N; ++i) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) rv.x[i][j] = (T)0.0f;
-            const int left = t0 + vrow + RV::ROWS * i < n ? vleft : 0;
-            if (FAST) {
-                if (left > 0) rv.x[i] = *reinterpret_cast<const typename Vec<T, 8>::type*>(vp);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (j < left) rv.x[i][j] = vp[j];
-            }
-            vp += vs;
+    float rg, rb;
+    int row, quarter, lane, wave;
+
+    // this thread's place in the chunk at frame t0
+    __device__ __forceinline__ Rows(const nnsp_delta_args& a, int s, int h, long long t0, int tid, int wv)
+        : row(tid >> 2), quarter(tid & 3), lane(tid & 63), wave(wv) {
+        const int hk = h / (a.value_heads / a.key_heads);
+        qp = (const T*)a.q + s * a.q_stride[0] + hk * a.q_stride[2] + (t0 + row) * a.q_stride[1] + quarter * 8;
+        kp = (const T*)a.k + s * a.k_stride[0] + hk * a.k_stride[2] + (t0 + row) * a.k_stride[1] + quarter * 8;
+        gp = a.g ? a.g + s * a.g_stride[0] + h * a.g_stride[2] + (t0 + lane) * a.g_stride[1] : nullptr;
+        bp = a.beta + s * a.beta_stride[0] + h * a.beta_stride[2] + (t0 + lane) * a.beta_stride[1];
+        qs = C * a.q_stride[1], ks = C * a.k_stride[1], gs = C * a.g_stride[1], bs = C * a.beta_stride[1];
+    }
+    // left: live frames from the chunk's first on
+    __device__ __forceinline__ void fetch(int dk, int left) {
+        fetch_rows<T, NKT, FAST>(rk, kp, quarter, dk, row < left);
+        fetch_rows<T, NKT, FAST>(rq, qp, quarter, dk, row < left);
+        rg = rb = 0.0f;
+        if (wave == 0 && lane < left) {
+            if (gp) rg = *gp;
+            rb = *bp;
         }
-        if (wave == 0) {
-            rg = rb = 0.0f;
-            if (t0 + lane < n) {
-                if (gp) rg = *gp;
-                rb = *bp;
-            }
-            if (gp) gp += gs;
-            bp += bs;
-        }
-    };
-    if (n > 0) fetch(0);
-    for (int t0 = 0; t0 < n; t0 += C) {
-        const int nt = min(4, (n - t0 + 15) >> 4);
-        float ss;
-        float inv = stage_rows<T, NKT, G::KP, G::KS>(rk, L.K, row, quarter, ss), len = 1.0f, f = 1.0f;
+    }
+    __device__ __forceinline__ void next() {
+        qp += qs, kp += ks, bp += bs;
+        if (gp) gp += gs;
+    }
+    __device__ __forceinline__ void stage(const nnsp_delta_args& a, KQ<T, NKT>& X, TP<T>& Y, Make& M) {
+        constexpr int KP = KQ<T, NKT>::KP, KS = KQ<T, NKT>::KS;
+        float ss, inv, f;
+        // a row of zeros has inv 0 and no part in anything, whatever its norm's reciprocal is
+        inv = stage_rows<T, NKT, KP, KS>(rk, X.K, row, quarter, ss);
         f = a.l2norm ? 1.0f / sqrtf(ss + a.eps) : 1.0f;
-        len = sqrtf(ss) * f;
-        if (quarter == 0) L.kx[row] = inv * f, L.kn[row] = len;
-        inv = stage_rows<T, NKT, G::KP, G::KS>(rq, L.Q, row, quarter, ss);
+        if (quarter == 0) M.kx[row] = inv > 0.0f ? inv * f : 0.0f, M.kn[row] = inv > 0.0f ? sqrtf(ss) * f : 0.0f;
+        inv = stage_rows<T, NKT, KP, KS>(rq, X.Q, row, quarter, ss);
         f = a.scale * (a.l2norm ? 1.0f / sqrtf(ss + a.eps) : 1.0f);
-        if (quarter == 0) L.qx[row] = inv * f, L.qn[row] = sqrtf(ss) * fabsf(f);
+        if (quarter == 0) M.qx[row] = inv > 0.0f ? inv * f : 0.0f, M.qn[row] = inv > 0.0f ? sqrtf(ss) * fabsf(f) : 0.0f;
         if (wave == 0) {
             // running sum of g in 64 bits, in units of log2, kept as two floats: differences of near frames stay exact
             double x = (double)decay_log(rg) * 1.4426950408889634;
@@ -687,75 +689,307 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(const nnsp_delta_ar
                 const double y = __shfl_up(x, d);
                 if (lane >= d) x += y;
             }
-            L.gh[lane] = (float)x;
-            L.gl[lane] = (float)(x - (double)(float)x);
-            L.beta[lane] = rb;
+            M.gh[lane] = (float)x;
+            M.gl[lane] = (float)(x - (double)(float)x);
+            Y.beta[lane] = rb;
         }
-        __syncthreads();
-        make_tp<T, NKT, NB>(L, wave, here(lane), nt);
+    }
+};
+
+// The same for a wave's columns of v, and for out the other way.
+template <class T, int NKT, int NB, bool FAST>
+struct Cols {
+    static constexpr int LPR = 2 * NB, ROWS = 64 / LPR, N = C / ROWS, VS = Geo<T, NKT, NB>::VS;
+    typedef typename Vec<T, 8>::raw V8;
+    typedef typename Vec<T, 8>::type V8u;
+    const T* vp;
+    T* op;
+    long long vs, os;
+    int row, col, left;  // left: columns from this lane's first on
+    V8 x[N];
+
+    __device__ __forceinline__ Cols(const nnsp_delta_args& a, int s, int h, long long t0, int c0, int lane)
+        : row(lane / LPR), col((lane % LPR) * 8), left(a.dv - c0 - (lane % LPR) * 8) {
+        vp = (const T*)a.v + s * a.v_stride[0] + h * a.v_stride[2] + (t0 + row) * a.v_stride[1] + c0 + col;
+        op = (T*)a.out + s * a.out_stride[0] + h * a.out_stride[2] + (t0 + row) * a.out_stride[1] + c0 + col;
+        vs = ROWS * a.v_stride[1], os = ROWS * a.out_stride[1];
+    }
+    // frames: live frames from the chunk's first on
+    __device__ __forceinline__ void fetch(int frames) {
 #pragma unroll
-        for (int i = 0; i < RV::N; ++i)
-            *reinterpret_cast<typename Vec<T, 8>::raw*>(&L.V[wave][vrow + RV::ROWS * i][vcol - c0]) = rv.x[i];
-        // the wave's own columns: LDS keeps its order within a wave, the compiler has to
-        asm volatile("" ::: "memory");
-        advance<T, NKT, NB>(L, S, sinv, wave, here(lane), nt, [&] {
-            if (t0 + C < n) fetch(t0 + C);
-        });
-        asm volatile("" ::: "memory");
+        for (int i = 0; i < N; ++i) {
 #pragma unroll
-        for (int i = 0; i < RV::N; ++i) {
-            const int r = vrow + RV::ROWS * i, left = t0 + r < n ? vleft : 0;
-            const auto x = *reinterpret_cast<const typename Vec<T, 8>::raw*>(&L.V[wave][r][vcol - c0]);
+            for (int j = 0; j < 8; ++j) x[i][j] = (T)0.0f;
+            const bool live = row + ROWS * i < frames;
             if (FAST) {
-                if (left > 0) *reinterpret_cast<typename Vec<T, 8>::type*>(op) = x;
+                if (live && left > 0) x[i] = *reinterpret_cast<const V8u*>(vp);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (j < left) op[j] = x[j];
+                    if (live && j < left) x[i][j] = vp[j];
+            }
+            vp += vs;
+        }
+    }
+    __device__ __forceinline__ void stage(T (*V)[VS]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) *reinterpret_cast<V8*>(&V[row + ROWS * i][col]) = x[i];
+        // the wave's own columns: LDS keeps its order within a wave, the compiler has to
+        asm volatile("" ::: "memory");
+    }
+    __device__ __forceinline__ void store(T (*V)[VS], int frames) {
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool live = row + ROWS * i < frames;
+            const V8 y = *reinterpret_cast<const V8*>(&V[row + ROWS * i][col]);
+            if (FAST) {
+                if (live && left > 0) *reinterpret_cast<V8u*>(op) = y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (live && j < left) op[j] = y[j];
             }
             op += os;
         }
-        __syncthreads();
     }
-    if (a.state_out) {
-        const int l = here(lane);
-        float* p = a.state_out + so;
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-#pragma unroll
-            for (int t = 0; t < 2 * NKT; ++t)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int rw = 32 * (t >> 1) + 8 * (l >> 4) + 4 * (t & 1) + r, col = c0 + 16 * j + (l & 15);
-                    if (rw < a.dk && col < a.dv) p[rw * a.dv + col] = S[t][j][r] * sinv[j];
-                }
-    }
+};
+
+__device__ __forceinline__ int frames_of(const nnsp_delta_args& a, int s) {
+    return a.lens ? max(0, min(a.lens[s], a.n_frames)) : a.n_frames;
 }
 
+// Many streams: a workgroup per stream, head and 64 NB columns goes through its
+// chunks alone, and the workgroups of a CU fill each other's waits.
+// FAST: dk and dv are multiples of 8.
 template <class T, int NKT, int NB, bool FAST>
-void launch_as(const nnsp_delta_args& a, hipStream_t st) {
+__global__ __launch_bounds__(256, 2) void delta_chunk_kernel(const nnsp_delta_args a) {
+    using G = Geo<T, NKT, NB>;
+    struct Lds {
+        KQ<T, NKT> X;
+        TP<T> Y;
+        Make M;
+        union {
+            TriA A;                        // until T is done
+            alignas(16) T V[4][C][G::VS];  // from then on: each wave's columns of v, then of out
+        };
+    };
+    __shared__ Lds L;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int ncb = (a.dv + G::W - 1) / G::W;
+    const int cb = blockIdx.x % ncb, h = (blockIdx.x / ncb) % a.value_heads, s = blockIdx.x / ncb / a.value_heads;
+    const int n = frames_of(a, s);
+    const int c0 = cb * G::W + wave * 16 * NB;  // first column of this wave
+    const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
+
+    f32x4 S[2 * NKT][NB];
+    float sinv = 1.0f;
+    each_state<NKT, NB>(a, c0, lane, [&](int t, int j, int r, int at, bool in) {
+        const float x = a.state_in ? (a.state_in + so)[at] : 0.0f;
+        S[t][j][r] = in ? x : 0.0f;
+    });
+    Rows<T, NKT, FAST> rows(a, s, h, 0, tid, wave);
+    Cols<T, NKT, NB, FAST> cols(a, s, h, 0, c0, lane);
+    if (n > 0) {
+        rows.fetch(a.dk, n);
+        cols.fetch(n);
+    }
+    for (int t0 = 0; t0 < n; t0 += C) {
+        const int left = n - t0, nt = min(4, (left + 15) >> 4);
+        rows.stage(a, L.X, L.Y, L.M);
+        __syncthreads();
+        make_tp<T, NKT>(L.X, L.Y, L.M, L.A, wave, here(lane), nt);
+        cols.stage(L.V[wave]);
+        advance<T, NKT, NB>(L.X, L.Y, L.V[wave], S, sinv, here(lane), nt, [&] {
+            if (left <= C) return;
+            rows.next();
+            rows.fetch(a.dk, left - C);
+            cols.fetch(left - C);
+        });
+        cols.store(L.V[wave], left);
+        __syncthreads();
+    }
+    if (a.state_out)
+        each_state<NKT, NB>(a, c0, here(lane), [&](int t, int j, int r, int at, bool in) {
+            if (in) (a.state_out + so)[at] = S[t][j][r] * sinv;
+        });
+}
+
+// Few streams, many frames: T and P of all chunks at once, one workgroup each
+// (prepare), then a short chain through the chunks (scan).  A slab of chunks
+// goes through both before the next, so that its images are read while the
+// caches still have them.
+struct Slab {
+    char *kq, *tp;          // images: [stream][key head][chunk of the slab], [stream][value head][chunk]
+    int first, chunks;      // the slab's first chunk and its number of chunks
+    const float* state_in;  // the chain's state before and after (NULL: zeros, dropped)
+    float* state_out;
+};
+
+template <class X>
+__device__ __forceinline__ void copy_out(char* dst, const X& src, int tid) {
+    static_assert(sizeof(X) % 16 == 0, "whole 16-byte pieces");
+    for (int i = tid; i < (int)(sizeof(X) / 16); i += 256)
+        reinterpret_cast<f32x4*>(dst)[i] = reinterpret_cast<const f32x4*>(&src)[i];
+}
+
+template <class T, int NKT, bool FAST>
+__global__ __launch_bounds__(256) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
+    struct Lds {
+        KQ<T, NKT> X;
+        TP<T> Y;
+        Make M;
+        TriA A;
+    };
+    __shared__ Lds L;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = blockIdx.x % b.chunks, h = (blockIdx.x / b.chunks) % a.value_heads, s = blockIdx.x / b.chunks / a.value_heads;
+    const int rep = a.value_heads / a.key_heads;
+    const int t0 = (b.first + c) * C, left = frames_of(a, s) - t0, nt = min(4, (left + 15) >> 4);
+    if (left <= 0) return;
+    Rows<T, NKT, FAST> rows(a, s, h, t0, tid, wave);
+    rows.fetch(a.dk, left);
+    rows.stage(a, L.X, L.Y, L.M);
+    __syncthreads();
+    if (h % rep == 0) copy_out(b.kq + (((long long)s * a.key_heads + h / rep) * b.chunks + c) * sizeof(KQ<T, NKT>), L.X, tid);
+    make_tp<T, NKT>(L.X, L.Y, L.M, L.A, wave, lane, nt);
+    copy_out(b.tp + (((long long)s * a.value_heads + h) * b.chunks + c) * sizeof(TP<T>), L.Y, tid);
+}
+
+// an image into LDS, past the registers: waves `wave` of `waves`, 1 KB an instruction
+template <class X>
+__device__ __forceinline__ void copy_in(X& dst, const char* src, int wave, int waves, int lane) {
+    constexpr int N = sizeof(X) / 16;
+    for (int i = wave * 64; i < N; i += waves * 64)
+        if (i + lane < N)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (long long)(i + lane) * 16),
+                                             (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(&dst) + i * 16), 16, 0, 0);
+}
+
+// Waves 0 .. 3 take the columns through the chunks, waves 4 .. 7 bring the next
+// chunk's images (BUFS 2; where LDS has room for one only, all wait for it).
+template <class T, int NKT, int NB, bool FAST, int BUFS>
+__global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a, const Slab b) {
+    using G = Geo<T, NKT, NB>;
+    struct Lds {
+        KQ<T, NKT> X[BUFS];
+        TP<T> Y[BUFS];
+        alignas(16) T V[4][C][G::VS];
+    };
+    __shared__ Lds L;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ncb = (a.dv + G::W - 1) / G::W;
+    const int cb = blockIdx.x % ncb, h = (blockIdx.x / ncb) % a.value_heads, s = blockIdx.x / ncb / a.value_heads;
+    const int hk = h / (a.value_heads / a.key_heads);
+    const int n = min(frames_of(a, s) - b.first * C, b.chunks * C);  // frames in this slab
+    if (wave >= 4) {
+        const char* kq = b.kq + ((long long)s * a.key_heads + hk) * b.chunks * sizeof(KQ<T, NKT>);
+        const char* tp = b.tp + ((long long)s * a.value_heads + h) * b.chunks * sizeof(TP<T>);
+        for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= BUFS - 1) {
+            copy_in(L.X[i], kq, wave - 4, 4, lane);
+            copy_in(L.Y[i], tp, wave - 4, 4, lane);
+            kq += sizeof(KQ<T, NKT>);
+            tp += sizeof(TP<T>);
+            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+            __syncthreads();                     // this chunk is here; with two buffers, the one before is done
+            if (BUFS == 1) __syncthreads();      // this chunk is done
+        }
+        return;
+    }
+    const int c0 = cb * G::W + wave * 16 * NB;
+    const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
+    f32x4 S[2 * NKT][NB];
+    float sinv = 1.0f;
+    each_state<NKT, NB>(a, c0, lane, [&](int t, int j, int r, int at, bool in) {
+        const float x = b.state_in ? (b.state_in + so)[at] : 0.0f;
+        S[t][j][r] = in ? x : 0.0f;
+    });
+    Cols<T, NKT, NB, FAST> cols(a, s, h, (long long)b.first * C, c0, lane);
+    if (n > 0) cols.fetch(n);
+    for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= BUFS - 1) {
+        const int left = n - t0, nt = min(4, (left + 15) >> 4);
+        cols.stage(L.V[wave]);
+        __syncthreads();
+        advance<T, NKT, NB>(L.X[i], L.Y[i], L.V[wave], S, sinv, here(lane), nt, [&] {
+            if (left > C) cols.fetch(left - C);
+        });
+        cols.store(L.V[wave], left);
+        if (BUFS == 1) __syncthreads();
+    }
+    if (b.state_out)
+        each_state<NKT, NB>(a, c0, here(lane), [&](int t, int j, int r, int at, bool in) {
+            if (in) (b.state_out + so)[at] = S[t][j][r] * sinv;
+        });
+}
+
+// ---- launches ----
+template <class T, int NKT, int NB, bool FAST>
+void launch_fused(const nnsp_delta_args& a, hipStream_t st) {
     const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 64 * NB - 1) / (64 * NB));
     delta_chunk_kernel<T, NKT, NB, FAST><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
 }
-template <class T, int NKT, bool FAST>
-void launch_nb(const nnsp_delta_args& a, hipStream_t st) {
-    if (a.dv <= 64) launch_as<T, NKT, 1, FAST>(a, st);
-    else launch_as<T, NKT, 2, FAST>(a, st);
+
+template <class T, int NKT>
+DeltaSplit plan_split(const nnsp_delta_args& a) {
+    DeltaSplit p;
+    const long long rows = (long long)a.n_streams * a.value_heads;
+    p.chunks = (a.n_frames + C - 1) / C;
+    p.kq_bytes = (long long)a.n_streams * a.key_heads * sizeof(KQ<T, NKT>);  // a chunk of all streams
+    p.tp_bytes = rows * sizeof(TP<T>);
+    const long long per = p.kq_bytes + p.tp_bytes;
+    p.slab = (int)(per * p.chunks <= DELTA_SLAB_BYTES ? p.chunks : DELTA_SLAB_BYTES / per < 1 ? 1 : DELTA_SLAB_BYTES / per);
+    p.state_bytes = p.slab < p.chunks ? (rows * a.dk * a.dv * 4 + 15) / 16 * 16 : 0;
+    return p;
 }
-template <class T>
-int launch_chunk(const nnsp_delta_args& a, hipStream_t st) {
-    if ((a.dk | a.dv) & 7) {
-        if (a.dk <= 64) launch_nb<T, 2, false>(a, st);
-        else launch_nb<T, 4, false>(a, st);
-    } else if (a.dk <= 32) {
-        launch_nb<T, 1, true>(a, st);
-    } else if (a.dk <= 64) {
-        launch_nb<T, 2, true>(a, st);
-    } else if (a.dk <= 96) {
-        launch_nb<T, 3, true>(a, st);
-    } else {
-        launch_nb<T, 4, true>(a, st);
+
+template <class T, int NKT, bool FAST>
+void launch_split(const nnsp_delta_args& a, hipStream_t st) {
+    constexpr int BUFS = 2 * (sizeof(KQ<T, NKT>) + sizeof(TP<T>)) + sizeof(T) * 4 * C * Geo<T, NKT, 1>::VS <= 160 * 1024 ? 2 : 1;
+    const DeltaSplit p = plan_split<T, NKT>(a);
+    const long long rows = (long long)a.n_streams * a.value_heads;
+    char* w = (char*)a.workspace;
+    float* carry = (float*)w;
+    Slab b;
+    b.kq = w + p.state_bytes;
+    b.tp = b.kq + p.kq_bytes * p.slab;
+    for (b.first = 0; b.first < p.chunks; b.first += p.slab) {
+        b.chunks = p.chunks - b.first < p.slab ? p.chunks - b.first : p.slab;
+        b.state_in = b.first ? carry : a.state_in;
+        b.state_out = b.first + b.chunks < p.chunks ? carry : a.state_out;
+        delta_prepare_kernel<T, NKT, FAST><<<dim3((unsigned)(rows * b.chunks)), dim3(256), 0, st>>>(a, b);
+        delta_scan_kernel<T, NKT, 1, FAST, BUFS><<<dim3((unsigned)(rows * ((a.dv + 63) / 64))), dim3(512), 0, st>>>(a, b);
     }
+}
+
+// f<NKT, FAST>() of this call's sizes
+template <class F>
+auto with_sizes(const nnsp_delta_args& a, const F& f) {
+    typedef std::integral_constant<int, 1> I1;
+    typedef std::integral_constant<int, 2> I2;
+    typedef std::integral_constant<int, 3> I3;
+    typedef std::integral_constant<int, 4> I4;
+    if ((a.dk | a.dv) & 7) return a.dk <= 64 ? f(I2(), std::false_type()) : f(I4(), std::false_type());
+    if (a.dk <= 32) return f(I1(), std::true_type());
+    if (a.dk <= 64) return f(I2(), std::true_type());
+    if (a.dk <= 96) return f(I3(), std::true_type());
+    return f(I4(), std::true_type());
+}
+
+template <class T>
+DeltaSplit chunk_plan(const nnsp_delta_args& a) {
+    return with_sizes(a, [&](auto nkt, auto) { return plan_split<T, decltype(nkt)::value>(a); });
+}
+
+template <class T>
+int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
+    with_sizes(a, [&](auto nkt, auto fast) {
+        constexpr int NKT = decltype(nkt)::value;
+        constexpr bool FAST = decltype(fast)::value;
+        if (split) launch_split<T, NKT, FAST>(a, st);
+        else if (a.dv <= 64) launch_fused<T, NKT, 1, FAST>(a, st);
+        else launch_fused<T, NKT, 2, FAST>(a, st);
+        return 0;
+    });
     return (int)hipGetLastError();
 }
 

@@ -15,10 +15,14 @@ extern "C" {
 #define NNSP_NORM_MAX_DIM 16384
 
 int nnspk_launch_delta_step(const nnsp_delta_args *a, void *stream);
-/* dk <= NNSP_DELTA_CHUNK_DK */
-int nnspk_launch_delta_chunk_f32(const nnsp_delta_args *a, void *stream);
-int nnspk_launch_delta_chunk_bf16(const nnsp_delta_args *a, void *stream);
-int nnspk_launch_delta_chunk_f16(const nnsp_delta_args *a, void *stream);
+/* dk <= NNSP_DELTA_CHUNK_DK; split: in two passes over the workspace, of
+ * nnspk_delta_split_bytes_*() bytes */
+int nnspk_launch_delta_chunk_f32(const nnsp_delta_args *a, int split, void *stream);
+int nnspk_launch_delta_chunk_bf16(const nnsp_delta_args *a, int split, void *stream);
+int nnspk_launch_delta_chunk_f16(const nnsp_delta_args *a, int split, void *stream);
+long long nnspk_delta_split_bytes_f32(const nnsp_delta_args *a);
+long long nnspk_delta_split_bytes_bf16(const nnsp_delta_args *a);
+long long nnspk_delta_split_bytes_f16(const nnsp_delta_args *a);
 int nnspk_launch_norm(const nnsp_norm_args *a, void *stream);
 
 /* 1: kernels on device `dev` can use p (its own device memory, pinned host or

@@ -241,6 +241,68 @@ def test_delta_chunks_then_frames():
         close(s, rs, "f32", T, 64, what + " state")
 
 
+def delta_ref_all(d, l2norm, scale, eps=1e-6):
+    """The rule in 64 bits on the GPU, all streams and heads of a frame at once."""
+    q, k, v, g, beta, st = (d[n].double() for n in ("q", "k", "v", "g", "beta", "state"))
+    rep = v.shape[2] // q.shape[2]
+    if l2norm:
+        q = q / (q.square().sum(-1, keepdim=True) + eps).sqrt()
+        k = k / (k.square().sum(-1, keepdim=True) + eps).sqrt()
+    out = torch.empty_like(v)
+    for t in range(v.shape[1]):
+        kt, qt = k[:, t].repeat_interleave(rep, 1), q[:, t].repeat_interleave(rep, 1)
+        st = st * torch.exp(g[:, t])[..., None, None]
+        u = beta[:, t][..., None] * (v[:, t] - (st * kt[..., None]).sum(2))
+        st = st + kt[..., None] * u[..., None, :]
+        out[:, t] = scale * (st * qt[..., None]).sum(2)
+    return out.cpu(), st.cpu()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("S,T,hk,hv,dk,dv", [
+    (1100, 70, 1, 1, 32, 32), (600, 130, 1, 2, 64, 64), (280, 100, 2, 4, 128, 128), (520, 75, 1, 2, 61, 100),  # many streams
+    (1030, 20, 1, 1, 96, 40),
+    (8, 330, 32, 32, 128, 128), (9, 300, 16, 32, 104, 72),  # few, and more images than a slab holds
+])
+def test_delta_many_streams_and_slabs(S, T, hk, hv, dk, dv, dtype):
+    d = make(S, T, hk, hv, dk, dv, dtype, seed=S)
+    out, so = run_delta(d, hk, dtype)
+    ro, rs = delta_ref_all(d, True, dk ** -0.5)
+    close(out, ro, dtype, T, dk, "out")
+    close(so, rs, "f32", T, dk, "state")
+
+
+@pytest.mark.parametrize("state", [True, False])
+def test_delta_slabs_ragged(state):
+    """Streams that end in the first slab, in the middle and in the last; the final state dropped or kept."""
+    S, T, h, d_ = 8, 330, 32, 128
+    lens = [0, 5, 64, 190, 191, 200, 329, 330]
+    d = make(S, T, h, h, d_, d_, "f32", seed=77)
+    out, so = run_delta(d, h, "f32", lens=lens, state=state)
+    for s, n in enumerate(lens):
+        one = {k: v[s:s + 1] for k, v in d.items()}
+        one = {k: (v[:, :n].contiguous() if k != "state" else v if state else torch.zeros_like(v)) for k, v in one.items()}
+        ro, rs = delta_ref_all(one, True, d_ ** -0.5)
+        assert bool((out[s, n:] == 7).all())
+        close(out[s:s + 1, :n], ro, "f32", T, d_, f"out {s}")
+        close(so[s:s + 1], rs, "f32", T, d_, f"state {s}")
+
+
+@pytest.mark.parametrize("T", [5, 60, 140])
+def test_delta_keys_of_zeros_and_of_all_lengths(T):
+    """Silence (keys and queries of zeros, also with eps 0) and frames far quieter than their neighbours."""
+    for dtype in ("bf16", "f16", "f32"):
+        d = make(2, T, 1, 2, 64, 64, dtype, seed=31)
+        quiet = 2.0 ** -torch.arange(T, dtype=torch.float32).remainder(13).cuda()[None, :, None, None]
+        d["k"], d["q"] = (d["k"].float() * quiet).to(DT[dtype]), (d["q"].float() * quiet.flip(1)).to(DT[dtype])
+        d["k"][:, 1::7] = 0
+        d["q"][:, 2::5] = 0
+        out, so = run_delta(d, 1, dtype)
+        ro, rs = delta_ref(d["q"], d["k"], d["v"], d["g"], d["beta"], d["state"], None, True, 64 ** -0.5)
+        close(out, ro, dtype, T, 64, "out")
+        close(so, rs, "f32", T, 64, "state")
+
+
 def test_delta_same_bits_every_time_and_by_stream():
     """Results do not depend on the run, nor on the other streams of the call."""
     d = make(40, 130, 2, 4, 64, 64, "bf16", seed=6)

@@ -45,7 +45,7 @@ def refused(call, message, code=_lib.NNSP_EINVAL):
     ((1, 1, 0, 1, 8, 8), "multiple of key_heads", -1), ((1, 1, 2, 3, 8, 8), "multiple of key_heads", -1),
     ((1, 1, 1, 0, 8, 8), "multiple of key_heads", -1),
     ((1, 1, 1, 1, 0, 8), "dk, dv", -2), ((1, 1, 1, 1, 257, 8), "dk, dv", -2), ((1, 1, 1, 1, 8, 257), "dk, dv", -2),
-    ((1 << 30, 1, 1, 2, 8, 8), "below 2", -2),
+    ((1 << 30, 1, 1, 2, 8, 8), "below 2", -2), ((1, (1 << 30) + 1, 1, 1, 8, 8), "n_frames", -2),
 ])
 def test_delta_sizes_refused(sizes, message, code):
     refused(lambda: GatedDelta(*sizes), message, code)
@@ -108,6 +108,17 @@ def test_delta_names_of_strides():
 @pytest.mark.parametrize("kw", [{"scale": float("inf")}, {"scale": float("nan")}, {"eps": -1.0}, {"eps": float("nan")}])
 def test_delta_scalars_refused(kw):
     refused(delta(**kw), "finite")
+
+
+def test_delta_workspace():
+    """Few streams over many frames ask for one, bounded however long they are; others do not."""
+    assert GatedDelta(1, 8, 1, 1, 64, 64).workspace_bytes == 0
+    assert GatedDelta(8192, 100, 2, 2, 64, 64).workspace_bytes == 0
+    assert GatedDelta(0, 1000, 2, 2, 64, 64).workspace_bytes == 0
+    n = [GatedDelta(1, T, 16, 32, 128, 128).workspace_bytes for T in (128, 16384, 1 << 30)]
+    assert 0 < n[0] < n[1] <= n[2] < 128 << 20
+    refused(delta(sizes=(2, 1000, 1, 2, 64, 64)), "workspace of 0 bytes")
+    refused(delta({"workspace": BAD + 8}, sizes=(2, 1000, 1, 2, 64, 64)), "workspace is not aligned")
 
 
 def test_delta_nothing_to_do():
