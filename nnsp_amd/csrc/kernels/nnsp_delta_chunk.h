@@ -155,7 +155,8 @@ struct TP {
     alignas(16) float beta[C], fx[C], fk[C], fq[C];  // factors of v, K S0, U into the state, Q S0
     alignas(16) float pi[C];                         // 2^-scale of P's rows
     float ti[4];                                     // 2^-scale of T's row tiles
-    float all, fkmax, pad[2];                        // decay over the whole chunk; largest fk
+    float all, fkmax;                                // decay over the whole chunk; largest fk
+    float bmax, xmax;                                // largest |beta|; |beta e(G) k^ . x| is at most xmax |x|_max
 };
 // what making T and P takes besides; s and e are the first and last frame of a frame's 16
 struct Make {
@@ -311,8 +312,9 @@ __device__ __forceinline__ void make_tp(const KQ<T, NKT>& X, TP<T>& Y, Make& M, 
             Y.fq[i] = up * M.qx[i];
             const float fk = exp2_fast((M.gh[C - 1] - h) + (M.gl[C - 1] - l)) * kx;
             Y.fk[i] = fk;
-            const float m = wave_max(fk);
-            if (i == C - 1) Y.all = up, Y.fkmax = m;
+            const float m = wave_max(fk), b = wave_max(fabsf(Y.beta[i]));
+            const float x = wave_max(fabsf(Y.beta[i]) * up * M.kn[i]) * sqrtf(32.0f * NKT);
+            if (i == C - 1) Y.all = up, Y.fkmax = m, Y.bmax = b, Y.xmax = x;
         }
     }
     __syncthreads();
@@ -430,6 +432,21 @@ __device__ __forceinline__ void make_tp(const KQ<T, NKT>& X, TP<T>& Y, Make& M, 
     __syncthreads();
 }
 
+// accumulator tile n of 16 staged rows of v
+template <class T, int VS>
+__device__ __forceinline__ f32x4 tile_of(const T (*V)[VS], int n, int l15, int g) {
+    f32x4 v;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = V[4 * g + r][16 * n + l15];
+    } else {
+        const auto t = __builtin_bit_cast(typename Vec<T, 4>::raw, read_tr(&V[4 * g + (l15 >> 2)][16 * n + 4 * (l15 & 3)]));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = (float)t[r];
+    }
+    return v;
+}
+
 // The products with the state for one chunk of nt live tiles of 16 frames: this
 // wave's columns.  S holds the state times 1 / sinv, a power of two; between()
 // runs once the state's 16-bit parts are dead (it holds the next chunk's loads).
@@ -490,17 +507,7 @@ __device__ __forceinline__ void advance(const KQ<T, NKT>& X, const TP<T>& Y, T (
             const f32x4 fx = ld4(&Y.fx[16 * m + 4 * g]) * -inv, fq = ld4(&Y.fq[16 * m + 4 * g]) * inv;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                f32x4 v;
-                if constexpr (G::WIDE) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = V[16 * m + 4 * g + r][16 * n + l15];
-                } else {
-                    const auto t = __builtin_bit_cast(typename Vec<T, 4>::raw,
-                                                      read_tr(&V[16 * m + 4 * g + (l15 >> 2)][16 * n + 4 * (l15 & 3)]));
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = (float)t[r];
-                }
-                v *= b;
+                const f32x4 v = tile_of<T>(V + 16 * m, n, l15, g) * b;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) R[m][n][r] = fmaf(fx[r], x[n][r], v[r]);
                 O[m][n] = o[n] * fq;
@@ -661,6 +668,9 @@ struct Rows {
     __device__ __forceinline__ void fetch(int dk, int left) {
         fetch_rows<T, NKT, FAST>(rk, kp, quarter, dk, row < left);
         fetch_rows<T, NKT, FAST>(rq, qp, quarter, dk, row < left);
+        fetch_gates(left);
+    }
+    __device__ __forceinline__ void fetch_gates(int left) {
         rg = rb = 0.0f;
         if (wave == 0 && lane < left) {
             if (gp) rg = *gp;
@@ -674,13 +684,16 @@ struct Rows {
     __device__ __forceinline__ void stage(const nnsp_delta_args& a, KQ<T, NKT>& X, TP<T>& Y, Make& M) {
         constexpr int KP = KQ<T, NKT>::KP, KS = KQ<T, NKT>::KS;
         float ss, inv, f;
-        // a row of zeros has inv 0 and no part in anything, whatever its norm's reciprocal is
+        // a row of zeros has inv 0 and no part in anything, whatever its norm's reciprocal is (v_rsq_f32: one unit)
         inv = stage_rows<T, NKT, KP, KS>(rk, X.K, row, quarter, ss);
-        f = a.l2norm ? 1.0f / sqrtf(ss + a.eps) : 1.0f;
-        if (quarter == 0) M.kx[row] = inv > 0.0f ? inv * f : 0.0f, M.kn[row] = inv > 0.0f ? sqrtf(ss) * f : 0.0f;
+        f = a.l2norm ? __builtin_amdgcn_rsqf(ss + a.eps) : 1.0f;
+        if (quarter == 0) M.kx[row] = inv > 0.0f ? inv * f : 0.0f, M.kn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * f : 0.0f;
         inv = stage_rows<T, NKT, KP, KS>(rq, X.Q, row, quarter, ss);
-        f = a.scale * (a.l2norm ? 1.0f / sqrtf(ss + a.eps) : 1.0f);
-        if (quarter == 0) M.qx[row] = inv > 0.0f ? inv * f : 0.0f, M.qn[row] = inv > 0.0f ? sqrtf(ss) * fabsf(f) : 0.0f;
+        f = a.scale * (a.l2norm ? __builtin_amdgcn_rsqf(ss + a.eps) : 1.0f);
+        if (quarter == 0) M.qx[row] = inv > 0.0f ? inv * f : 0.0f, M.qn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * fabsf(f) : 0.0f;
+        stage_gates(Y, M);
+    }
+    __device__ __forceinline__ void stage_gates(TP<T>& Y, Make& M) {
         if (wave == 0) {
             // running sum of g in 64 bits, in units of log2, kept as two floats: differences of near frames stay exact
             double x = (double)decay_log(rg) * 1.4426950408889634;
@@ -696,25 +709,26 @@ struct Rows {
     }
 };
 
-// The same for a wave's columns of v, and for out the other way.
-template <class T, int NKT, int NB, bool FAST>
+// The same for FR frames of 16 NB columns of v by one wave, and for out the other way.
+template <class T, int NKT, int NB, bool FAST, int FR>
 struct Cols {
-    static constexpr int LPR = 2 * NB, ROWS = 64 / LPR, N = C / ROWS, VS = Geo<T, NKT, NB>::VS;
+    static constexpr int LPR = 2 * NB, ROWS = 64 / LPR < FR ? 64 / LPR : FR, N = FR / ROWS, VS = Geo<T, NKT, NB>::VS;
     typedef typename Vec<T, 8>::raw V8;
     typedef typename Vec<T, 8>::type V8u;
     const T* vp;
     T* op;
-    long long vs, os;
+    long long vs, os, vc, oc;
     int row, col, left;  // left: columns from this lane's first on
     V8 x[N];
 
     __device__ __forceinline__ Cols(const nnsp_delta_args& a, int s, int h, long long t0, int c0, int lane)
-        : row(lane / LPR), col((lane % LPR) * 8), left(a.dv - c0 - (lane % LPR) * 8) {
+        : row(lane / LPR), col((lane % LPR) * 8), left(row < ROWS ? a.dv - c0 - col : 0) {
         vp = (const T*)a.v + s * a.v_stride[0] + h * a.v_stride[2] + (t0 + row) * a.v_stride[1] + c0 + col;
         op = (T*)a.out + s * a.out_stride[0] + h * a.out_stride[2] + (t0 + row) * a.out_stride[1] + c0 + col;
         vs = ROWS * a.v_stride[1], os = ROWS * a.out_stride[1];
+        vc = (C - FR) * a.v_stride[1], oc = (C - FR) * a.out_stride[1];  // from a chunk's last frame here to the next's first
     }
-    // frames: live frames from the chunk's first on
+    // frames: live frames from the first here on
     __device__ __forceinline__ void fetch(int frames) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -730,10 +744,20 @@ struct Cols {
             }
             vp += vs;
         }
+        vp += vc;
+    }
+    __device__ __forceinline__ float largest() const {
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf((float)x[i][j]));
+        return m;
     }
     __device__ __forceinline__ void stage(T (*V)[VS]) const {
+        if (row < ROWS)
 #pragma unroll
-        for (int i = 0; i < N; ++i) *reinterpret_cast<V8*>(&V[row + ROWS * i][col]) = x[i];
+            for (int i = 0; i < N; ++i) *reinterpret_cast<V8*>(&V[row + ROWS * i][col]) = x[i];
         // the wave's own columns: LDS keeps its order within a wave, the compiler has to
         asm volatile("" ::: "memory");
     }
@@ -741,17 +765,17 @@ struct Cols {
         asm volatile("" ::: "memory");
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const bool live = row + ROWS * i < frames;
-            const V8 y = *reinterpret_cast<const V8*>(&V[row + ROWS * i][col]);
+            const bool live = row < ROWS && row + ROWS * i < frames;
             if (FAST) {
-                if (live && left > 0) *reinterpret_cast<V8u*>(op) = y;
+                if (live && left > 0) *reinterpret_cast<V8u*>(op) = *reinterpret_cast<const V8*>(&V[row + ROWS * i][col]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (live && j < left) op[j] = y[j];
+                    if (live && j < left) op[j] = V[row + ROWS * i][col + j];
             }
             op += os;
         }
+        op += oc;
     }
 };
 
@@ -789,7 +813,7 @@ __global__ __launch_bounds__(256, 2) void delta_chunk_kernel(const nnsp_delta_ar
         S[t][j][r] = in ? x : 0.0f;
     });
     Rows<T, NKT, FAST> rows(a, s, h, 0, tid, wave);
-    Cols<T, NKT, NB, FAST> cols(a, s, h, 0, c0, lane);
+    Cols<T, NKT, NB, FAST, C> cols(a, s, h, 0, c0, lane);
     if (n > 0) {
         rows.fetch(a.dk, n);
         cols.fetch(n);
@@ -833,8 +857,9 @@ __device__ __forceinline__ void copy_out(char* dst, const X& src, int tid) {
         reinterpret_cast<f32x4*>(dst)[i] = reinterpret_cast<const f32x4*>(&src)[i];
 }
 
+// One workgroup per stream, key head and chunk, for all the key head's value heads.
 template <class T, int NKT, bool FAST>
-__global__ __launch_bounds__(256) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
+__global__ __launch_bounds__(256, 2) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
     struct Lds {
         KQ<T, NKT> X;
         TP<T> Y;
@@ -843,17 +868,29 @@ __global__ __launch_bounds__(256) void delta_prepare_kernel(const nnsp_delta_arg
     };
     __shared__ Lds L;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int c = blockIdx.x % b.chunks, h = (blockIdx.x / b.chunks) % a.value_heads, s = blockIdx.x / b.chunks / a.value_heads;
-    const int rep = a.value_heads / a.key_heads;
-    const int t0 = (b.first + c) * C, left = frames_of(a, s) - t0, nt = min(4, (left + 15) >> 4);
+    const int c = blockIdx.x % b.chunks, hk = (blockIdx.x / b.chunks) % a.key_heads, s = blockIdx.x / b.chunks / a.key_heads;
+    const int rep = a.value_heads / a.key_heads, h0 = hk * rep;
+    const int t0 = (b.first + c) * C, left = frames_of(a, s) - t0;
     if (left <= 0) return;
-    Rows<T, NKT, FAST> rows(a, s, h, t0, tid, wave);
+    Rows<T, NKT, FAST> rows(a, s, h0, t0, tid, wave);
     rows.fetch(a.dk, left);
     rows.stage(a, L.X, L.Y, L.M);
     __syncthreads();
-    if (h % rep == 0) copy_out(b.kq + (((long long)s * a.key_heads + h / rep) * b.chunks + c) * sizeof(KQ<T, NKT>), L.X, tid);
-    make_tp<T, NKT>(L.X, L.Y, L.M, L.A, wave, lane, nt);
-    copy_out(b.tp + (((long long)s * a.value_heads + h) * b.chunks + c) * sizeof(TP<T>), L.Y, tid);
+    copy_out(b.kq + (((long long)s * a.key_heads + hk) * b.chunks + c) * sizeof(KQ<T, NKT>), L.X, tid);
+    for (int r = 0; r < rep; ++r) {
+        if (r + 1 < rep) {
+            if (rows.gp) rows.gp += a.g_stride[2];
+            rows.bp += a.beta_stride[2];
+            rows.fetch_gates(left);
+        }
+        make_tp<T, NKT>(L.X, L.Y, L.M, L.A, wave, here(lane), 4);
+        copy_out(b.tp + (((long long)s * a.value_heads + h0 + r) * b.chunks + c) * sizeof(TP<T>), L.Y, tid);
+        if (r + 1 < rep) {
+            __syncthreads();
+            rows.stage_gates(L.Y, L.M);
+            __syncthreads();
+        }
+    }
 }
 
 // an image into LDS, past the registers: waves `wave` of `waves`, 1 KB an instruction
@@ -866,59 +903,261 @@ __device__ __forceinline__ void copy_in(X& dst, const char* src, int wave, int w
                                              (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(&dst) + i * 16), 16, 0, 0);
 }
 
-// Waves 0 .. 3 take the columns through the chunks, waves 4 .. 7 bring the next
-// chunk's images (BUFS 2; where LDS has room for one only, all wait for it).
+// a tile times its rows' factors, as half of the high and low B operand that it is part of
+template <bool LOW>
+__device__ __forceinline__ void put_part(h8 (*dst)[64], int lane, int half, const f32x4& x, const f32x4& s) {
+    typedef unsigned u2 __attribute__((ext_vector_type(2)));
+    const h4 hi = __builtin_bit_cast(h4, u2{pack(x[0], s[0], x[1], s[1]), pack(x[2], s[2], x[3], s[3])});
+    reinterpret_cast<h4*>(&dst[0][lane])[half] = hi;
+    if (LOW) {
+        h4 lo;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) lo[i] = (_Float16)fmaf(x[i], s[i], -(float)hi[i]);
+        reinterpret_cast<h4*>(&dst[1][lane])[half] = lo;
+    }
+}
+
+// What the four waves of a scan hand each other: B operands of 32 rows x 16
+// columns, high and low, and the largest magnitudes that set their scales.
+template <int NKT, int NB>
+struct Exchange {
+    h8 S[NKT][NB][2][64], R[2][NB][2][64], U[2][NB][2][64], F[2][NB][2][64];  // S0, R, U for the output, U fk for the state
+    float smax[4], vmax[4], fmax[4];
+};
+
+template <class T, int NKT, int NB, int BUFS>
+struct ScanLds {
+    KQ<T, NKT> X[BUFS];
+    TP<T> Y[BUFS];
+    Exchange<NKT, NB> E;
+    alignas(16) T V[4][16][Geo<T, NKT, NB>::VS];
+};
+
+// The chain through the chunks for 16 NB columns.  Its length is what counts, so
+// each of waves 0 .. 3 does a quarter of every product: a tile of 16 frames in
+// K S0, T R, Q S0 and P U, a quarter of the state's rows in K^T U, handing its
+// results on through LDS (three barriers a chunk).  Waves 4 .. 7 bring the next
+// chunk's images meanwhile (BUFS 2; where LDS has room for one, all wait).
+// Scales have to be the same for all four before anybody has seen all values:
+// they come from bounds (|R| <= bmax |v| + xmax |S|, |u| <= 64 2^30,
+// |S1| <= all |S0| + 64 2^15 |U fk|) over the magnitudes exchanged at the
+// barriers, looser than the largest value by 2^4 to 2^8.
 template <class T, int NKT, int NB, bool FAST, int BUFS>
 __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a, const Slab b) {
     using G = Geo<T, NKT, NB>;
-    struct Lds {
-        KQ<T, NKT> X[BUFS];
-        TP<T> Y[BUFS];
-        alignas(16) T V[4][C][G::VS];
-    };
-    __shared__ Lds L;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int ncb = (a.dv + G::W - 1) / G::W;
-    const int cb = blockIdx.x % ncb, h = (blockIdx.x / ncb) % a.value_heads, s = blockIdx.x / ncb / a.value_heads;
+    constexpr bool LOW = G::OP == 2;
+    constexpr int TPW = (2 * NKT + 3) / 4;  // state tiles of a wave
+    __shared__ ScanLds<T, NKT, NB, BUFS> L;
+    const int lane_ = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // streams and heads vary fastest: a multiple of 8 of them puts all workgroups of a head on one XCD and its L2
+    const unsigned rows = (unsigned)a.n_streams * a.value_heads;
+    const int cb = blockIdx.x / rows, row = blockIdx.x % rows, h = row % a.value_heads, s = row / a.value_heads;
     const int hk = h / (a.value_heads / a.key_heads);
     const int n = min(frames_of(a, s) - b.first * C, b.chunks * C);  // frames in this slab
     if (wave >= 4) {
         const char* kq = b.kq + ((long long)s * a.key_heads + hk) * b.chunks * sizeof(KQ<T, NKT>);
         const char* tp = b.tp + ((long long)s * a.value_heads + h) * b.chunks * sizeof(TP<T>);
-        for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= BUFS - 1) {
-            copy_in(L.X[i], kq, wave - 4, 4, lane);
-            copy_in(L.Y[i], tp, wave - 4, 4, lane);
+        const auto load = [&](int i) {
+            copy_in(L.X[i], kq, wave - 4, 4, lane_);
+            copy_in(L.Y[i], tp, wave - 4, 4, lane_);
             kq += sizeof(KQ<T, NKT>);
             tp += sizeof(TP<T>);
+        };
+        if (n > 0) load(0);
+        __syncthreads();
+        for (int t0 = 0, i = 0; t0 < n; t0 += C) {
             __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-            __syncthreads();                     // this chunk is here; with two buffers, the one before is done
-            if (BUFS == 1) __syncthreads();      // this chunk is done
+            __syncthreads();                     // this chunk is here, and the one before done with its buffer (BUFS 2)
+            if (BUFS == 2 && n - t0 > C) load(i ^= 1);
+            __syncthreads();
+            __syncthreads();
+            if (BUFS == 1) {
+                __syncthreads();  // this chunk is done with the buffer
+                if (n - t0 > C) load(0);
+            }
         }
         return;
     }
-    const int c0 = cb * G::W + wave * 16 * NB;
+    const int c0 = cb * 16 * NB;
     const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
-    f32x4 S[2 * NKT][NB];
-    float sinv = 1.0f;
-    each_state<NKT, NB>(a, c0, lane, [&](int t, int j, int r, int at, bool in) {
+    const f32x4 zero = {0, 0, 0, 0};
+    f32x4 S[TPW][NB];
+    float sinv = 1.0f, m = 0.0f;
+    // f(i, j, r, at, in) for element r of tile (i, j), as each_state
+    const auto own_state = [&](int lane, const auto& f) {
+        const int l15 = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < TPW; ++i) {
+            const int t = wave * TPW + i;
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int rw = 32 * (t >> 1) + 4 * (t & 1) + r + 8 * g, col = c0 + 16 * j + l15;
+                    f(i, j, r, min(rw, a.dk - 1) * a.dv + min(col, a.dv - 1), rw < a.dk && col < a.dv);
+                }
+        }
+    };
+    own_state(lane_, [&](int i, int j, int r, int at, bool in) {
         const float x = b.state_in ? (b.state_in + so)[at] : 0.0f;
-        S[t][j][r] = in ? x : 0.0f;
+        S[i][j][r] = in ? x : 0.0f;
+        m = fmaxf(m, fabsf(S[i][j][r]));
     });
-    Cols<T, NKT, NB, FAST> cols(a, s, h, (long long)b.first * C, c0, lane);
-    if (n > 0) cols.fetch(n);
+    m = wave_max(m);
+    if (lane_ == 0) L.E.smax[wave] = m;
+    __syncthreads();
+    const auto max4 = [](const float* p) {
+        const f32x4 x = ld4(p);
+        return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    };
+    float sbound = max4(L.E.smax);  // of |S|, the registers' values
+
+    Cols<T, NKT, NB, FAST, 16> cols(a, s, h, (long long)b.first * C + 16 * wave, c0, lane_);
+    if (n > 0) cols.fetch(n - 16 * wave);
     for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= BUFS - 1) {
-        const int left = n - t0, nt = min(4, (left + 15) >> 4);
-        cols.stage(L.V[wave]);
+        const int lane = here(lane_), l15 = lane & 15, g = lane >> 4, left = n - t0;
+        const KQ<T, NKT>& X = L.X[i];
+        const TP<T>& Y = L.Y[i];
+        Exchange<NKT, NB>& E = L.E;
+        // 1: the state's parts, and what bounds R
+        float inv;
+        {
+            const float sc = scale_of(sbound, inv);
+            inv *= sinv;
+            m = 0.0f;
+#pragma unroll
+            for (int j = 0; j < TPW; ++j) {
+                const int t = wave * TPW + j;
+                if (t >= 2 * NKT) continue;
+#pragma unroll
+                for (int k = 0; k < NB; ++k) {
+                    put_part<true>(E.S[t >> 1][k], lane, t & 1, S[j][k], all4(sc));
+                    m = amax4(m, S[j][k]);
+                }
+            }
+            m = wave_max(m);
+            const float v = wave_max(cols.largest());
+            cols.stage(L.V[wave]);
+            if (lane == 0) E.smax[wave] = m, E.vmax[wave] = v;
+        }
         __syncthreads();
-        advance<T, NKT, NB>(L.X[i], L.Y[i], L.V[wave], S, sinv, here(lane), nt, [&] {
-            if (left > C) cols.fetch(left - C);
-        });
-        cols.store(L.V[wave], left);
+        // 2: R and Q S0 of this wave's frames
+        const float sreg = max4(E.smax), smax = sreg * sinv;  // the registers' values, the true ones
+        float rinv;
+        f32x4 O[NB];
+        {
+            const float sc = scale_of(Y.bmax * max4(E.vmax) + Y.xmax * smax, rinv);
+            f32x4 x[NB];
+#pragma unroll
+            for (int s = 0; s < NKT; ++s) {
+                const int c = 32 * s + 8 * g;
+                const h8 k = *reinterpret_cast<const h8*>(&X.K[0][16 * wave + l15][c]);
+                const h8 q = *reinterpret_cast<const h8*>(&X.Q[0][16 * wave + l15][c]);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const h8 hi = E.S[s][n][0][lane], lo = E.S[s][n][1][lane];
+                    x[n] = mma(k, lo, mma(k, hi, s ? x[n] : zero));
+                    O[n] = mma(q, hi, s ? O[n] : zero);
+                    if (LOW) O[n] = mma(q, lo, O[n]);
+                    if (G::KP == 2) {
+                        x[n] = mma(*reinterpret_cast<const h8*>(&X.K[G::KP - 1][16 * wave + l15][c]), hi, x[n]);
+                        O[n] = mma(*reinterpret_cast<const h8*>(&X.Q[G::KP - 1][16 * wave + l15][c]), hi, O[n]);
+                    }
+                }
+            }
+            const f32x4 bt = ld4(&Y.beta[16 * wave + 4 * g]), fx = ld4(&Y.fx[16 * wave + 4 * g]) * -inv;
+            const f32x4 fq = ld4(&Y.fq[16 * wave + 4 * g]) * inv;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                f32x4 r = tile_of<T>(L.V[wave], n, l15, g) * bt;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) r[e] = fmaf(fx[e], x[n][e], r[e]);
+                put_part<true>(E.R[wave >> 1][n], lane, wave & 1, r, all4(sc));
+                O[n] *= fq;
+            }
+        }
+        if (left > C) cols.fetch(left - C - 16 * wave);
+        __syncthreads();
+        // 3: U of this wave's frames; see advance() for the scales
+        const float tmax = max4(Y.ti), cinv = tmax * 0x1p22f, c = 1.0f / cinv, all = Y.all;
+        float zi, li;
+        const float z = scale_of(Y.fkmax, zi) * 0x1p-14f, low = scale_of(fmaxf(smax * (all * 0x1p-13f), 0x1p-86f), li);
+        const float s1 = fminf(c * z / rinv, low), d = all * s1 * sinv;
+        {
+            f32x4 u[NB];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (2 * s > wave) continue;
+                const h8 th = Y.T_[0].operand(wave, l15, s, g), tl = Y.T_[1].operand(wave, l15, s, g);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const h8 hi = E.R[s][n][0][lane], lo = E.R[s][n][1][lane];
+                    u[n] = mma(tl, hi, mma(th, lo, mma(th, hi, s ? u[n] : zero)));
+                }
+            }
+            const float ti = Y.ti[wave];
+            const f32x4 f = ld4(&Y.fk[16 * wave + 4 * g]) * (ti * (s1 * rinv));
+            m = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                put_part<true>(E.F[wave >> 1][n], lane, wave & 1, u[n], f);
+                put_part<LOW>(E.U[wave >> 1][n], lane, wave & 1, u[n], all4(ti * c));
+                m = amax4(m, u[n] * f);
+            }
+            m = wave_max(m);
+            if (lane == 0) E.fmax[wave] = m;
+        }
+        __syncthreads();
+        // 4: this wave's rows of the state, its frames of the output
+        sbound = fmaf(d, sreg, 0x1p21f * max4(E.fmax));
+        sinv = 1.0f / s1;
+#pragma unroll
+        for (int j = 0; j < TPW; ++j) {
+            const int t = wave * TPW + j;
+            if (t >= 2 * NKT) continue;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) S[j][n] *= d;
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int rw = 32 * s + 4 * g + (l15 >> 2), col = 32 * (t >> 1) + 8 * (l15 & 3) + 4 * (t & 1);
+#pragma unroll
+                for (int part = 0; part < G::KP; ++part) {
+                    const h4 x = __builtin_bit_cast(h4, read_tr(&X.K[part][rw][col]));
+                    const h4 y = __builtin_bit_cast(h4, read_tr(&X.K[part][rw + 16][col]));
+                    const h8 k = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        S[j][n] = mma(k, E.F[s][n][0][lane], S[j][n]);
+                        if (part == 0) S[j][n] = mma(k, E.F[s][n][1][lane], S[j][n]);
+                    }
+                }
+            }
+        }
+        {
+            f32x4 o[NB];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                if (2 * s > wave) continue;
+                const h8 ph = Y.P_[0].operand(wave, l15, s, g);
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    const h8 hi = E.U[s][n][0][lane];
+                    o[n] = mma(ph, hi, s ? o[n] : zero);
+                    if (LOW) o[n] = mma(Y.P_[G::OP - 1].operand(wave, l15, s, g), hi, mma(ph, E.U[s][n][1][lane], o[n]));
+                }
+            }
+            const f32x4 pi = ld4(&Y.pi[16 * wave + 4 * g]) * (rinv * cinv);
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) L.V[wave][4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], O[n][r]);
+        }
+        cols.store(L.V[wave], left - 16 * wave);
         if (BUFS == 1) __syncthreads();
     }
     if (b.state_out)
-        each_state<NKT, NB>(a, c0, here(lane), [&](int t, int j, int r, int at, bool in) {
-            if (in) (b.state_out + so)[at] = S[t][j][r] * sinv;
+        own_state(here(lane_), [&](int i, int j, int r, int at, bool in) {
+            if (in) (b.state_out + so)[at] = S[i][j][r] * sinv;
         });
 }
 
@@ -942,9 +1181,15 @@ DeltaSplit plan_split(const nnsp_delta_args& a) {
     return p;
 }
 
+template <class T, int NKT, int NB, bool FAST>
+void launch_scan(const nnsp_delta_args& a, const Slab& b, hipStream_t st) {
+    constexpr int BUFS = sizeof(ScanLds<T, NKT, NB, 2>) <= 160 * 1024 ? 2 : 1;
+    const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 16 * NB - 1) / (16 * NB));
+    delta_scan_kernel<T, NKT, NB, FAST, BUFS><<<dim3((unsigned)grid), dim3(512), 0, st>>>(a, b);
+}
+
 template <class T, int NKT, bool FAST>
 void launch_split(const nnsp_delta_args& a, hipStream_t st) {
-    constexpr int BUFS = 2 * (sizeof(KQ<T, NKT>) + sizeof(TP<T>)) + sizeof(T) * 4 * C * Geo<T, NKT, 1>::VS <= 160 * 1024 ? 2 : 1;
     const DeltaSplit p = plan_split<T, NKT>(a);
     const long long rows = (long long)a.n_streams * a.value_heads;
     char* w = (char*)a.workspace;
@@ -956,8 +1201,10 @@ void launch_split(const nnsp_delta_args& a, hipStream_t st) {
         b.chunks = p.chunks - b.first < p.slab ? p.chunks - b.first : p.slab;
         b.state_in = b.first ? carry : a.state_in;
         b.state_out = b.first + b.chunks < p.chunks ? carry : a.state_out;
-        delta_prepare_kernel<T, NKT, FAST><<<dim3((unsigned)(rows * b.chunks)), dim3(256), 0, st>>>(a, b);
-        delta_scan_kernel<T, NKT, 1, FAST, BUFS><<<dim3((unsigned)(rows * ((a.dv + 63) / 64))), dim3(512), 0, st>>>(a, b);
+        delta_prepare_kernel<T, NKT, FAST>
+            <<<dim3((unsigned)((long long)a.n_streams * a.key_heads * b.chunks)), dim3(256), 0, st>>>(a, b);
+        if (rows * ((a.dv + 15) / 16) <= 256) launch_scan<T, NKT, 1, FAST>(a, b, st);
+        else launch_scan<T, NKT, 2, FAST>(a, b, st);
     }
 }
 
