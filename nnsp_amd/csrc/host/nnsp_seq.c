@@ -163,7 +163,7 @@ static int delta_way(const nnsp_delta_args *a)
 {
     if (a->n_frames <= NNSP_DELTA_STEP_FRAMES || a->dk > NNSP_DELTA_CHUNK_DK) return DELTA_STEP;
     const long long rows = (long long)a->n_streams * a->value_heads * ((a->dv + 127) / 128);
-    return rows < 1024 && a->n_frames > 64 ? DELTA_SPLIT : DELTA_CHUNK;
+    return rows <= 128 && a->n_frames > 64 ? DELTA_SPLIT : DELTA_CHUNK;
 }
 
 int nnsp_delta_workspace(const nnsp_delta_args *a, size_t *bytes)

@@ -1,4 +1,4 @@
-// nnsp_delta_chunk.h -- the gated delta rule over chunks of 64 frames on the
+// nnsp_delta_chunk.h -- the gated delta rule over chunks of frames on the
 // matrix cores (include/nnsp_seq.h); one .hip file per element type launches it.
 //
 // Within a chunk, with G_i the sum of g up to frame i and S0 the state before it,
@@ -6,9 +6,9 @@
 //   A_ij = beta_i e^(G_i - G_j) k_i . k_j   (j < i)        T = (I + A)^-1
 //   U    = T (beta V - beta e^G (K S0))
 //   O    = scale (e^G (Q S0) + P U)         P_ij = e^(G_i - G_j) q_i . k_j (j <= i)
-//   S1   = e^(G_63) S0 + K^T (e^(G_63 - G) U)
+//   S1   = e^(G_n) S0 + K^T (e^(G_n - G) U)       (n the chunk's last frame)
 //
-// which is the rule of 64 frames with the recurrence left in one 64 x 64
+// which is the rule of a chunk's frames with the recurrence left in one
 // triangular inverse.  T and P need no state; the rest is five matrix products.
 //
 // Numbers.  The state, T and U are 32-bit values, and the matrix cores take 16
@@ -43,7 +43,9 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
-constexpr int C = 64;       // frames of a chunk
+// frames of a chunk: 64 where a chain of chunks is what takes time, 32 where
+// many streams fill the device and registers and LDS decide how well
+constexpr int C = 64, CF = 32;
 constexpr long long DELTA_SLAB_BYTES = 96ll << 20;
 
 // sizes of a call in two passes
@@ -91,20 +93,18 @@ __device__ __forceinline__ int here(int x) {
     return x;
 }
 
-// a s0 and b s1 rounded to fp16
-__device__ __forceinline__ unsigned pack(float a, float s0, float b, float s1) {
-    unsigned d;
-    asm("v_fma_mixlo_f16 %0, %1, %2, 0" : "=v"(d) : "v"(a), "v"(s0));
-    asm("v_fma_mixhi_f16 %0, %1, %2, 0" : "+v"(d) : "v"(b), "v"(s1));
-    return d;
+// x s rounded to fp16, as one mixed-precision fma with a zero that the compiler cannot see through
+__device__ __forceinline__ _Float16 half_of(float x, float s) {
+    float zero = 0.0f;
+    asm("" : "+s"(zero));
+    return (_Float16)fmaf(x, s, zero);
 }
 // two accumulator tiles times their rows' factors s as the high and low B
 // operand of a 32-deep product
 template <bool LOW>
 __device__ __forceinline__ void split(const f32x4& a, const f32x4& b, const f32x4& sa, const f32x4& sb, h8& hi, h8& lo) {
-    typedef unsigned u4 __attribute__((ext_vector_type(4)));
-    hi = __builtin_bit_cast(h8, u4{pack(a[0], sa[0], a[1], sa[1]), pack(a[2], sa[2], a[3], sa[3]),
-                                   pack(b[0], sb[0], b[1], sb[1]), pack(b[2], sb[2], b[3], sb[3])});
+#pragma unroll
+    for (int i = 0; i < 8; ++i) hi[i] = half_of(i < 4 ? a[i & 3] : b[i & 3], i < 4 ? sa[i & 3] : sb[i & 3]);
     if (LOW)
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -117,18 +117,22 @@ __device__ __forceinline__ s4 read_tr(const void* p) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p);
 }
 
-// T and P in LDS: row tiles 0 and 1 hold 32 frames a row, 2 and 3 all 64, in the
-// k order of two stacked accumulator tiles; 8 halves of padding spread 16 rows
-// over all banks
+// T and P in LDS, in the k order of two stacked accumulator tiles: row tiles 0
+// and 1 hold 32 frames a row, 2 and 3 (of 64-frame chunks) all 64; 8 halves of
+// padding spread 16 rows over all banks
+template <int C>
 struct Tri {
-    alignas(16) _Float16 x[32 * 40 + 32 * 72];
-    // frames 32 s + 8-element group g of row
+    alignas(16) _Float16 x[32 * 40 + (C - 32) * 72];
+    static __device__ __forceinline__ int row(int m, int l15) {
+        return m < 2 ? (16 * m + l15) * 40 : 1280 + (16 * m - 32 + l15) * 72;
+    }
+    // frames 32 s + 8-element group g of row 16 m + l15
     __device__ __forceinline__ h8 operand(int m, int l15, int s, int g) const {
-        return *reinterpret_cast<const h8*>(x + (m < 2 ? (16 * m + l15) * 40 : 1280 + (16 * m - 32 + l15) * 72) + 32 * s + 8 * g);
+        return *reinterpret_cast<const h8*>(x + row(m, l15) + 32 * s + 8 * g);
     }
     // frames 16 j + 4 g .. + 3 of row 16 m + l15
     __device__ __forceinline__ void put(int m, int l15, int j, int g, h4 v) {
-        *reinterpret_cast<h4*>(x + (m < 2 ? (16 * m + l15) * 40 : 1280 + (16 * m - 32 + l15) * 72) + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) = v;
+        *reinterpret_cast<h4*>(x + row(m, l15) + 32 * (j >> 1) + 8 * g + 4 * (j & 1)) = v;
     }
 };
 
@@ -137,21 +141,20 @@ struct Geo {
     static constexpr bool WIDE = std::is_same<T, float>::value;       // 32-bit input
     static constexpr int KP = WIDE ? 2 : 1;                           // parts of q and k
     static constexpr int OP = std::is_same<T, __bf16>::value ? 1 : 2; // parts of what only the output takes
-    static constexpr int W = 64 * NB;                                 // columns of a workgroup
-    static constexpr int VS = 16 * NB + (WIDE ? 4 : 8);               // row of a wave's V, elements
+    static constexpr int VS = 16 * NB + 4;                            // row of a wave's V, elements
 };
 
 // q and k of a chunk as the products take them
-template <class T, int NKT>
+template <class T, int NKT, int C>
 struct KQ {
     static constexpr int KP = std::is_same<T, float>::value ? 2 : 1, KS = NKT * 32 + 8;
     alignas(16) _Float16 K[KP][C][KS], Q[KP][C][KS];
 };
 // what else a chunk's products take; e() is a decay, G the sum of g
-template <class T>
+template <class T, int C>
 struct TP {
     static constexpr int OP = std::is_same<T, __bf16>::value ? 1 : 2;
-    Tri T_[2], P_[OP];
+    Tri<C> T_[2], P_[OP];
     alignas(16) float beta[C], fx[C], fk[C], fq[C];  // factors of v, K S0, U into the state, Q S0
     alignas(16) float pi[C];                         // 2^-scale of P's rows
     float ti[4];                                     // 2^-scale of T's row tiles
@@ -159,6 +162,7 @@ struct TP {
     float bmax, xmax;                                // largest |beta|; |beta e(G) k^ . x| is at most xmax |x|_max
 };
 // what making T and P takes besides; s and e are the first and last frame of a frame's 16
+template <int C>
 struct Make {
     alignas(16) float kx[C], qx[C], kn[C], qn[C];  // norm times 2^-scale, length after the norm
     alignas(16) float gh[C], gl[C];                // log2 of the decay up to the frame (two parts)
@@ -166,45 +170,50 @@ struct Make {
     alignas(16) float pb[C], pr[C];                // P rows: qx 2^scale, times e(G - G_s)
     alignas(16) float kc[C];                       // columns of both: kx e(G_e - G)
 };
+template <int C>
 struct TriA {
     alignas(16) float A[C][C + 4];  // A transposed
 };
+template <int C>
 struct Diag {
-    alignas(16) float D[4][16][20];  // transposed inverses of the diagonal blocks
+    alignas(16) float D[C / 16][16][20];  // transposed inverses of the diagonal blocks
 };
-static_assert(sizeof(Diag) <= 2 * sizeof(Tri), "the inverses lie where T is written afterwards");
+static_assert(sizeof(Diag<64>) <= 2 * sizeof(Tri<64>) && sizeof(Diag<32>) <= 2 * sizeof(Tri<32>),
+              "the inverses lie where T is written afterwards");
 
-// raw rows of q and k on their way to LDS: thread (row, quarter) holds chunks of
-// 8 elements quarter, quarter + 4, ...
-template <class T, int NKT>
+// raw rows of q and k on their way to LDS, PR threads a row: thread (row, part)
+// holds chunks of 8 elements part, part + PR, ...
+template <class T, int NKT, int PR>
 struct RawRows {
-    typename Vec<T, 8>::raw x[NKT];
+    static constexpr int N = (4 * NKT + PR - 1) / PR;
+    typename Vec<T, 8>::raw x[N];
 };
-template <class T, int NKT, bool FAST>
-__device__ __forceinline__ void fetch_rows(RawRows<T, NKT>& r, const T* p, int quarter, int n, bool live) {
+template <bool FAST, class T, int NKT, int PR>
+__device__ __forceinline__ void fetch_rows(RawRows<T, NKT, PR>& r, const T* p, int part, int n, bool live) {
 #pragma unroll
-    for (int i = 0; i < NKT; ++i) {
-        const int c = (quarter + 4 * i) * 8;
+    for (int i = 0; i < r.N; ++i) {
+        const int c = (part + PR * i) * 8;
 #pragma unroll
         for (int j = 0; j < 8; ++j) r.x[i][j] = (T)0.0f;
         if (FAST) {
-            if (live && c < n) r.x[i] = *reinterpret_cast<const typename Vec<T, 8>::type*>(p + 32 * i);
+            if (live && c < n) r.x[i] = *reinterpret_cast<const typename Vec<T, 8>::type*>(p + 8 * PR * i);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (live && c + j < n) r.x[i][j] = p[32 * i + j];
+                if (live && c + j < n) r.x[i][j] = p[8 * PR * i + j];
         }
     }
 }
 // scaled fp16 parts to LDS; returns 2^-scale (0 of a row of zeros), sets the sum of squares
-template <class T, int NKT, int KP, int KS>
-__device__ __forceinline__ float stage_rows(const RawRows<T, NKT>& r, _Float16 (*dst)[C][KS], int row, int quarter, float& ss) {
+template <int KP, int C, int KS, class T, int NKT, int PR>
+__device__ __forceinline__ float stage_rows(const RawRows<T, NKT, PR>& r, _Float16 (*dst)[C][KS], int row, int part, float& ss) {
+    constexpr int N = RawRows<T, NKT, PR>::N;
     ss = 0.0f;
     float inv;
     if constexpr (std::is_same<T, _Float16>::value) {
         // rows to a length of 2^5 .. 2^6, by the exponent of the sum of squares (which fp16 keeps in fp32's range)
 #pragma unroll
-        for (int i = 0; i < NKT; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -212,15 +221,18 @@ __device__ __forceinline__ float stage_rows(const RawRows<T, NKT>& r, _Float16 (
                 ss = __builtin_amdgcn_fdot2(x, x, ss, false);
             }
         ss = add_xor2(add_xor1(ss));
+        if (PR >= 8) ss = add_mirror4(ss);
+        if (PR >= 16) ss = add_xor8(ss);
         const int e = min(max(5 - (((__float_as_int(ss) >> 23) - 127) >> 1), -14), 15);
         const _Float16 s = __builtin_bit_cast(_Float16, (unsigned short)((15 + e) << 10));
         inv = ss > 0.0f ? __int_as_float((127 - e) << 23) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < NKT; ++i) *reinterpret_cast<h8*>(&dst[0][row][(quarter + 4 * i) * 8]) = r.x[i] * s;
+        for (int i = 0; i < N; ++i)
+            if (4 * NKT % PR == 0 || part + PR * i < 4 * NKT) *reinterpret_cast<h8*>(&dst[0][row][(part + PR * i) * 8]) = r.x[i] * s;
     } else {
         float m = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NKT; ++i)
+        for (int i = 0; i < N; ++i)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float x = (float)r.x[i][j];
@@ -228,11 +240,15 @@ __device__ __forceinline__ float stage_rows(const RawRows<T, NKT>& r, _Float16 (
                 ss = fmaf(x, x, ss);
             }
         ss = add_xor2(add_xor1(ss));
+        if (PR >= 8) ss = add_mirror4(ss);
+        if (PR >= 16) ss = add_xor8(ss);
         m = max_dpp<0x4e>(max_dpp<0xb1>(m));
+        if (PR >= 8) m = max_dpp<0x141>(m);
+        if (PR >= 16) m = max_dpp<0x128>(m);
         const float s = scale_of(m, inv);
         if (m == 0.0f) inv = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NKT; ++i) {
+        for (int i = 0; i < N; ++i) {
             h8 hi, lo;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -240,7 +256,8 @@ __device__ __forceinline__ float stage_rows(const RawRows<T, NKT>& r, _Float16 (
                 hi[j] = (_Float16)(x * s);
                 if (KP == 2) lo[j] = (_Float16)fmaf(x, s, -(float)hi[j]);
             }
-            const int c = (quarter + 4 * i) * 8;
+            const int c = (part + PR * i) * 8;
+            if (4 * NKT % PR != 0 && c >= 32 * NKT) continue;
             *reinterpret_cast<h8*>(&dst[0][row][c]) = hi;
             if (KP == 2) *reinterpret_cast<h8*>(&dst[KP - 1][row][c]) = lo;
         }
@@ -249,7 +266,7 @@ __device__ __forceinline__ float stage_rows(const RawRows<T, NKT>& r, _Float16 (
 }
 
 // tile (mi, mj) of X Y^T
-template <int NKT, int KP, int KS>
+template <int NKT, int KP, int C, int KS>
 __device__ __forceinline__ f32x4 dot_tile(const _Float16 (*X)[C][KS], const _Float16 (*Y)[C][KS], int mi, int mj, int l15, int g) {
     f32x4 acc = {0, 0, 0, 0};
 #pragma unroll
@@ -267,123 +284,159 @@ __device__ __forceinline__ f32x4 dot_tile(const _Float16 (*X)[C][KS], const _Flo
 }
 __device__ __forceinline__ f32x4 ld4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 
-// Everything of the staged chunk that needs no state, by all four waves: the
-// factors, T and P.  Starts and ends with the workgroup together.
+// Factors of the staged frames (of C / 64 waves' lanes each): part 0 those of A, part
+// 1 those of P, part 2 those of the products with the state.
 //
 // A decay between two frames of different 16s is a product of three that are
 // each at most 1 (to the end of the column's 16, between, from the start of
 // the row's), so it costs two multiplications an element; within a 16 it is an
 // exponential of the difference.  P's row scale comes from a bound (lengths of
 // q and k, the largest decay ratio), which an fp16's exponent has room for.
+template <int NKT, class T, int C>
+__device__ __forceinline__ void make_factors(const KQ<T, NKT, C>&, TP<T, C>& Y, Make<C>& M, int part, int lane) {
+    const int i = lane & (C - 1), s = i & ~15, e = i | 15;
+    const float h = M.gh[i], l = M.gl[i], kx = M.kx[i];
+    if (part == 0) {
+        const float b = Y.beta[i] * kx, r = exp2_fast((h - M.gh[s]) + (l - M.gl[s]));
+        M.ab[i] = b;
+        M.ar[i] = b * r;
+        M.kc[i] = exp2_fast((M.gh[e] - h) + (M.gl[e] - l)) * kx;
+    } else if (part == 1) {
+        // largest decay ratio of a row: e(G_i - min over j <= i of G_j); largest length of a key
+        float lo = h;
+        const float kn = wave_max(M.kn[i]);
+#pragma unroll
+        for (int d = 1; d < C; d <<= 1) {
+            const float y = __shfl_up(lo, d);
+            if (i >= d) lo = fminf(lo, y);
+        }
+        float inv;
+        const float qx = M.qx[i], sc = scale_of(M.qn[i] * kn * exp2_fast(fminf(h - lo, 120.0f)), inv);
+        Y.pi[i] = inv;
+        M.pb[i] = qx * sc;
+        M.pr[i] = qx * sc * exp2_fast((h - M.gh[s]) + (l - M.gl[s]));
+    } else {
+        const float up = exp2_fast(h), b = Y.beta[i];
+        Y.fx[i] = b * up * kx;
+        Y.fq[i] = up * M.qx[i];
+        const float fk = exp2_fast((M.gh[C - 1] - h) + (M.gl[C - 1] - l)) * kx;
+        Y.fk[i] = fk;
+        const float m = wave_max(fk);
+        if (i == C - 1) Y.all = up, Y.fkmax = m;
+        if (C == 64) {  // bounds for a scan
+            const float bm = wave_max(fabsf(b)), x = wave_max(fabsf(b) * up * M.kn[i]) * sqrtf(32.0f * NKT);
+            if (i == C - 1) Y.bmax = bm, Y.xmax = x;
+        }
+    }
+}
+
+// tile (mi, j) of A from that of K K^T
+template <int C>
+__device__ __forceinline__ void put_a(const Make<C>& M, TriA<C>& A, const f32x4& acc, int mi, int j, int l15, int g) {
+    const int col = 16 * j + l15, row = 16 * mi + 4 * g;
+    f32x4 f;
+    if (j == mi) {
+        const f32x4 h = ld4(&M.gh[row]), l = ld4(&M.gl[row]), b = ld4(&M.ab[row]);
+        const float hj = M.gh[col], lj = M.gl[col], kj = M.kx[col];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) f[r] = exp2_fast(fminf((h[r] - hj) + (l[r] - lj), 120.0f)) * (b[r] * kj);
+    } else {
+        const int a = 16 * mi, e = 16 * j + 15;
+        f = ld4(&M.ar[row]) * (M.kc[col] * exp2_fast((M.gh[a] - M.gh[e]) + (M.gl[a] - M.gl[e])));
+    }
+    *reinterpret_cast<f32x4*>(&A.A[col][row]) = acc * f;
+}
+
+// tile (mi, j) of P from that of K Q^T (so that a lane has 4 frames of a row); zeros above the diagonal
+template <class T, int C>
+__device__ __forceinline__ void put_p(TP<T, C>& Y, const Make<C>& M, const f32x4& p, int mi, int j, int l15, int g) {
+    h4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    if (j <= mi) {
+        const int row = 16 * mi + l15, col = 16 * j + 4 * g;
+        f32x4 f;
+        if (j == mi) {
+            const f32x4 h = ld4(&M.gh[col]), l = ld4(&M.gl[col]), k = ld4(&M.kx[col]);
+            const float pb = M.pb[row], hi = M.gh[row], li = M.gl[row];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) f[r] = exp2_fast(fminf((hi - h[r]) + (li - l[r]), 120.0f)) * (k[r] * pb);
+        } else {
+            const int s = 16 * mi, e = 16 * j + 15;
+            f = ld4(&M.kc[col]) * (M.pr[row] * exp2_fast((M.gh[s] - M.gh[e]) + (M.gl[s] - M.gl[e])));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float x = j == mi && col + r > row ? 0.0f : p[r] * f[r];
+            a[r] = (_Float16)x;
+            b[r] = (_Float16)fmaf(p[r], f[r], -(float)a[r]);
+            if (j == mi && col + r > row) b[r] = (_Float16)0.0f;
+        }
+    }
+    Y.P_[0].put(mi, l15, j, g, a);
+    if (TP<T, C>::OP == 2) Y.P_[TP<T, C>::OP - 1].put(mi, l15, j, g, b);
+}
+
+// block (mi, j) of T, transposed, times s
+template <class T, int C>
+__device__ __forceinline__ void put_t(TP<T, C>& Y, const f32x4& t, float s, int mi, int j, int l15, int g) {
+    h4 a, b;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        a[r] = (_Float16)(t[r] * s);
+        b[r] = (_Float16)fmaf(t[r], s, -(float)a[r]);
+    }
+    Y.T_[0].put(mi, l15, j, g, a);
+    Y.T_[1].put(mi, l15, j, g, b);
+}
+
+// the inverses of the diagonal blocks by one wave, a column per lane, by substitution from the top
+template <int C>
+__device__ __forceinline__ void invert_diagonal(const TriA<C>& A, Diag<C>& D, int g, int l15) {
+    const int k = g & (C / 16 - 1), b = 16 * k;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = i == l15 ? 1.0f : 0.0f;
+#pragma unroll
+    for (int j = 0; j < 15; ++j) {
+        asm volatile("" : "+v"(x[j]) : : "memory");  // not all of A in registers at once
+#pragma unroll
+        for (int q = (j + 1) / 4; q < 4; ++q) {
+            const f32x4 a = ld4(&A.A[b + j][b + 4 * q]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (4 * q + r > j) x[4 * q + r] = fmaf(-a[r], x[j], x[4 * q + r]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&D.D[k][l15][4 * q]) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+}
+
+// Everything of a staged chunk of 64 that needs no state, by four waves.  Starts
+// and ends with the workgroup together.
 template <class T, int NKT>
-__device__ __forceinline__ void make_tp(const KQ<T, NKT>& X, TP<T>& Y, Make& M, TriA& A, int wave, int lane, int nt) {
-    constexpr int KP = KQ<T, NKT>::KP, KS = KQ<T, NKT>::KS;
-    Diag& D = *reinterpret_cast<Diag*>(Y.T_);
+__device__ __forceinline__ void make_tp(const KQ<T, NKT, 64>& X, TP<T, 64>& Y, Make<64>& M, TriA<64>& A, int wave, int lane) {
+    constexpr int KP = KQ<T, NKT, 64>::KP, OP = TP<T, 64>::OP;
+    Diag<64>& D = *reinterpret_cast<Diag<64>*>(Y.T_);
     const int l15 = lane & 15, g = lane >> 4;
     f32x4 acc[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        if (j <= wave) acc[j] = dot_tile<NKT, KP, KS>(X.K, X.K, wave, j, l15, g);
-    {
-        const int i = lane, s = i & ~15, e = i | 15;
-        const float h = M.gh[i], l = M.gl[i], kx = M.kx[i];
-        if (wave == 0) {
-            const float b = Y.beta[i] * kx, r = exp2_fast((h - M.gh[s]) + (l - M.gl[s]));
-            M.ab[i] = b;
-            M.ar[i] = b * r;
-            M.kc[i] = exp2_fast((M.gh[e] - h) + (M.gl[e] - l)) * kx;
-        } else if (wave == 1) {
-            // largest decay ratio of a row: e(G_i - min over j <= i of G_j); largest length of a key
-            float lo = h, kn = M.kn[i];
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const float y = __shfl_up(lo, d);
-                if (lane >= d) lo = fminf(lo, y);
-                kn = fmaxf(kn, __shfl_xor(kn, d));
-            }
-            float inv;
-            const float qx = M.qx[i], sc = scale_of(M.qn[i] * kn * exp2_fast(fminf(h - lo, 120.0f)), inv);
-            Y.pi[i] = inv;
-            M.pb[i] = qx * sc;
-            M.pr[i] = qx * sc * exp2_fast((h - M.gh[s]) + (l - M.gl[s]));
-        } else if (wave == 2) {
-            const float up = exp2_fast(h);
-            Y.fx[i] = Y.beta[i] * up * kx;
-            Y.fq[i] = up * M.qx[i];
-            const float fk = exp2_fast((M.gh[C - 1] - h) + (M.gl[C - 1] - l)) * kx;
-            Y.fk[i] = fk;
-            const float m = wave_max(fk), b = wave_max(fabsf(Y.beta[i]));
-            const float x = wave_max(fabsf(Y.beta[i]) * up * M.kn[i]) * sqrtf(32.0f * NKT);
-            if (i == C - 1) Y.all = up, Y.fkmax = m, Y.bmax = b, Y.xmax = x;
-        }
-    }
+        if (j <= wave) acc[j] = dot_tile<NKT, KP>(X.K, X.K, wave, j, l15, g);
+    if (wave < 3) make_factors<NKT>(X, Y, M, wave, lane);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (j > wave) continue;
-        const int col = 16 * j + l15, row = 16 * wave + 4 * g;
-        f32x4 f;
-        if (j == wave) {
-            const f32x4 h = ld4(&M.gh[row]), l = ld4(&M.gl[row]), b = ld4(&M.ab[row]);
-            const float hj = M.gh[col], lj = M.gl[col], kj = M.kx[col];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) f[r] = exp2_fast(fminf((h[r] - hj) + (l[r] - lj), 120.0f)) * (b[r] * kj);
-        } else {
-            const float k = M.kc[col] * exp2_fast(M.gh[16 * wave] - M.gh[16 * j + 15]);
-            f = ld4(&M.ar[row]) * k;
-        }
-        *reinterpret_cast<f32x4*>(&A.A[col][row]) = acc[j] * f;
+        put_a(M, A, acc[j], wave, j, l15, g);
     }
     __syncthreads();
     if (wave == 0) {
-        // the four diagonal blocks, a column of the inverse per lane, by substitution from the top
-        const int b = 16 * g;
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = i == l15 ? 1.0f : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 15; ++j) {
-#pragma unroll
-            for (int q = (j + 1) / 4; q < 4; ++q) {
-                const f32x4 a = ld4(&A.A[b + j][b + 4 * q]);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (4 * q + r > j) x[4 * q + r] = fmaf(-a[r], x[j], x[4 * q + r]);
-            }
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&D.D[g][l15][4 * q]) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+        invert_diagonal(A, D, g, l15);
     } else {
-        // P meanwhile: rows of tile 3, 2, and 1 with 0; as K Q^T, so that a lane has 4 frames of a row
+        // P meanwhile: rows of tile 3, 2, and 1 with 0
         const int first = wave == 1 ? 3 : wave == 2 ? 2 : 0, last = wave == 3 ? 1 : first;
-        for (int mi = first; mi <= last && mi < nt; ++mi) {
-            const int row = 16 * mi + l15;
-            const float pb = M.pb[row], pr = M.pr[row], hi_ = M.gh[row], li = M.gl[row], hs = M.gh[16 * mi];
-            for (int j = 0; j <= (mi | 1); ++j) {
-                h4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-                if (j <= mi) {
-                    const f32x4 p = dot_tile<NKT, KP, KS>(X.K, X.Q, j, mi, l15, g);
-                    const int col = 16 * j + 4 * g;
-                    f32x4 f;
-                    if (j == mi) {
-                        const f32x4 h = ld4(&M.gh[col]), l = ld4(&M.gl[col]), k = ld4(&M.kx[col]);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            f[r] = col + r <= row ? exp2_fast(fminf((hi_ - h[r]) + (li - l[r]), 120.0f)) * (k[r] * pb) : 0.0f;
-                    } else {
-                        f = ld4(&M.kc[col]) * (pr * exp2_fast(hs - M.gh[16 * j + 15]));
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float x = j == mi && col + r > row ? 0.0f : p[r] * f[r];
-                        a[r] = (_Float16)x;
-                        b[r] = (_Float16)(x - (float)a[r]);
-                    }
-                }
-                Y.P_[0].put(mi, l15, j, g, a);
-                if (TP<T>::OP == 2) Y.P_[TP<T>::OP - 1].put(mi, l15, j, g, b);
-            }
-        }
+        for (int mi = first; mi <= last; ++mi)
+            for (int j = 0; j <= (mi | 1); ++j)
+                put_p(Y, M, j <= mi ? dot_tile<NKT, KP>(X.K, X.Q, j, mi, l15, g) : f32x4{0, 0, 0, 0}, mi, j, l15, g);
     }
     __syncthreads();
     // block row i = wave of T, transposed: N_ij = -T_jj^T sum over j < k <= i of A_kj^T N_ik, in 32 bits
@@ -392,7 +445,7 @@ __device__ __forceinline__ void make_tp(const KQ<T, NKT>& X, TP<T>& Y, Make& M, 
 #pragma unroll
     for (int j = 3; j >= 0; --j) {
         t[j] = f32x4{0, 0, 0, 0};
-        if (j > wave || wave >= nt) continue;
+        if (j > wave) continue;
         if (j == wave) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) t[j][r] = D.D[j][4 * g + r][l15];
@@ -412,24 +465,40 @@ __device__ __forceinline__ void make_tp(const KQ<T, NKT>& X, TP<T>& Y, Make& M, 
         m = amax4(m, t[j]);
     }
     __syncthreads();
-    if (wave < nt) {
+    {
         float inv;
         const float s = scale_of(wave_max(m), inv);
         if (lane == 0) Y.ti[wave] = inv;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (j > (wave | 1)) continue;
-            h4 a, b;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                a[r] = (_Float16)(t[j][r] * s);
-                b[r] = (_Float16)fmaf(t[j][r], s, -(float)a[r]);
-            }
-            Y.T_[0].put(wave, l15, j, g, a);
-            Y.T_[1].put(wave, l15, j, g, b);
-        }
+        for (int j = 0; j < 4; ++j)
+            if (j <= (wave | 1)) put_t(Y, t[j], s, wave, j, l15, g);
     }
     __syncthreads();
+}
+
+// T of a chunk of 32 by one wave: both diagonal inverses, then N_10 = -T_00^T A_10^T T_11^T
+template <class T>
+__device__ __forceinline__ void make_t(TP<T, 32>& Y, const TriA<32>& A, int lane) {
+    const int l15 = lane & 15, g = lane >> 4;
+    Diag<32>& D = *reinterpret_cast<Diag<32>*>(Y.T_);
+    invert_diagonal(A, D, g, l15);
+    asm volatile("" ::: "memory");  // LDS keeps its order within a wave, the compiler has to
+    f32x4 t0, t1, y = {0, 0, 0, 0}, t = {0, 0, 0, 0};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t0[r] = D.D[0][4 * g + r][l15], t1[r] = D.D[1][4 * g + r][l15];
+    const f32x4 a = ld4(&A.A[l15][16 + 4 * g]), d = ld4(&D.D[0][l15][4 * g]);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], t1[r], y, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t = __builtin_amdgcn_mfma_f32_16x16x4f32(-d[r], y[r], t, 0, 0, 0);
+    float inv;
+    const float s = scale_of(wave_max(amax4(amax4(amax4(0.0f, t0), t1), t)), inv);
+    if (lane == 0) Y.ti[0] = inv;
+    put_t(Y, t0, s, 0, 0, l15, g);
+    put_t(Y, f32x4{0, 0, 0, 0}, s, 0, 1, l15, g);
+    put_t(Y, t, s, 1, 0, l15, g);
+    put_t(Y, t1, s, 1, 1, l15, g);
 }
 
 // accumulator tile n of 16 staged rows of v
@@ -447,232 +516,210 @@ __device__ __forceinline__ f32x4 tile_of(const T (*V)[VS], int n, int l15, int g
     return v;
 }
 
-// The products with the state for one chunk of nt live tiles of 16 frames: this
-// wave's columns.  S holds the state times 1 / sinv, a power of two; between()
-// runs once the state's 16-bit parts are dead (it holds the next chunk's loads).
-template <class T, int NKT, int NB, class F>
-__device__ __forceinline__ void advance(const KQ<T, NKT>& X, const TP<T>& Y, T (*V)[Geo<T, NKT, NB>::VS],
-                                        f32x4 (&S)[2 * NKT][NB], float& sinv, int lane, int nt, const F& between) {
+// K S0 and R of a chunk of 32 with nt live tiles of 16 frames, for this wave's
+// columns; with LOW outputs also Q S0, whose high part outlasts R otherwise (in
+// fewer registers).  S holds the state times 1 / sinv, a power of two.
+template <class T, int NKT, int NB>
+struct Chunk {
     using G = Geo<T, NKT, NB>;
-    constexpr bool LOW = G::OP == 2;
-    const int l15 = lane & 15, g = lane >> 4;
-    const f32x4 zero = {0, 0, 0, 0};
-    f32x4 R[4][NB], O[4][NB];
-    float smax = 0.0f, rmax = 0.0f;
-    {
-        h8 hi[NKT][NB], lo[NKT][NB];
+    static constexpr bool LOW = G::OP == 2;
+    f32x4 R[2][NB], O[LOW ? 2 : 1][NB];
+    h8 shi[NKT][NB];
+    float smax, rmax, sout;
+
+    __device__ __forceinline__ void first(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], const f32x4 (&S)[2 * NKT][NB],
+                                          float sinv, int lane, int nt) {
+        const int l15 = lane & 15, g = lane >> 4;
+        const f32x4 zero = {0, 0, 0, 0};
+        h8 lo[NKT][NB];
+        smax = rmax = 0.0f;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
             for (int t = 0; t < 2 * NKT; ++t) smax = amax4(smax, S[t][n]);
         smax = wave_max(smax);
         float inv;
-        const float s = scale_of(smax, inv);
+        const float sc = scale_of(smax, inv);
         inv *= sinv;
+        sout = inv;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int t = 0; t < NKT; ++t) split<true>(S[2 * t][n], S[2 * t + 1][n], all4(s), all4(s), hi[t][n], lo[t][n]);
+            for (int t = 0; t < NKT; ++t) split<true>(S[2 * t][n], S[2 * t + 1][n], all4(sc), all4(sc), shi[t][n], lo[t][n]);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int m = 0; m < 2; ++m) {
             if (m >= nt) {
 #pragma unroll
                 for (int n = 0; n < NB; ++n) R[m][n] = zero;
                 continue;
             }
-            no_hoist();
             f32x4 x[NB], o[NB];
 #pragma unroll
             for (int s = 0; s < NKT; ++s) {
                 const int c = 32 * s + 8 * g;
                 const h8 k = *reinterpret_cast<const h8*>(&X.K[0][16 * m + l15][c]);
-                const h8 q = *reinterpret_cast<const h8*>(&X.Q[0][16 * m + l15][c]);
+                h8 q, kl, ql;
+                if (LOW) q = *reinterpret_cast<const h8*>(&X.Q[0][16 * m + l15][c]);
+                if (G::KP == 2) {
+                    kl = *reinterpret_cast<const h8*>(&X.K[G::KP - 1][16 * m + l15][c]);
+                    ql = *reinterpret_cast<const h8*>(&X.Q[G::KP - 1][16 * m + l15][c]);
+                }
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    x[n] = mma(k, lo[s][n], mma(k, hi[s][n], s ? x[n] : zero));
-                    o[n] = mma(q, hi[s][n], s ? o[n] : zero);
-                    if (LOW) o[n] = mma(q, lo[s][n], o[n]);
-                }
-                if (G::KP == 2) {
-                    const h8 kl = *reinterpret_cast<const h8*>(&X.K[G::KP - 1][16 * m + l15][c]);
-                    const h8 ql = *reinterpret_cast<const h8*>(&X.Q[G::KP - 1][16 * m + l15][c]);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        x[n] = mma(kl, hi[s][n], x[n]);
-                        o[n] = mma(ql, hi[s][n], o[n]);
+                    x[n] = mma(k, lo[s][n], mma(k, shi[s][n], s ? x[n] : zero));
+                    if (LOW) o[n] = mma(q, lo[s][n], mma(q, shi[s][n], s ? o[n] : zero));
+                    if (G::KP == 2) {
+                        x[n] = mma(kl, shi[s][n], x[n]);
+                        o[n] = mma(ql, shi[s][n], o[n]);
                     }
                 }
             }
-            const f32x4 b = ld4(&Y.beta[16 * m + 4 * g]);
-            const f32x4 fx = ld4(&Y.fx[16 * m + 4 * g]) * -inv, fq = ld4(&Y.fq[16 * m + 4 * g]) * inv;
+            const f32x4 b = ld4(&Y.beta[16 * m + 4 * g]), fx = ld4(&Y.fx[16 * m + 4 * g]) * -inv;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 const f32x4 v = tile_of<T>(V + 16 * m, n, l15, g) * b;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) R[m][n][r] = fmaf(fx[r], x[n][r], v[r]);
-                O[m][n] = o[n] * fq;
+                if (LOW) O[LOW ? m : 0][n] = o[n] * (ld4(&Y.fq[16 * m + 4 * g]) * inv);
                 rmax = amax4(rmax, R[m][n]);
             }
         }
     }
-    between();
-    // U = u ti rinv, where |u| is at most 64 products of 2^30
-    f32x4 u[4][NB];
-    float rinv, ti[4], tmax = 0.0f;
-    {
-        h8 hi[2][NB], lo[2][NB];
-        const float s = scale_of(wave_max(rmax), rinv);
+
+    // U, the output (into V) and the state after the chunk
+    __device__ __forceinline__ void second(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], f32x4 (&S)[2 * NKT][NB],
+                                           float& sinv, int lane, int nt) {
+        const int l15 = lane & 15, g = lane >> 4;
+        const f32x4 zero = {0, 0, 0, 0};
+        f32x4 u[2][NB];  // U = u ti rinv, where |u| is at most 32 products of 2^30
+        float rinv;
+        h8 hi[NB], lo[NB];
+        const float rs = scale_of(wave_max(rmax), rinv);
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < NB; ++n) split<true>(R[0][n], R[1][n], all4(rs), all4(rs), hi[n], lo[n]);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) split<true>(R[2 * t][n], R[2 * t + 1][n], all4(s), all4(s), hi[t][n], lo[t][n]);
+        for (int m = 0; m < 2; ++m) {
+            const h8 th = Y.T_[0].operand(m, l15, 0, g), tl = Y.T_[1].operand(m, l15, 0, g);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            ti[m] = 0.0f;
-            if (m >= nt) {
-#pragma unroll
-                for (int n = 0; n < NB; ++n) u[m][n] = zero;
-                continue;
-            }
-            no_hoist();
-            ti[m] = Y.ti[m];
-            tmax = fmaxf(tmax, ti[m]);
-#pragma unroll
-            for (int s = 0; s <= m / 2; ++s) {
-                const h8 th = Y.T_[0].operand(m, l15, s, g), tl = Y.T_[1].operand(m, l15, s, g);
-#pragma unroll
-                for (int n = 0; n < NB; ++n) u[m][n] = mma(tl, hi[s][n], mma(th, lo[s][n], mma(th, hi[s][n], s ? u[m][n] : zero)));
-            }
+            for (int n = 0; n < NB; ++n) u[m][n] = mma(tl, hi[n], mma(th, lo[n], mma(th, hi[n], zero)));
         }
-    }
-    // to below 2^14: U = (u ti c) rinv / c
-    const float cinv = tmax * 0x1p22f, c = 1.0f / cinv;
-    // O += P U
-    {
-        h8 hi[2][NB], lo[2][NB];
+        const float ti = Y.ti[0] * rinv;  // u to below 2^14: times 2^-22
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < NB; ++n) split<LOW>(u[0][n], u[1][n], all4(0x1p-22f), all4(0x1p-22f), hi[n], lo[n]);
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-                split<LOW>(u[2 * t][n], u[2 * t + 1][n], all4(ti[2 * t] * c), all4(ti[2 * t + 1] * c), hi[t][n], lo[t][n]);
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
+        for (int m = 0; m < 2; ++m) {
             if (m >= nt) continue;
-            no_hoist();
-            f32x4 o[NB];
+            const h8 ph = Y.P_[0].operand(m, l15, 0, g);
+            f32x4 o[NB], qs[NB];
 #pragma unroll
-            for (int s = 0; s <= m / 2; ++s) {
-                const h8 ph = Y.P_[0].operand(m, l15, s, g);
-#pragma unroll
-                for (int n = 0; n < NB; ++n) o[n] = mma(ph, hi[s][n], s ? o[n] : zero);
-                if (LOW) {
-                    const h8 pl = Y.P_[G::OP - 1].operand(m, l15, s, g);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) o[n] = mma(pl, hi[s][n], mma(ph, lo[s][n], o[n]));
-                }
+            for (int n = 0; n < NB; ++n) {
+                o[n] = mma(ph, hi[n], zero);
+                if (LOW) o[n] = mma(Y.P_[G::OP - 1].operand(m, l15, 0, g), hi[n], mma(ph, lo[n], o[n]));
             }
-            const f32x4 pi = ld4(&Y.pi[16 * m + 4 * g]) * (rinv * cinv);
+            if (!LOW)
+#pragma unroll
+                for (int s = 0; s < NKT; ++s) {
+                    const h8 q = *reinterpret_cast<const h8*>(&X.Q[0][16 * m + l15][32 * s + 8 * g]);
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) qs[n] = mma(q, shi[s][n], s ? qs[n] : zero);
+                }
+            const f32x4 pi = ld4(&Y.pi[16 * m + 4 * g]) * (ti * 0x1p22f), fq = ld4(&Y.fq[16 * m + 4 * g]) * sout;
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    V[16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], O[m][n][r]);
+                    V[16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], LOW ? O[LOW ? m : 0][n][r] : fq[r] * qs[n][r]);
         }
-    }
-    // S1, accumulated onto the decayed state in the scale s of U fk; where U is next to nothing, in 2^13 of the decayed
-    // state's own, so that neither leaves its range (2^100 at most: the state's factor stays finite)
-    {
-        h8 hi[2][NB], lo[2][NB];
+        // S1, accumulated onto the decayed state in the scale s of U fk; where U is next to nothing, in 2^13 of the
+        // decayed state's own, so that neither leaves its range (2^100 at most: the state's factor stays finite)
         const float all = Y.all;
         float zi, li;
-        const float z = scale_of(Y.fkmax, zi) * 0x1p-14f, low = scale_of(fmaxf(smax * sinv * (all * 0x1p-13f), 0x1p-86f), li);
-        const float s = fminf(c * z / rinv, low), k = s * rinv;  // true U fk times s = u ti fk k
-        f32x4 f[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) f[t] = ld4(&Y.fk[16 * t + 4 * g]) * (ti[t] * k);
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int t = 0; t < 2; ++t) split<true>(u[2 * t][n], u[2 * t + 1][n], f[2 * t], f[2 * t + 1], hi[t][n], lo[t][n]);
-        const float d = all * s * sinv;
+        const float z = scale_of(Y.fkmax, zi) * 0x1p-36f, low = scale_of(fmaxf(smax * sinv * (all * 0x1p-13f), 0x1p-86f), li);
+        const float s = fminf(z / ti, low), d = all * s * sinv;  // true U fk times s = u fk (ti s)
         sinv = 1.0f / s;
+        const f32x4 f0 = ld4(&Y.fk[4 * g]) * (ti * s), f1 = ld4(&Y.fk[16 + 4 * g]) * (ti * s);
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < NB; ++n) {
+            split<true>(u[0][n], u[1][n], f0, f1, hi[n], lo[n]);
 #pragma unroll
             for (int t = 0; t < 2 * NKT; ++t) S[t][n] *= d;
+        }
 #pragma unroll
         for (int t = 0; t < 2 * NKT; ++t) {
-            if (t & 1) no_hoist();
+            const int row = 4 * g + (l15 >> 2), col = 32 * (t >> 1) + 8 * (l15 & 3) + 4 * (t & 1);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                if (2 * s >= nt) continue;
-                const int row = 32 * s + 4 * g + (l15 >> 2), col = 32 * (t >> 1) + 8 * (l15 & 3) + 4 * (t & 1);
-                const auto kt = [&](int part) {
-                    const s4 a = read_tr(&X.K[part][row][col]), b = read_tr(&X.K[part][row + 16][col]);
-                    const h4 x = __builtin_bit_cast(h4, a), y = __builtin_bit_cast(h4, b);
-                    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-                };
-                const h8 k = kt(0);
+            for (int part = 0; part < G::KP; ++part) {
+                const h4 x = __builtin_bit_cast(h4, read_tr(&X.K[part][row][col]));
+                const h4 y = __builtin_bit_cast(h4, read_tr(&X.K[part][row + 16][col]));
+                const h8 k = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-                for (int n = 0; n < NB; ++n) S[t][n] = mma(k, lo[s][n], mma(k, hi[s][n], S[t][n]));
-                if (G::KP == 2) {
-                    const h8 kl = kt(G::KP - 1);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) S[t][n] = mma(kl, hi[s][n], S[t][n]);
+                for (int n = 0; n < NB; ++n) {
+                    S[t][n] = mma(k, hi[n], S[t][n]);
+                    if (part == 0) S[t][n] = mma(k, lo[n], S[t][n]);
                 }
             }
         }
     }
-}
+};
 
-// f(t, j, r, at, in) for element r of accumulator tile (t, j): its place in the
-// head's state, kept inside it, and whether it is one of it
+// f(t, j, r, base, at, in) for element r of accumulator tile (t, j): its place base
+// + at in the head's state (base the same for all lanes), kept inside it, and
+// whether it is one of it
 template <int NKT, int NB, class F>
 __device__ __forceinline__ void each_state(const nnsp_delta_args& a, int c0, int lane, const F& f) {
     const int l15 = lane & 15, g = lane >> 4;
-    const bool whole = a.dk == 32 * NKT && c0 + 16 * NB <= a.dv;
+    if (a.dk == 32 * NKT && c0 + 16 * NB <= a.dv) {
+        const unsigned at = 8 * g * a.dv + l15;
 #pragma unroll
-    for (int j = 0; j < NB; ++j)
+        for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int t = 0; t < 2 * NKT; ++t)
+            for (int t = 0; t < 2 * NKT; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 32 * (t >> 1) + 4 * (t & 1) + r, col = c0 + 16 * j;  // of lane 0
-                if (whole) f(t, j, r, row * a.dv + col + (8 * g * a.dv + l15), true);
-                else f(t, j, r, min(row + 8 * g, a.dk - 1) * a.dv + min(col + l15, a.dv - 1), row + 8 * g < a.dk && col + l15 < a.dv);
-            }
+                for (int r = 0; r < 4; ++r) f(t, j, r, (32 * (t >> 1) + 4 * (t & 1) + r) * a.dv + c0 + 16 * j, at, true);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int t = 0; t < 2 * NKT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 32 * (t >> 1) + 4 * (t & 1) + r + 8 * g, col = c0 + 16 * j + l15;
+                    f(t, j, r, 0, (unsigned)(min(row, a.dk - 1) * a.dv + min(col, a.dv - 1)), row < a.dk && col < a.dv);
+                }
+    }
 }
 
 // A chunk's rows of q, k, g and beta of one stream and head: from global memory to
 // registers, from there to LDS with what make_tp starts from.
-template <class T, int NKT, bool FAST>
+template <class T, int NKT, int C, int PR, bool FAST>
 struct Rows {
     const T *qp, *kp;
     const float *gp, *bp;
     long long qs, ks, gs, bs;
-    RawRows<T, NKT> rq, rk;
+    RawRows<T, NKT, PR> rq, rk;
     float rg, rb;
-    int row, quarter, lane, wave;
+    int row, part, lane, wave;
 
     // this thread's place in the chunk at frame t0
     __device__ __forceinline__ Rows(const nnsp_delta_args& a, int s, int h, long long t0, int tid, int wv)
-        : row(tid >> 2), quarter(tid & 3), lane(tid & 63), wave(wv) {
+        : row(tid / PR), part(tid % PR), lane(tid & 63), wave(wv) {
         const int hk = h / (a.value_heads / a.key_heads);
-        qp = (const T*)a.q + s * a.q_stride[0] + hk * a.q_stride[2] + (t0 + row) * a.q_stride[1] + quarter * 8;
-        kp = (const T*)a.k + s * a.k_stride[0] + hk * a.k_stride[2] + (t0 + row) * a.k_stride[1] + quarter * 8;
-        gp = a.g ? a.g + s * a.g_stride[0] + h * a.g_stride[2] + (t0 + lane) * a.g_stride[1] : nullptr;
-        bp = a.beta + s * a.beta_stride[0] + h * a.beta_stride[2] + (t0 + lane) * a.beta_stride[1];
+        qp = (const T*)a.q + s * a.q_stride[0] + hk * a.q_stride[2] + (t0 + row) * a.q_stride[1] + part * 8;
+        kp = (const T*)a.k + s * a.k_stride[0] + hk * a.k_stride[2] + (t0 + row) * a.k_stride[1] + part * 8;
+        const long long t = t0 + (lane & (C - 1));
+        gp = a.g ? a.g + s * a.g_stride[0] + h * a.g_stride[2] + t * a.g_stride[1] : nullptr;
+        bp = a.beta + s * a.beta_stride[0] + h * a.beta_stride[2] + t * a.beta_stride[1];
         qs = C * a.q_stride[1], ks = C * a.k_stride[1], gs = C * a.g_stride[1], bs = C * a.beta_stride[1];
     }
     // left: live frames from the chunk's first on
     __device__ __forceinline__ void fetch(int dk, int left) {
-        fetch_rows<T, NKT, FAST>(rk, kp, quarter, dk, row < left);
-        fetch_rows<T, NKT, FAST>(rq, qp, quarter, dk, row < left);
+        fetch_rows<FAST>(rk, kp, part, dk, row < left);
+        fetch_rows<FAST>(rq, qp, part, dk, row < left);
         fetch_gates(left);
     }
     __device__ __forceinline__ void fetch_gates(int left) {
         rg = rb = 0.0f;
-        if (wave == 0 && lane < left) {
+        if (wave == 0 && (lane & (C - 1)) < left) {
             if (gp) rg = *gp;
             rb = *bp;
         }
@@ -681,40 +728,42 @@ struct Rows {
         qp += qs, kp += ks, bp += bs;
         if (gp) gp += gs;
     }
-    __device__ __forceinline__ void stage(const nnsp_delta_args& a, KQ<T, NKT>& X, TP<T>& Y, Make& M) {
-        constexpr int KP = KQ<T, NKT>::KP, KS = KQ<T, NKT>::KS;
+    __device__ __forceinline__ void stage(const nnsp_delta_args& a, KQ<T, NKT, C>& X, TP<T, C>& Y, Make<C>& M) {
+        constexpr int KP = KQ<T, NKT, C>::KP;
         float ss, inv, f;
         // a row of zeros has inv 0 and no part in anything, whatever its norm's reciprocal is (v_rsq_f32: one unit)
-        inv = stage_rows<T, NKT, KP, KS>(rk, X.K, row, quarter, ss);
+        inv = stage_rows<KP>(rk, X.K, row, part, ss);
         f = a.l2norm ? __builtin_amdgcn_rsqf(ss + a.eps) : 1.0f;
-        if (quarter == 0) M.kx[row] = inv > 0.0f ? inv * f : 0.0f, M.kn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * f : 0.0f;
-        inv = stage_rows<T, NKT, KP, KS>(rq, X.Q, row, quarter, ss);
+        if (part == 0) M.kx[row] = inv > 0.0f ? inv * f : 0.0f, M.kn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * f : 0.0f;
+        inv = stage_rows<KP>(rq, X.Q, row, part, ss);
         f = a.scale * (a.l2norm ? __builtin_amdgcn_rsqf(ss + a.eps) : 1.0f);
-        if (quarter == 0) M.qx[row] = inv > 0.0f ? inv * f : 0.0f, M.qn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * fabsf(f) : 0.0f;
+        if (part == 0) M.qx[row] = inv > 0.0f ? inv * f : 0.0f, M.qn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * fabsf(f) : 0.0f;
         stage_gates(Y, M);
     }
-    __device__ __forceinline__ void stage_gates(TP<T>& Y, Make& M) {
+    __device__ __forceinline__ void stage_gates(TP<T, C>& Y, Make<C>& M) {
         if (wave == 0) {
             // running sum of g in 64 bits, in units of log2, kept as two floats: differences of near frames stay exact
             double x = (double)decay_log(rg) * 1.4426950408889634;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
+            for (int d = 1; d < C; d <<= 1) {
                 const double y = __shfl_up(x, d);
-                if (lane >= d) x += y;
+                if ((lane & (C - 1)) >= d) x += y;
             }
-            M.gh[lane] = (float)x;
-            M.gl[lane] = (float)(x - (double)(float)x);
-            Y.beta[lane] = rb;
+            const int i = lane & (C - 1);  // of a chunk of 32, both halves of the wave alike
+            M.gh[i] = (float)x;
+            M.gl[i] = (float)(x - (double)(float)x);
+            Y.beta[i] = rb;
         }
     }
 };
 
 // The same for FR frames of 16 NB columns of v by one wave, and for out the other way.
-template <class T, int NKT, int NB, bool FAST, int FR>
+template <class T, int NKT, int NB, bool FAST, int FR, int C>
 struct Cols {
     static constexpr int LPR = 2 * NB, ROWS = 64 / LPR < FR ? 64 / LPR : FR, N = FR / ROWS, VS = Geo<T, NKT, NB>::VS;
     typedef typename Vec<T, 8>::raw V8;
     typedef typename Vec<T, 8>::type V8u;
+    typedef V8 V8s __attribute__((aligned(8)));  // in LDS
     const T* vp;
     T* op;
     long long vs, os, vc, oc;
@@ -757,7 +806,7 @@ struct Cols {
     __device__ __forceinline__ void stage(T (*V)[VS]) const {
         if (row < ROWS)
 #pragma unroll
-            for (int i = 0; i < N; ++i) *reinterpret_cast<V8*>(&V[row + ROWS * i][col]) = x[i];
+            for (int i = 0; i < N; ++i) *reinterpret_cast<V8s*>(&V[row + ROWS * i][col]) = x[i];
         // the wave's own columns: LDS keeps its order within a wave, the compiler has to
         asm volatile("" ::: "memory");
     }
@@ -767,7 +816,7 @@ struct Cols {
         for (int i = 0; i < N; ++i) {
             const bool live = row < ROWS && row + ROWS * i < frames;
             if (FAST) {
-                if (live && left > 0) *reinterpret_cast<V8u*>(op) = *reinterpret_cast<const V8*>(&V[row + ROWS * i][col]);
+                if (live && left > 0) *reinterpret_cast<V8u*>(op) = *reinterpret_cast<const V8s*>(&V[row + ROWS * i][col]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -783,60 +832,79 @@ __device__ __forceinline__ int frames_of(const nnsp_delta_args& a, int s) {
     return a.lens ? max(0, min(a.lens[s], a.n_frames)) : a.n_frames;
 }
 
-// Many streams: a workgroup per stream, head and 64 NB columns goes through its
-// chunks alone, and the workgroups of a CU fill each other's waits.
+// Many streams: a workgroup per stream, head and 16 NB NW columns goes through its
+// chunks of 32 alone, and the workgroups of a CU fill each other's waits.
 // FAST: dk and dv are multiples of 8.
-template <class T, int NKT, int NB, bool FAST>
-__global__ __launch_bounds__(256, 2) void delta_chunk_kernel(const nnsp_delta_args a) {
+template <class T, int NKT, int NB, int NW, bool FAST>
+__global__ __launch_bounds__(64 * NW, (Geo<T, NKT, NB>::WIDE || NB == 2 ? 2 : 3)) void delta_chunk_kernel(const nnsp_delta_args a) {
     using G = Geo<T, NKT, NB>;
     struct Lds {
-        KQ<T, NKT> X;
-        TP<T> Y;
-        Make M;
-        union {
-            TriA A;                        // until T is done
-            alignas(16) T V[4][C][G::VS];  // from then on: each wave's columns of v, then of out
-        };
+        KQ<T, NKT, CF> X;
+        TP<T, CF> Y;
+        Make<CF> M;
+        TriA<CF> A;
+        alignas(16) T V[NW][CF][G::VS];  // each wave's columns of v, then of out
     };
     __shared__ Lds L;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int ncb = (a.dv + G::W - 1) / G::W;
+    const int ncb = (a.dv + 16 * NB * NW - 1) / (16 * NB * NW);
     const int cb = blockIdx.x % ncb, h = (blockIdx.x / ncb) % a.value_heads, s = blockIdx.x / ncb / a.value_heads;
     const int n = frames_of(a, s);
-    const int c0 = cb * G::W + wave * 16 * NB;  // first column of this wave
+    const int c0 = (cb * NW + wave) * 16 * NB;  // first column of this wave
     const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
+    const int role = (wave + blockIdx.x) & (NW - 1);  // who does what of the tiles: another SIMD each workgroup
 
     f32x4 S[2 * NKT][NB];
     float sinv = 1.0f;
-    each_state<NKT, NB>(a, c0, lane, [&](int t, int j, int r, int at, bool in) {
-        const float x = a.state_in ? (a.state_in + so)[at] : 0.0f;
+    const float* sp = a.state_in + so;
+    each_state<NKT, NB>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
+        const float x = a.state_in ? (sp + base)[at] : 0.0f;
         S[t][j][r] = in ? x : 0.0f;
     });
-    Rows<T, NKT, FAST> rows(a, s, h, 0, tid, wave);
-    Cols<T, NKT, NB, FAST, C> cols(a, s, h, 0, c0, lane);
+    Rows<T, NKT, CF, 2 * NW, FAST> rows(a, s, h, 0, tid, wave);
+    Cols<T, NKT, NB, FAST, CF, CF> cols(a, s, h, 0, c0, lane);
     if (n > 0) {
         rows.fetch(a.dk, n);
         cols.fetch(n);
     }
-    for (int t0 = 0; t0 < n; t0 += C) {
-        const int left = n - t0, nt = min(4, (left + 15) >> 4);
+    for (int t0 = 0; t0 < n; t0 += CF) {
+        const int left = n - t0, nt = left > 16 ? 2 : 1, ln = here(lane), l15 = ln & 15, g = ln >> 4;
         rows.stage(a, L.X, L.Y, L.M);
-        __syncthreads();
-        make_tp<T, NKT>(L.X, L.Y, L.M, L.A, wave, here(lane), nt);
         cols.stage(L.V[wave]);
-        advance<T, NKT, NB>(L.X, L.Y, L.V[wave], S, sinv, here(lane), nt, [&] {
-            if (left <= C) return;
+        __syncthreads();
+        // the tiles of A ((0,0), (1,0), (1,1)) and of P, and the factors, which the tiles take afterwards
+        constexpr int KP = KQ<T, NKT, CF>::KP;
+        const int at = role, pt = NW == 4 ? (role == 3 ? 1 : role == 1 ? 3 : role) : role - 3;
+        f32x4 ta, tp;
+        if (at < 3) ta = dot_tile<NKT, KP>(L.X.K, L.X.K, at > 0, at > 1, l15, g);
+        if (pt >= 0 && pt < 3) tp = dot_tile<NKT, KP>(L.X.K, L.X.Q, pt > 1, pt > 0, l15, g);
+        if (role == 1) make_factors<NKT>(L.X, L.Y, L.M, 0, ln);
+        if (role == NW - 1) make_factors<NKT>(L.X, L.Y, L.M, 1, ln);
+        if (role == (NW == 4 ? 1 : 6)) make_factors<NKT>(L.X, L.Y, L.M, 2, ln);
+        __syncthreads();
+        if (at < 3) put_a(L.M, L.A, ta, at > 0, at > 1, l15, g);
+        if (pt >= 0 && pt < 3) put_p(L.Y, L.M, tp, pt > 0, pt > 1, l15, g);
+        if (pt == 0) put_p(L.Y, L.M, tp, 0, 1, l15, g);
+        __syncthreads();
+        if (role == 0) make_t(L.Y, L.A, ln);
+        Chunk<T, NKT, NB> c;
+        c.first(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
+        if (left > CF) {
             rows.next();
-            rows.fetch(a.dk, left - C);
-            cols.fetch(left - C);
-        });
+            rows.fetch(a.dk, left - CF);
+            cols.fetch(left - CF);
+        }
+        __syncthreads();
+        c.second(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
         cols.store(L.V[wave], left);
         __syncthreads();
     }
-    if (a.state_out)
-        each_state<NKT, NB>(a, c0, here(lane), [&](int t, int j, int r, int at, bool in) {
-            if (in) (a.state_out + so)[at] = S[t][j][r] * sinv;
+    if (a.state_out) {
+        float* sq = a.state_out + so;
+        each_state<NKT, NB>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
+            if (in) (sq + base)[at] = S[t][j][r] * sinv;
         });
+    }
 }
 
 // Few streams, many frames: T and P of all chunks at once, one workgroup each
@@ -861,10 +929,10 @@ __device__ __forceinline__ void copy_out(char* dst, const X& src, int tid) {
 template <class T, int NKT, bool FAST>
 __global__ __launch_bounds__(256, 2) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
     struct Lds {
-        KQ<T, NKT> X;
-        TP<T> Y;
-        Make M;
-        TriA A;
+        KQ<T, NKT, C> X;
+        TP<T, C> Y;
+        Make<C> M;
+        TriA<C> A;
     };
     __shared__ Lds L;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -872,19 +940,19 @@ __global__ __launch_bounds__(256, 2) void delta_prepare_kernel(const nnsp_delta_
     const int rep = a.value_heads / a.key_heads, h0 = hk * rep;
     const int t0 = (b.first + c) * C, left = frames_of(a, s) - t0;
     if (left <= 0) return;
-    Rows<T, NKT, FAST> rows(a, s, h0, t0, tid, wave);
+    Rows<T, NKT, C, 4, FAST> rows(a, s, h0, t0, tid, wave);
     rows.fetch(a.dk, left);
     rows.stage(a, L.X, L.Y, L.M);
     __syncthreads();
-    copy_out(b.kq + (((long long)s * a.key_heads + hk) * b.chunks + c) * sizeof(KQ<T, NKT>), L.X, tid);
+    copy_out(b.kq + (((long long)s * a.key_heads + hk) * b.chunks + c) * sizeof(KQ<T, NKT, C>), L.X, tid);
     for (int r = 0; r < rep; ++r) {
         if (r + 1 < rep) {
             if (rows.gp) rows.gp += a.g_stride[2];
             rows.bp += a.beta_stride[2];
             rows.fetch_gates(left);
         }
-        make_tp<T, NKT>(L.X, L.Y, L.M, L.A, wave, here(lane), 4);
-        copy_out(b.tp + (((long long)s * a.value_heads + h0 + r) * b.chunks + c) * sizeof(TP<T>), L.Y, tid);
+        make_tp(L.X, L.Y, L.M, L.A, wave, here(lane));
+        copy_out(b.tp + (((long long)s * a.value_heads + h0 + r) * b.chunks + c) * sizeof(TP<T, C>), L.Y, tid);
         if (r + 1 < rep) {
             __syncthreads();
             rows.stage_gates(L.Y, L.M);
@@ -906,8 +974,9 @@ __device__ __forceinline__ void copy_in(X& dst, const char* src, int wave, int w
 // a tile times its rows' factors, as half of the high and low B operand that it is part of
 template <bool LOW>
 __device__ __forceinline__ void put_part(h8 (*dst)[64], int lane, int half, const f32x4& x, const f32x4& s) {
-    typedef unsigned u2 __attribute__((ext_vector_type(2)));
-    const h4 hi = __builtin_bit_cast(h4, u2{pack(x[0], s[0], x[1], s[1]), pack(x[2], s[2], x[3], s[3])});
+    h4 hi;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) hi[i] = half_of(x[i], s[i]);
     reinterpret_cast<h4*>(&dst[0][lane])[half] = hi;
     if (LOW) {
         h4 lo;
@@ -927,8 +996,8 @@ struct Exchange {
 
 template <class T, int NKT, int NB, int BUFS>
 struct ScanLds {
-    KQ<T, NKT> X[BUFS];
-    TP<T> Y[BUFS];
+    KQ<T, NKT, C> X[BUFS];
+    TP<T, C> Y[BUFS];
     Exchange<NKT, NB> E;
     alignas(16) T V[4][16][Geo<T, NKT, NB>::VS];
 };
@@ -949,19 +1018,19 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
     constexpr int TPW = (2 * NKT + 3) / 4;  // state tiles of a wave
     __shared__ ScanLds<T, NKT, NB, BUFS> L;
     const int lane_ = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // streams and heads vary fastest: a multiple of 8 of them puts all workgroups of a head on one XCD and its L2
-    const unsigned rows = (unsigned)a.n_streams * a.value_heads;
-    const int cb = blockIdx.x / rows, row = blockIdx.x % rows, h = row % a.value_heads, s = row / a.value_heads;
-    const int hk = h / (a.value_heads / a.key_heads);
+    // streams and key heads vary fastest: with a multiple of 8 of them, all workgroups that read an image are on one XCD
+    const unsigned keys = (unsigned)a.n_streams * a.key_heads;
+    const int rep = a.value_heads / a.key_heads, hk = blockIdx.x % a.key_heads, s = blockIdx.x % keys / a.key_heads;
+    const int cb = blockIdx.x / keys / rep, h = hk * rep + blockIdx.x / keys % rep;
     const int n = min(frames_of(a, s) - b.first * C, b.chunks * C);  // frames in this slab
     if (wave >= 4) {
-        const char* kq = b.kq + ((long long)s * a.key_heads + hk) * b.chunks * sizeof(KQ<T, NKT>);
-        const char* tp = b.tp + ((long long)s * a.value_heads + h) * b.chunks * sizeof(TP<T>);
+        const char* kq = b.kq + ((long long)s * a.key_heads + hk) * b.chunks * sizeof(KQ<T, NKT, C>);
+        const char* tp = b.tp + ((long long)s * a.value_heads + h) * b.chunks * sizeof(TP<T, C>);
         const auto load = [&](int i) {
             copy_in(L.X[i], kq, wave - 4, 4, lane_);
             copy_in(L.Y[i], tp, wave - 4, 4, lane_);
-            kq += sizeof(KQ<T, NKT>);
-            tp += sizeof(TP<T>);
+            kq += sizeof(KQ<T, NKT, C>);
+            tp += sizeof(TP<T, C>);
         };
         if (n > 0) load(0);
         __syncthreads();
@@ -1012,12 +1081,12 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
     };
     float sbound = max4(L.E.smax);  // of |S|, the registers' values
 
-    Cols<T, NKT, NB, FAST, 16> cols(a, s, h, (long long)b.first * C + 16 * wave, c0, lane_);
+    Cols<T, NKT, NB, FAST, 16, C> cols(a, s, h, (long long)b.first * C + 16 * wave, c0, lane_);
     if (n > 0) cols.fetch(n - 16 * wave);
     for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= BUFS - 1) {
         const int lane = here(lane_), l15 = lane & 15, g = lane >> 4, left = n - t0;
-        const KQ<T, NKT>& X = L.X[i];
-        const TP<T>& Y = L.Y[i];
+        const KQ<T, NKT, C>& X = L.X[i];
+        const TP<T, C>& Y = L.Y[i];
         Exchange<NKT, NB>& E = L.E;
         // 1: the state's parts, and what bounds R
         float inv;
@@ -1028,7 +1097,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
 #pragma unroll
             for (int j = 0; j < TPW; ++j) {
                 const int t = wave * TPW + j;
-                if (t >= 2 * NKT) continue;
+                if (t >= 2 * NKT) continue;  // not a tile of the state; its registers are never handed on
 #pragma unroll
                 for (int k = 0; k < NB; ++k) {
                     put_part<true>(E.S[t >> 1][k], lane, t & 1, S[j][k], all4(sc));
@@ -1077,26 +1146,31 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
             }
         }
         if (left > C) cols.fetch(left - C - 16 * wave);
-        __syncthreads();
-        // 3: U of this wave's frames; see advance() for the scales
-        const float tmax = max4(Y.ti), cinv = tmax * 0x1p22f, c = 1.0f / cinv, all = Y.all;
+        // what the next steps take of the images and know of the scales (see advance()), before the waits
+        const float tmax = max4(Y.ti), cinv = tmax * 0x1p22f, c = 1.0f / cinv, all = Y.all, ti = Y.ti[wave];
         float zi, li;
         const float z = scale_of(Y.fkmax, zi) * 0x1p-14f, low = scale_of(fmaxf(smax * (all * 0x1p-13f), 0x1p-86f), li);
         const float s1 = fminf(c * z / rinv, low), d = all * s1 * sinv;
+        const f32x4 f = ld4(&Y.fk[16 * wave + 4 * g]) * (ti * (s1 * rinv));
+        h8 th[2], tl[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            if (2 * s <= wave) th[s] = Y.T_[0].operand(wave, l15, s, g), tl[s] = Y.T_[1].operand(wave, l15, s, g);
+        __syncthreads();
+        // 3: U of this wave's frames
+        h8 kt[TPW][2][G::KP], ph[2], pl[2];
+        f32x4 pi;
         {
             f32x4 u[NB];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 if (2 * s > wave) continue;
-                const h8 th = Y.T_[0].operand(wave, l15, s, g), tl = Y.T_[1].operand(wave, l15, s, g);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     const h8 hi = E.R[s][n][0][lane], lo = E.R[s][n][1][lane];
-                    u[n] = mma(tl, hi, mma(th, lo, mma(th, hi, s ? u[n] : zero)));
+                    u[n] = mma(tl[s], hi, mma(th[s], lo, mma(th[s], hi, s ? u[n] : zero)));
                 }
             }
-            const float ti = Y.ti[wave];
-            const f32x4 f = ld4(&Y.fk[16 * wave + 4 * g]) * (ti * (s1 * rinv));
             m = 0.0f;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
@@ -1106,47 +1180,56 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
             }
             m = wave_max(m);
             if (lane == 0) E.fmax[wave] = m;
+#pragma unroll
+            for (int j = 0; j < TPW; ++j) {
+                const int t = min(wave * TPW + j, 2 * NKT - 1);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int part = 0; part < G::KP; ++part) {
+                        const int rw = 32 * s + 4 * g + (l15 >> 2), col = 32 * (t >> 1) + 8 * (l15 & 3) + 4 * (t & 1);
+                        const h4 x = __builtin_bit_cast(h4, read_tr(&X.K[part][rw][col]));
+                        const h4 y = __builtin_bit_cast(h4, read_tr(&X.K[part][rw + 16][col]));
+                        kt[j][s][part] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                    }
+#pragma unroll
+                for (int n = 0; n < NB; ++n) S[j][n] *= d;
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+                if (2 * s <= wave) {
+                    ph[s] = Y.P_[0].operand(wave, l15, s, g);
+                    if (LOW) pl[s] = Y.P_[G::OP - 1].operand(wave, l15, s, g);
+                }
+            pi = ld4(&Y.pi[16 * wave + 4 * g]) * (rinv * cinv);
         }
         __syncthreads();
         // 4: this wave's rows of the state, its frames of the output
         sbound = fmaf(d, sreg, 0x1p21f * max4(E.fmax));
         sinv = 1.0f / s1;
 #pragma unroll
-        for (int j = 0; j < TPW; ++j) {
-            const int t = wave * TPW + j;
-            if (t >= 2 * NKT) continue;
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int n = 0; n < NB; ++n) S[j][n] *= d;
+            for (int n = 0; n < NB; ++n) {
+                const h8 hi = E.F[s][n][0][lane], lo = E.F[s][n][1][lane];
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int rw = 32 * s + 4 * g + (l15 >> 2), col = 32 * (t >> 1) + 8 * (l15 & 3) + 4 * (t & 1);
-#pragma unroll
-                for (int part = 0; part < G::KP; ++part) {
-                    const h4 x = __builtin_bit_cast(h4, read_tr(&X.K[part][rw][col]));
-                    const h4 y = __builtin_bit_cast(h4, read_tr(&X.K[part][rw + 16][col]));
-                    const h8 k = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) {
-                        S[j][n] = mma(k, E.F[s][n][0][lane], S[j][n]);
-                        if (part == 0) S[j][n] = mma(k, E.F[s][n][1][lane], S[j][n]);
-                    }
+                for (int j = 0; j < TPW; ++j) {
+                    S[j][n] = mma(kt[j][s][0], lo, mma(kt[j][s][0], hi, S[j][n]));
+                    if (G::KP == 2) S[j][n] = mma(kt[j][s][G::KP - 1], hi, S[j][n]);
                 }
             }
-        }
         {
             f32x4 o[NB];
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                 if (2 * s > wave) continue;
-                const h8 ph = Y.P_[0].operand(wave, l15, s, g);
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     const h8 hi = E.U[s][n][0][lane];
-                    o[n] = mma(ph, hi, s ? o[n] : zero);
-                    if (LOW) o[n] = mma(Y.P_[G::OP - 1].operand(wave, l15, s, g), hi, mma(ph, E.U[s][n][1][lane], o[n]));
+                    o[n] = mma(ph[s], hi, s ? o[n] : zero);
+                    if (LOW) o[n] = mma(pl[s], hi, mma(ph[s], E.U[s][n][1][lane], o[n]));
                 }
             }
-            const f32x4 pi = ld4(&Y.pi[16 * wave + 4 * g]) * (rinv * cinv);
 #pragma unroll
             for (int n = 0; n < NB; ++n)
 #pragma unroll
@@ -1162,10 +1245,10 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
 }
 
 // ---- launches ----
-template <class T, int NKT, int NB, bool FAST>
+template <class T, int NKT, int NB, int NW, bool FAST>
 void launch_fused(const nnsp_delta_args& a, hipStream_t st) {
-    const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 64 * NB - 1) / (64 * NB));
-    delta_chunk_kernel<T, NKT, NB, FAST><<<dim3((unsigned)grid), dim3(256), 0, st>>>(a);
+    const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 16 * NB * NW - 1) / (16 * NB * NW));
+    delta_chunk_kernel<T, NKT, NB, NW, FAST><<<dim3((unsigned)grid), dim3(64 * NW), 0, st>>>(a);
 }
 
 template <class T, int NKT>
@@ -1173,10 +1256,12 @@ DeltaSplit plan_split(const nnsp_delta_args& a) {
     DeltaSplit p;
     const long long rows = (long long)a.n_streams * a.value_heads;
     p.chunks = (a.n_frames + C - 1) / C;
-    p.kq_bytes = (long long)a.n_streams * a.key_heads * sizeof(KQ<T, NKT>);  // a chunk of all streams
-    p.tp_bytes = rows * sizeof(TP<T>);
+    p.kq_bytes = (long long)a.n_streams * a.key_heads * sizeof(KQ<T, NKT, C>);  // a chunk of all streams
+    p.tp_bytes = rows * sizeof(TP<T, C>);
     const long long per = p.kq_bytes + p.tp_bytes;
-    p.slab = (int)(per * p.chunks <= DELTA_SLAB_BYTES ? p.chunks : DELTA_SLAB_BYTES / per < 1 ? 1 : DELTA_SLAB_BYTES / per);
+    const int most = (int)(per * p.chunks <= DELTA_SLAB_BYTES ? p.chunks : DELTA_SLAB_BYTES / per < 1 ? 1 : DELTA_SLAB_BYTES / per);
+    const int slabs = (p.chunks + most - 1) / most;
+    p.slab = (p.chunks + slabs - 1) / slabs;  // of equal size
     p.state_bytes = p.slab < p.chunks ? (rows * a.dk * a.dv * 4 + 15) / 16 * 16 : 0;
     return p;
 }
@@ -1233,8 +1318,8 @@ int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
         constexpr int NKT = decltype(nkt)::value;
         constexpr bool FAST = decltype(fast)::value;
         if (split) launch_split<T, NKT, FAST>(a, st);
-        else if (a.dv <= 64) launch_fused<T, NKT, 1, FAST>(a, st);
-        else launch_fused<T, NKT, 2, FAST>(a, st);
+        else if (a.dv <= 64) launch_fused<T, NKT, 1, 4, FAST>(a, st);
+        else launch_fused<T, NKT, Geo<T, NKT, 1>::WIDE ? 1 : 2, Geo<T, NKT, 1>::WIDE ? 8 : 4, FAST>(a, st);
         return 0;
     });
     return (int)hipGetLastError();
