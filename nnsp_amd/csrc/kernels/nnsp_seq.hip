@@ -182,31 +182,53 @@ void launch_step(const nnsp_delta_args& a, hipStream_t st) {
 // ---- norms around a block ---------------------------------------------------
 // One pass: TPR threads hold a row in registers (NCH chunks of 8 elements a
 // thread), so each input is read once and each output written once; the call
-// is bound by those bytes.  Rows up to 1024 elements take 8 .. 64 lanes of a
-// wave and sum by lane permutes; longer ones a whole workgroup and one LDS
-// exchange per sum.
-template <class T>
-__device__ __forceinline__ void load8(float (&d)[8], const T* p, int c, int n) {
-    if (c + 8 <= n) {
-        T x[8];
-        load_raw(x, p + c);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = (float)x[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) d[j] = c + j < n ? (float)p[c + j] : 0.0f;
+// is bound by those bytes, provided that a gate's exponential and reciprocal
+// are the hardware's (with their exact forms the vector units were the bound).
+// Rows up to 1024 elements take 8 .. 64 lanes of a wave, U rows each so that
+// more is in flight, and sum by lane permutes; longer ones a whole workgroup
+// and one LDS exchange per sum.
+//
+// ROW_FULL: the row is 8 TPR NCH elements.  ROW_TAIL: the row ends within a
+// thread's chunk; that chunk then starts at n - 8, and what it has of the
+// elements before is kept out of the sums (and stored twice, the same).
+// ROW_TINY: fewer than 8 elements.
+enum { ROW_FULL, ROW_TAIL, ROW_TINY };
+
+template <int MODE>
+struct Place {
+    int c, first, n;  // where the chunk is, its first element that counts, the row's length
+    Place() = default;
+    __device__ __forceinline__ Place(int chunk, int n_) : c(chunk * 8), first(0), n(n_) {
+        if (MODE == ROW_TAIL) {
+            c = min(chunk * 8, n - 8);
+            first = min(chunk * 8 - c, 8);
+        }
     }
-}
-template <class T>
-__device__ __forceinline__ void store8(T* p, const float (&s)[8], int c, int n) {
-    if (c + 8 <= n) {
-        store_vec(p + c, s);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (c + j < n) p[c + j] = (T)s[j];
+    __device__ __forceinline__ bool counts(int j) const {
+        return MODE == ROW_FULL || (MODE == ROW_TAIL ? j >= first : c + j < n);
     }
-}
+    template <class T>
+    __device__ __forceinline__ typename Vec<T, 8>::raw load(const T* p) const {
+        typename Vec<T, 8>::raw x;
+        if (MODE == ROW_TINY) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = p[min(c + j, n - 1)];
+        } else {
+            x = *reinterpret_cast<const typename Vec<T, 8>::type*>(p + c);
+        }
+        return x;
+    }
+    template <class T>
+    __device__ __forceinline__ void store(T* p, const float (&s)[8]) const {
+        if (MODE == ROW_TINY) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c + j < n) p[c + j] = (T)s[j];
+        } else if (MODE == ROW_FULL || first < 8) {
+            store_vec(p + c, s);
+        }
+    }
+};
 
 template <int TPR>
 struct RowSum {
@@ -225,133 +247,186 @@ struct RowSum {
     }
 };
 
-template <int TPR, int NCH>
-__device__ __forceinline__ void norm_row(float (&h)[NCH][8], int kind, float eps, const float* w, const float* b, int tid,
-                                         int n, RowSum<TPR>& sum) {
-    if (kind == NNSP_NORM_NONE) return;
+// the parts of a row in this thread, normed; w and b: this thread's weights
+template <int TPR, int NCH, int MODE>
+__device__ __forceinline__ void norm_row(float (&h)[NCH][8], int kind, float eps, const float (&w)[NCH][8], const float* bias,
+                                         const Place<MODE> (&at)[NCH], int n, RowSum<TPR>& sum) {
     const float inv_n = 1.0f / (float)n;
     if (kind == NNSP_NORM_LAYER) {
         float m = 0.0f;
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) m += h[i][j];
+            for (int j = 0; j < 8; ++j) m += at[i].counts(j) ? h[i][j] : 0.0f;
         m = sum(m) * inv_n;
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = (i * TPR + tid) * 8 + j < n ? h[i][j] - m : 0.0f;
+            for (int j = 0; j < 8; ++j) h[i][j] -= m;
     }
     float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v = fmaf(h[i][j], h[i][j], v);
-    const float r = 1.0f / sqrtf(sum(v) * inv_n + eps);
+        for (int j = 0; j < 8; ++j) v = at[i].counts(j) ? fmaf(h[i][j], h[i][j], v) : v;
+    // v_rsq_f32 is good to one unit in the last place; a row whose variance and eps are both 0 is infinite times 0, as
+    // its definition is
+    const float r = __builtin_amdgcn_rsqf(fmaf(sum(v), inv_n, eps));
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-        const int c = (i * TPR + tid) * 8;
-        float x[8];
-        if (w) {
-            load8(x, w, c, n);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] *= r * x[j];
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] *= r;
-        }
-        if (b) {
-            load8(x, b, c, n);
+        for (int j = 0; j < 8; ++j) h[i][j] *= r * w[i][j];
+        if (bias) {
+            const auto x = at[i].load(bias);
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[i][j] += x[j];
         }
     }
 }
 
-template <class T, class R, int TPR, int NCH>
+// sigmoid(z); PRECISE: the rounding of z log2(e), which the exponential takes up, is put back (fp32 outputs show it)
+template <bool PRECISE>
+__device__ __forceinline__ float sigmoid(float z) {
+    const float l2e = 1.44269504f, t = -z * l2e;
+    float e = __builtin_amdgcn_exp2f(t);
+    if (PRECISE && fabsf(t) < 126.0f) {
+        const float low = fmaf(-z, l2e, -t) - z * 1.925963e-8f;  // what t lacks of -z log2(e)
+        e = fmaf(e, low * 0.69314718f, e);
+    }
+    return __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+template <class T, class R, int TPR, int NCH, int U, int MODE>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(const nnsp_norm_args a) {
-    constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;  // rows per workgroup
+    constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;  // rows of a workgroup at a time
     __shared__ float red[4 * (TPR > 64 ? TPR / 64 : 1)];
     RowSum<TPR> sum{red};
     const int tid = threadIdx.x % TPR, n = a.dim;
-    const long long row = (long long)blockIdx.x * RPB + threadIdx.x / TPR;
-    if (row >= a.rows * a.groups) return;  // TPR > 64: one row per workgroup, all its threads together
-    const long long ro = (unsigned)row / (unsigned)a.groups, ri = (unsigned)row % (unsigned)a.groups;
-    const T* xp = (const T*)a.x + ro * a.x_stride[0] + ri * a.x_stride[1];
-    const T* zp = (const T*)a.gate + ro * a.gate_stride[0] + ri * a.gate_stride[1];
-    const R* rp = (const R*)a.res_in + ro * a.res_in_stride[0] + ri * a.res_in_stride[1];
-
-    float h[NCH][8], z[NCH][8], r[NCH][8];
+    const unsigned rows = (unsigned)a.rows * (unsigned)a.groups;
+    const unsigned row0 = blockIdx.x * (unsigned)(RPB * U) + threadIdx.x / TPR;  // < 2^31 + 2^10
+    Place<MODE> at[NCH];
 #pragma unroll
-    for (int i = 0; i < NCH; ++i) load8(h[i], xp, (i * TPR + tid) * 8, n);
-    if (a.act != NNSP_GATE_NONE)
+    for (int i = 0; i < NCH; ++i) at[i] = Place<MODE>(i * TPR + tid, n);
+    typename Vec<T, 8>::raw x[U][NCH], z[U][NCH];
+    typename Vec<R, 8>::raw q[U][NCH];
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) load8(z[i], zp, (i * TPR + tid) * 8, n);
-    if (a.res_in) {
+    for (int u = 0; u < U; ++u) {
+        // rows past the last read the last again (and store nothing)
+        const unsigned row = min(row0 + u * RPB, rows - 1);
+        long long ro = row, ri = 0;
+        if (a.groups > 1) ro = row / (unsigned)a.groups, ri = row % (unsigned)a.groups;
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) load8(r[i], rp, (i * TPR + tid) * 8, n);
-    } else {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) r[i][j] = 0.0f;
-    }
-
-    norm_row<TPR, NCH>(h, a.post, a.eps_post, a.w_post, a.b_post, tid, n, sum);
-    if (a.act != NNSP_GATE_NONE) {
-#pragma unroll
-        for (int i = 0; i < NCH; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float g = 1.0f / (1.0f + expf(-z[i][j]));
-                h[i][j] *= a.act == NNSP_GATE_SILU ? z[i][j] * g : g;
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < NCH; ++i) {
-        const int c = (i * TPR + tid) * 8;
-        if (a.col_scale) {
-            float x[8];
-            load8(x, a.col_scale, c, n);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] *= x[j];
+        for (int i = 0; i < NCH; ++i) {
+            x[u][i] = at[i].load((const T*)a.x + ro * a.x_stride[0] + ri * a.x_stride[1]);
+            if (a.act != NNSP_GATE_NONE) z[u][i] = at[i].load((const T*)a.gate + ro * a.gate_stride[0] + ri * a.gate_stride[1]);
+            if (a.res_in) q[u][i] = at[i].load((const R*)a.res_in + ro * a.res_in_stride[0] + ri * a.res_in_stride[1]);
         }
-        // columns past the row's end hold 0 again (a bias or a gate of 0 may have moved them)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) h[i][j] = c + j < n ? fmaf(a.res_scale, h[i][j], r[i][j]) : 0.0f;
     }
-    if (a.res_out) {
-        R* p = (R*)a.res_out + ro * a.res_out_stride[0] + ri * a.res_out_stride[1];
+    float wp[NCH][8], wn[NCH][8];
+    const auto weights = [&](float (&w)[NCH][8], const float* p) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) store8(p, h[i], (i * TPR + tid) * 8, n);
-    }
-    if (a.y) {
-        norm_row<TPR, NCH>(h, a.pre, a.eps_pre, a.w_pre, a.b_pre, tid, n, sum);
-        T* p = (T*)a.y + ro * a.y_stride[0] + ri * a.y_stride[1];
+        for (int i = 0; i < NCH; ++i) {
+            if (p) {
+                const auto v = at[i].load(p);
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) store8(p, h[i], (i * TPR + tid) * 8, n);
+                for (int j = 0; j < 8; ++j) w[i][j] = v[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[i][j] = 1.0f;
+            }
+        }
+    };
+    if (a.post != NNSP_NORM_NONE) weights(wp, a.w_post);
+    if (a.pre != NNSP_NORM_NONE) weights(wn, a.w_pre);
+    // in place and without a norm, nothing else keeps a wave's stores behind the others' loads of the same tail
+    if (TPR > 64 && MODE == ROW_TAIL && a.post == NNSP_NORM_NONE) __syncthreads();
+
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const unsigned row = row0 + u * RPB;
+        float h[NCH][8];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] = (float)x[u][i][j];
+        if (a.post != NNSP_NORM_NONE) norm_row<TPR, NCH, MODE>(h, a.post, a.eps_post, wp, a.b_post, at, n, sum);
+        if (a.act != NNSP_GATE_NONE)
+#pragma unroll
+            for (int i = 0; i < NCH; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float g = (float)z[u][i][j], s = sigmoid<sizeof(T) == 4>(g);
+                    h[i][j] *= a.act == NNSP_GATE_SILU ? g * s : s;
+                }
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            if (a.col_scale) {
+                const auto c = at[i].load(a.col_scale);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[i][j] *= c[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] = a.res_in ? fmaf(a.res_scale, h[i][j], (float)q[u][i][j]) : a.res_scale * h[i][j];
+        }
+        long long ro = row, ri = 0;
+        if (a.groups > 1) ro = row / (unsigned)a.groups, ri = row % (unsigned)a.groups;
+        if (a.res_out && row < rows) {
+            R* p = (R*)a.res_out + ro * a.res_out_stride[0] + ri * a.res_out_stride[1];
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) at[i].store(p, h[i]);
+        }
+        if (a.y) {
+            if (a.pre != NNSP_NORM_NONE) norm_row<TPR, NCH, MODE>(h, a.pre, a.eps_pre, wn, a.b_pre, at, n, sum);
+            if (row < rows) {
+                T* p = (T*)a.y + ro * a.y_stride[0] + ri * a.y_stride[1];
+#pragma unroll
+                for (int i = 0; i < NCH; ++i) at[i].store(p, h[i]);
+            }
+        }
     }
 }
 
-template <class T, class R, int TPR, int NCH>
+template <class T, class R, int TPR, int NCH, int U, int MODE>
 void launch_norm_as(const nnsp_norm_args& a, hipStream_t st) {
-    constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;
+    constexpr int PER = (TPR > 256 ? 1 : 256 / TPR) * U;
     const long long rows = a.rows * a.groups;
-    norm_kernel<T, R, TPR, NCH><<<dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(TPR > 256 ? TPR : 256), 0, st>>>(a);
+    norm_kernel<T, R, TPR, NCH, U, MODE><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(TPR > 256 ? TPR : 256), 0, st>>>(a);
+}
+
+// U rows a thread once that still leaves every CU its workgroups
+template <class T, class R, int TPR, int NCH, int U>
+void launch_norm_u(const nnsp_norm_args& a, hipStream_t st) {
+    const bool full = a.dim == 8 * TPR * NCH;
+    if (U > 1 && a.rows * a.groups >= 2048ll * (256 / TPR) * U) {
+        if (full) launch_norm_as<T, R, TPR, NCH, U, ROW_FULL>(a, st);
+        else launch_norm_as<T, R, TPR, NCH, U, ROW_TAIL>(a, st);
+    } else {
+        if (full) launch_norm_as<T, R, TPR, NCH, 1, ROW_FULL>(a, st);
+        else launch_norm_as<T, R, TPR, NCH, 1, ROW_TAIL>(a, st);
+    }
 }
 
 template <class T, class R>
-void launch_norm_t(const nnsp_norm_args& a, hipStream_t st) {
+void launch_norm_t(nnsp_norm_args a, hipStream_t st) {
+    // rows and groups as one dimension where every tensor has them so
+    const auto joined = [&](const int64_t* s) { return s[0] == s[1] * a.groups; };
+    if (a.groups > 1 && joined(a.x_stride) && (!a.act || joined(a.gate_stride)) && (!a.res_in || joined(a.res_in_stride)) &&
+        (!a.res_out || joined(a.res_out_stride)) && (!a.y || joined(a.y_stride))) {
+        for (int64_t* s : {a.x_stride, a.gate_stride, a.res_in_stride, a.res_out_stride, a.y_stride}) s[0] = s[1];
+        a.rows *= a.groups;
+        a.groups = 1;
+    }
     const int nc = (a.dim + 7) / 8;  // chunks of 8 elements
-    if (nc <= 8) launch_norm_as<T, R, 8, 1>(a, st);
-    else if (nc <= 16) launch_norm_as<T, R, 16, 1>(a, st);
-    else if (nc <= 32) launch_norm_as<T, R, 32, 1>(a, st);
-    else if (nc <= 64) launch_norm_as<T, R, 64, 1>(a, st);
-    else if (nc <= 128) launch_norm_as<T, R, 64, 2>(a, st);
-    else if (nc <= 256) launch_norm_as<T, R, 256, 1>(a, st);
-    else if (nc <= 512) launch_norm_as<T, R, 256, 2>(a, st);
-    else if (nc <= 1024) launch_norm_as<T, R, 512, 2>(a, st);
-    else launch_norm_as<T, R, 1024, 2>(a, st);
+    if (a.dim < 8) launch_norm_as<T, R, 8, 1, 1, ROW_TINY>(a, st);
+    else if (nc <= 8) launch_norm_u<T, R, 8, 1, 4>(a, st);
+    else if (nc <= 16) launch_norm_u<T, R, 16, 1, 4>(a, st);
+    else if (nc <= 32) launch_norm_u<T, R, 32, 1, 4>(a, st);
+    else if (nc <= 64) launch_norm_u<T, R, 64, 1, 4>(a, st);
+    else if (nc <= 128) launch_norm_u<T, R, 64, 2, 2>(a, st);
+    else if (nc <= 256) launch_norm_u<T, R, 256, 1, 1>(a, st);
+    else if (nc <= 512) launch_norm_u<T, R, 256, 2, 1>(a, st);
+    else if (nc <= 1024) launch_norm_u<T, R, 512, 2, 1>(a, st);
+    else launch_norm_u<T, R, 1024, 2, 1>(a, st);
 }
 
 int ok(hipError_t e) { return e == hipSuccess ? 0 : (int)e; }

@@ -33,6 +33,12 @@ def _set_strides(args, strides: dict | None, names: tuple, dims: int) -> None:
         getattr(args, name + "_stride")[:] = [int(x) for x in st]
 
 
+def _fields(args, first: str, last: str):
+    """The 8-byte fields first .. last of a struct as one array (a call sets them all, in one go)."""
+    begin, end = getattr(type(args), first).offset, getattr(type(args), last).offset + 8
+    return (C.c_uint64 * ((end - begin) // 8)).from_buffer(args, begin)
+
+
 class GatedDelta:
     """Plan of nnsp_delta_exec_device.
 
@@ -50,6 +56,7 @@ class GatedDelta:
         a.l2norm, a.eps = int(bool(l2norm)), eps
         L = _lib.lib()
         self._ref, self._call = C.byref(a), L.nnsp_delta_exec_device
+        self._ptrs = _fields(a, "q", "workspace_bytes")
         _lib.check(L.nnsp_delta_contiguous(self._ref), "nnsp_delta_contiguous")
         a.scale = dk ** -0.5 if scale is None else scale
         _set_strides(a, strides, ("q", "k", "v", "g", "beta", "out"), 3)
@@ -61,11 +68,11 @@ class GatedDelta:
                     state_out: int | None = None, lens: int | None = None, workspace: int | None = None,
                     stream: int | None = None) -> None:
         """One call; ``workspace``: workspace_bytes bytes of device memory."""
-        a = self.args
-        a.q, a.k, a.v, a.g, a.beta, a.out = q, k, v, g, beta, out
-        a.state_in, a.state_out, a.lens, a.workspace = state_in, state_out, lens, workspace
-        a.workspace_bytes = self.workspace_bytes if workspace else 0
-        _lib.check(self._call(self._ref, stream), "nnsp_delta_exec_device")
+        self._ptrs[:] = (q or 0, k or 0, v or 0, g or 0, beta or 0, lens or 0, state_in or 0, out or 0, state_out or 0,
+                         workspace or 0, self.workspace_bytes if workspace else 0)
+        rc = self._call(self._ref, stream)
+        if rc:
+            _lib.check(rc, "nnsp_delta_exec_device")
 
 
 class BlockNorm:
@@ -86,6 +93,7 @@ class BlockNorm:
         a.eps_pre, a.eps_post, a.res_scale = eps, eps if eps_post is None else eps_post, res_scale
         L = _lib.lib()
         self._ref, self._call = C.byref(a), L.nnsp_norm_exec_device
+        self._ptrs = _fields(a, "x", "y")
         _lib.check(L.nnsp_norm_contiguous(self._ref), "nnsp_norm_contiguous")
         _set_strides(a, strides, ("x", "gate", "res_in", "res_out", "y"), 2)
 
@@ -93,7 +101,8 @@ class BlockNorm:
                     b_post: int | None = None, col_scale: int | None = None, w_pre: int | None = None,
                     b_pre: int | None = None, res_in: int | None = None, res_out: int | None = None,
                     stream: int | None = None) -> None:
-        a = self.args
-        a.x, a.y, a.gate, a.res_in, a.res_out = x, y, gate, res_in, res_out
-        a.w_post, a.b_post, a.col_scale, a.w_pre, a.b_pre = w_post, b_post, col_scale, w_pre, b_pre
-        _lib.check(self._call(self._ref, stream), "nnsp_norm_exec_device")
+        self._ptrs[:] = (x or 0, gate or 0, res_in or 0, w_post or 0, b_post or 0, col_scale or 0, w_pre or 0, b_pre or 0,
+                         res_out or 0, y or 0)
+        rc = self._call(self._ref, stream)
+        if rc:
+            _lib.check(rc, "nnsp_norm_exec_device")
