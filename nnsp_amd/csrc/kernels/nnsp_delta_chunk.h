@@ -83,6 +83,48 @@ __device__ __forceinline__ float amax4(float m, const f32x4& x) {
     return fmaxf(fmaxf(fmaxf(m, fabsf(x[0])), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
 }
 
+// the value of the lane N before in the row of 16; the first N keep `first`
+template <int N>
+__device__ __forceinline__ float row_shr(float x, float first) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(first), __float_as_int(x), 0x110 + N, 0xf, 0xf, false));
+}
+template <int N>
+__device__ __forceinline__ double row_shr(double x) {
+    const long long b = __builtin_bit_cast(long long, x);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, 0x110 + N, 0xf, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), 0x110 + N, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (unsigned)lo | (long long)hi << 32);
+}
+__device__ __forceinline__ double lane_of(double x, int l) {
+    const long long b = __builtin_bit_cast(long long, x);
+    const int lo = __builtin_amdgcn_readlane((int)b, l), hi = __builtin_amdgcn_readlane((int)(b >> 32), l);
+    return __builtin_bit_cast(double, (unsigned)lo | (long long)hi << 32);
+}
+// sum and minimum over the lanes up to this one of each group of C (32, 64)
+template <int C>
+__device__ __forceinline__ double scan_sum(double x, int lane) {
+    x += row_shr<1>(x);
+    x += row_shr<2>(x);
+    x += row_shr<4>(x);
+    x += row_shr<8>(x);
+    const double a = lane_of(x, 15), b = lane_of(x, 47);
+    if (C == 32) return lane & 16 ? x + (lane & 32 ? b : a) : x;
+    const double m = lane_of(x, 31) + a;
+    return x + (lane < 16 ? 0.0 : lane < 32 ? a : lane < 48 ? m : m + b);
+}
+template <int C>
+__device__ __forceinline__ float scan_min(float x, int lane) {
+    x = fminf(x, row_shr<1>(x, x));
+    x = fminf(x, row_shr<2>(x, x));
+    x = fminf(x, row_shr<4>(x, x));
+    x = fminf(x, row_shr<8>(x, x));
+    const auto of = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); };
+    const float a = of(15), b = of(47);
+    if (C == 32) return lane & 16 ? fminf(x, lane & 32 ? b : a) : x;
+    const float m = fminf(of(31), a);
+    return lane < 16 ? x : fminf(x, lane < 32 ? a : lane < 48 ? m : fminf(m, b));
+}
+
 // keeps the operands of later products out of the registers until theirs are done
 __device__ __forceinline__ void no_hoist() { __builtin_amdgcn_sched_barrier(0); }
 
@@ -303,13 +345,7 @@ __device__ __forceinline__ void make_factors(const KQ<T, NKT, C>&, TP<T, C>& Y, 
         M.kc[i] = exp2_fast((M.gh[e] - h) + (M.gl[e] - l)) * kx;
     } else if (part == 1) {
         // largest decay ratio of a row: e(G_i - min over j <= i of G_j); largest length of a key
-        float lo = h;
-        const float kn = wave_max(M.kn[i]);
-#pragma unroll
-        for (int d = 1; d < C; d <<= 1) {
-            const float y = __shfl_up(lo, d);
-            if (i >= d) lo = fminf(lo, y);
-        }
+        const float lo = scan_min<C>(h, lane), kn = wave_max(M.kn[i]);
         float inv;
         const float qx = M.qx[i], sc = scale_of(M.qn[i] * kn * exp2_fast(fminf(h - lo, 120.0f)), inv);
         Y.pi[i] = inv;
@@ -395,16 +431,20 @@ __device__ __forceinline__ void invert_diagonal(const TriA<C>& A, Diag<C>& D, in
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) x[i] = i == l15 ? 1.0f : 0.0f;
+    // column j of A, what is below the diagonal, two steps ahead of its use (all at once would be 144 registers)
+    f32x4 a[3][4];
+    const auto column = [&](int j) {
+#pragma unroll
+        for (int q = (j + 1) / 4; q < 4; ++q) a[j % 3][q] = ld4(&A.A[b + j][b + 4 * q]);
+    };
+    column(0);
+    column(1);
 #pragma unroll
     for (int j = 0; j < 15; ++j) {
-        asm volatile("" : "+v"(x[j]) : : "memory");  // not all of A in registers at once
+        if (j + 2 < 15) column(j + 2);
+        asm volatile("" : "+v"(x[j]) : : "memory");
 #pragma unroll
-        for (int q = (j + 1) / 4; q < 4; ++q) {
-            const f32x4 a = ld4(&A.A[b + j][b + 4 * q]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                if (4 * q + r > j) x[4 * q + r] = fmaf(-a[r], x[j], x[4 * q + r]);
-        }
+        for (int i = j + 1; i < 16; ++i) x[i] = fmaf(-a[j % 3][i / 4][i % 4], x[j], x[i]);
     }
 #pragma unroll
     for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4*>(&D.D[k][l15][4 * q]) = f32x4{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
@@ -743,12 +783,7 @@ struct Rows {
     __device__ __forceinline__ void stage_gates(TP<T, C>& Y, Make<C>& M) {
         if (wave == 0) {
             // running sum of g in 64 bits, in units of log2, kept as two floats: differences of near frames stay exact
-            double x = (double)decay_log(rg) * 1.4426950408889634;
-#pragma unroll
-            for (int d = 1; d < C; d <<= 1) {
-                const double y = __shfl_up(x, d);
-                if ((lane & (C - 1)) >= d) x += y;
-            }
+            const double x = scan_sum<C>((double)decay_log(rg) * 1.4426950408889634, lane);
             const int i = lane & (C - 1);  // of a chunk of 32, both halves of the wave alike
             M.gh[i] = (float)x;
             M.gl[i] = (float)(x - (double)(float)x);
