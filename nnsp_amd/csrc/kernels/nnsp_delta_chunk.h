@@ -196,12 +196,13 @@ struct KQ {
 template <class T, int C>
 struct TP {
     static constexpr int OP = std::is_same<T, __bf16>::value ? 1 : 2;
-    Tri<C> T_[2], P_[OP];
+    Tri<C> P_[OP];
     alignas(16) float beta[C], fx[C], fk[C], fq[C];  // factors of v, K S0, U into the state, Q S0
     alignas(16) float pi[C];                         // 2^-scale of P's rows
     float ti[4];                                     // 2^-scale of T's row tiles
     float all, fkmax;                                // decay over the whole chunk; largest fk
     float bmax, xmax;                                // largest |beta|; |beta e(G) k^ . x| is at most xmax |x|_max
+    Tri<C> T_[2];                                    // last: what T is made from lies here and beyond until then
 };
 // what making T and P takes besides; s and e are the first and last frame of a frame's 16
 template <int C>
@@ -220,8 +221,7 @@ template <int C>
 struct Diag {
     alignas(16) float D[C / 16][16][20];  // transposed inverses of the diagonal blocks
 };
-static_assert(sizeof(Diag<64>) <= 2 * sizeof(Tri<64>) && sizeof(Diag<32>) <= 2 * sizeof(Tri<32>),
-              "the inverses lie where T is written afterwards");
+static_assert(sizeof(Diag<32>) <= 2 * sizeof(Tri<32>), "the inverses lie where T is written afterwards");
 
 // raw rows of q and k on their way to LDS, PR threads a row: thread (row, part)
 // holds chunks of 8 elements part, part + PR, ...
@@ -451,11 +451,11 @@ __device__ __forceinline__ void invert_diagonal(const TriA<C>& A, Diag<C>& D, in
 }
 
 // Everything of a staged chunk of 64 that needs no state, by four waves.  Starts
-// and ends with the workgroup together.
+// and ends with the workgroup together.  A may lie where T is written.
 template <class T, int NKT>
-__device__ __forceinline__ void make_tp(const KQ<T, NKT, 64>& X, TP<T, 64>& Y, Make<64>& M, TriA<64>& A, int wave, int lane) {
+__device__ __forceinline__ void make_tp(const KQ<T, NKT, 64>& X, TP<T, 64>& Y, Make<64>& M, Diag<64>& D, TriA<64>& A, int wave,
+                                        int lane) {
     constexpr int KP = KQ<T, NKT, 64>::KP, OP = TP<T, 64>::OP;
-    Diag<64>& D = *reinterpret_cast<Diag<64>*>(Y.T_);
     const int l15 = lane & 15, g = lane >> 4;
     f32x4 acc[4];
 #pragma unroll
@@ -965,9 +965,10 @@ template <class T, int NKT, bool FAST>
 __global__ __launch_bounds__(256, 2) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
     struct Lds {
         KQ<T, NKT, C> X;
-        TP<T, C> Y;
         Make<C> M;
-        TriA<C> A;
+        Diag<C> D;
+        TP<T, C> Y;
+        char tail[sizeof(TriA<C>) - 2 * sizeof(Tri<C>)];  // A takes T's place and this
     };
     __shared__ Lds L;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -986,7 +987,7 @@ __global__ __launch_bounds__(256, 2) void delta_prepare_kernel(const nnsp_delta_
             rows.bp += a.beta_stride[2];
             rows.fetch_gates(left);
         }
-        make_tp(L.X, L.Y, L.M, L.A, wave, here(lane));
+        make_tp(L.X, L.Y, L.M, L.D, *reinterpret_cast<TriA<C>*>(L.Y.T_), wave, here(lane));
         copy_out(b.tp + (((long long)s * a.value_heads + h0 + r) * b.chunks + c) * sizeof(TP<T, C>), L.Y, tid);
         if (r + 1 < rep) {
             __syncthreads();
