@@ -65,6 +65,11 @@ __device__ __forceinline__ float scale_of(float m, float& inv) {
     inv = __int_as_float((254 - s) << 23);
     return __int_as_float(s << 23);
 }
+// 1 / x of a power of two from 2^-126 to 2^126
+__device__ __forceinline__ float inverse2(float x) { return __int_as_float((254 << 23) - __float_as_int(x)); }
+// 0, or NaN of an infinite magnitude: a scale that holds an infinity would leave
+// the values beside it 0, so it is made to show
+__device__ __forceinline__ float poison(float m) { return m * 0.0f; }
 __device__ __forceinline__ float max_xor16_32(float x) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -246,10 +251,16 @@ __device__ __forceinline__ void fetch_rows(RawRows<T, NKT, PR>& r, const T* p, i
         }
     }
 }
-// scaled fp16 parts to LDS; returns 2^-scale (0 of a row of zeros), sets the sum of squares
+// scaled fp16 parts to LDS; returns 2^-scale (0 of a row of zeros) and the sum of
+// the scaled values' squares, which stays in range however loud or faint the row is
 template <int KP, int C, int KS, class T, int NKT, int PR>
 __device__ __forceinline__ float stage_rows(const RawRows<T, NKT, PR>& r, _Float16 (*dst)[C][KS], int row, int part, float& ss) {
     constexpr int N = RawRows<T, NKT, PR>::N;
+    const auto sum = [](float x) {
+        x = add_xor2(add_xor1(x));
+        if (PR >= 8) x = add_mirror4(x);
+        return PR >= 16 ? add_xor8(x) : x;
+    };
     ss = 0.0f;
     float inv;
     if constexpr (std::is_same<T, _Float16>::value) {
@@ -262,12 +273,11 @@ __device__ __forceinline__ float stage_rows(const RawRows<T, NKT, PR>& r, _Float
                 const h2 x = {r.x[i][j], r.x[i][j + 1]};
                 ss = __builtin_amdgcn_fdot2(x, x, ss, false);
             }
-        ss = add_xor2(add_xor1(ss));
-        if (PR >= 8) ss = add_mirror4(ss);
-        if (PR >= 16) ss = add_xor8(ss);
+        ss = sum(ss);
         const int e = min(max(5 - (((__float_as_int(ss) >> 23) - 127) >> 1), -14), 15);
         const _Float16 s = __builtin_bit_cast(_Float16, (unsigned short)((15 + e) << 10));
         inv = ss > 0.0f ? __int_as_float((127 - e) << 23) : 0.0f;
+        ss *= __int_as_float((127 + 2 * e) << 23);
 #pragma unroll
         for (int i = 0; i < N; ++i)
             if (4 * NKT % PR == 0 || part + PR * i < 4 * NKT) *reinterpret_cast<h8*>(&dst[0][row][(part + PR * i) * 8]) = r.x[i] * s;
@@ -276,14 +286,7 @@ __device__ __forceinline__ float stage_rows(const RawRows<T, NKT, PR>& r, _Float
 #pragma unroll
         for (int i = 0; i < N; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = (float)r.x[i][j];
-                m = fmaxf(m, fabsf(x));
-                ss = fmaf(x, x, ss);
-            }
-        ss = add_xor2(add_xor1(ss));
-        if (PR >= 8) ss = add_mirror4(ss);
-        if (PR >= 16) ss = add_xor8(ss);
+            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf((float)r.x[i][j]));
         m = max_dpp<0x4e>(max_dpp<0xb1>(m));
         if (PR >= 8) m = max_dpp<0x141>(m);
         if (PR >= 16) m = max_dpp<0x128>(m);
@@ -294,15 +297,17 @@ __device__ __forceinline__ float stage_rows(const RawRows<T, NKT, PR>& r, _Float
             h8 hi, lo;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float x = (float)r.x[i][j];
-                hi[j] = (_Float16)(x * s);
-                if (KP == 2) lo[j] = (_Float16)fmaf(x, s, -(float)hi[j]);
+                const float x = (float)r.x[i][j] * s;
+                ss = fmaf(x, x, ss);
+                hi[j] = (_Float16)x;
+                if (KP == 2) lo[j] = (_Float16)(x - (float)hi[j]);
             }
             const int c = (part + PR * i) * 8;
             if (4 * NKT % PR != 0 && c >= 32 * NKT) continue;
             *reinterpret_cast<h8*>(&dst[0][row][c]) = hi;
             if (KP == 2) *reinterpret_cast<h8*>(&dst[KP - 1][row][c]) = lo;
         }
+        ss = sum(ss);
     }
     return inv;
 }
@@ -580,7 +585,7 @@ struct Chunk {
         smax = wave_max(smax);
         float inv;
         const float sc = scale_of(smax, inv);
-        inv *= sinv;
+        inv = fmaf(inv, sinv, poison(smax));
         sout = inv;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
@@ -634,7 +639,8 @@ struct Chunk {
         f32x4 u[2][NB];  // U = u ti rinv, where |u| is at most 32 products of 2^30
         float rinv;
         h8 hi[NB], lo[NB];
-        const float rs = scale_of(wave_max(rmax), rinv);
+        rmax = wave_max(rmax);
+        const float rs = scale_of(rmax, rinv);
 #pragma unroll
         for (int n = 0; n < NB; ++n) split<true>(R[0][n], R[1][n], all4(rs), all4(rs), hi[n], lo[n]);
 #pragma unroll
@@ -643,7 +649,7 @@ struct Chunk {
 #pragma unroll
             for (int n = 0; n < NB; ++n) u[m][n] = mma(tl, hi[n], mma(th, lo[n], mma(th, hi[n], zero)));
         }
-        const float ti = Y.ti[0] * rinv;  // u to below 2^14: times 2^-22
+        const float ti = fmaf(Y.ti[0], rinv, poison(rmax));  // u to below 2^14: times 2^-22
 #pragma unroll
         for (int n = 0; n < NB; ++n) split<LOW>(u[0][n], u[1][n], all4(0x1p-22f), all4(0x1p-22f), hi[n], lo[n]);
 #pragma unroll
@@ -675,8 +681,8 @@ struct Chunk {
         const float all = Y.all;
         float zi, li;
         const float z = scale_of(Y.fkmax, zi) * 0x1p-36f, low = scale_of(fmaxf(smax * sinv * (all * 0x1p-13f), 0x1p-86f), li);
-        const float s = fminf(z / ti, low), d = all * s * sinv;  // true U fk times s = u fk (ti s)
-        sinv = 1.0f / s;
+        const float s = fminf(z * inverse2(Y.ti[0]) * rs, low), d = all * s * sinv;  // true U fk times s = u fk (ti s)
+        sinv = inverse2(s);
         const f32x4 f0 = ld4(&Y.fk[4 * g]) * (ti * s), f1 = ld4(&Y.fk[16 + 4 * g]) * (ti * s);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
@@ -768,16 +774,20 @@ struct Rows {
         qp += qs, kp += ks, bp += bs;
         if (gp) gp += gs;
     }
+    // of a scaled row, to its length 1 or to what it was; v_rsq_f32 and v_sqrt_f32 are good to one unit
+    static __device__ __forceinline__ float factor(const nnsp_delta_args& a, float inv, float ss) {
+        if (!(inv > 0.0f)) return 0.0f;  // a row of zeros
+        if (!a.l2norm) return inv;
+        const float s = inverse2(inv), e = a.eps * s * s;  // eps in the row's scale
+        return e < INFINITY ? __builtin_amdgcn_rsqf(ss + e) : inv * __builtin_amdgcn_rsqf(a.eps);
+    }
     __device__ __forceinline__ void stage(const nnsp_delta_args& a, KQ<T, NKT, C>& X, TP<T, C>& Y, Make<C>& M) {
         constexpr int KP = KQ<T, NKT, C>::KP;
-        float ss, inv, f;
-        // a row of zeros has inv 0 and no part in anything, whatever its norm's reciprocal is (v_rsq_f32: one unit)
-        inv = stage_rows<KP>(rk, X.K, row, part, ss);
-        f = a.l2norm ? __builtin_amdgcn_rsqf(ss + a.eps) : 1.0f;
-        if (part == 0) M.kx[row] = inv > 0.0f ? inv * f : 0.0f, M.kn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * f : 0.0f;
+        float ss, inv = stage_rows<KP>(rk, X.K, row, part, ss), x = factor(a, inv, ss);
+        if (part == 0) M.kx[row] = x, M.kn[row] = x * __builtin_amdgcn_sqrtf(ss);
         inv = stage_rows<KP>(rq, X.Q, row, part, ss);
-        f = a.scale * (a.l2norm ? __builtin_amdgcn_rsqf(ss + a.eps) : 1.0f);
-        if (part == 0) M.qx[row] = inv > 0.0f ? inv * f : 0.0f, M.qn[row] = inv > 0.0f ? __builtin_amdgcn_sqrtf(ss) * fabsf(f) : 0.0f;
+        x = a.scale * factor(a, inv, ss);
+        if (part == 0) M.qx[row] = x, M.qn[row] = fabsf(x) * __builtin_amdgcn_sqrtf(ss);
         stage_gates(Y, M);
     }
     __device__ __forceinline__ void stage_gates(TP<T, C>& Y, Make<C>& M) {
@@ -1148,10 +1158,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
         __syncthreads();
         // 2: R and Q S0 of this wave's frames
         const float sreg = max4(E.smax), smax = sreg * sinv;  // the registers' values, the true ones
+        const float vmax = max4(E.vmax), bad = poison(sreg) + poison(vmax);
         float rinv;
+        const float sc = scale_of(Y.bmax * vmax + Y.xmax * smax, rinv);
+        rinv += bad;
+        inv += bad;
         f32x4 O[NB];
         {
-            const float sc = scale_of(Y.bmax * max4(E.vmax) + Y.xmax * smax, rinv);
             f32x4 x[NB];
 #pragma unroll
             for (int s = 0; s < NKT; ++s) {
@@ -1183,10 +1196,10 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
         }
         if (left > C) cols.fetch(left - C - 16 * wave);
         // what the next steps take of the images and know of the scales (see advance()), before the waits
-        const float tmax = max4(Y.ti), cinv = tmax * 0x1p22f, c = 1.0f / cinv, all = Y.all, ti = Y.ti[wave];
+        const float tmax = max4(Y.ti), cinv = tmax * 0x1p22f, c = inverse2(cinv), all = Y.all, ti = Y.ti[wave];
         float zi, li;
         const float z = scale_of(Y.fkmax, zi) * 0x1p-14f, low = scale_of(fmaxf(smax * (all * 0x1p-13f), 0x1p-86f), li);
-        const float s1 = fminf(c * z / rinv, low), d = all * s1 * sinv;
+        const float s1 = fminf(c * z * sc, low), d = all * s1 * sinv;
         const f32x4 f = ld4(&Y.fk[16 * wave + 4 * g]) * (ti * (s1 * rinv));
         h8 th[2], tl[2];
 #pragma unroll
@@ -1242,7 +1255,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
         __syncthreads();
         // 4: this wave's rows of the state, its frames of the output
         sbound = fmaf(d, sreg, 0x1p21f * max4(E.fmax));
-        sinv = 1.0f / s1;
+        sinv = inverse2(s1);
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll

@@ -106,26 +106,45 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const nnsp_delta_args a
         const float dec = expf(decay_log(raw.g)), beta = raw.beta;
         if (t + 1 < n) fetch(t + 1);
 
-        float sk[4] = {0, 0, 0, 0}, sq[4] = {0, 0, 0, 0}, kk = 0, qq = 0, kq = 0;
+        float sk[4], sq[4], kk, qq, kq;
+        const auto sums = [&] {
+            kk = qq = kq = 0.0f;
 #pragma unroll
-        for (int r = 0; r < RK; ++r) {
-            kk = fmaf(k[r], k[r], kk);
-            qq = fmaf(q[r], q[r], qq);
-            kq = fmaf(k[r], q[r], kq);
+            for (int j = 0; j < 4; ++j) sk[j] = sq[j] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sk[j] = fmaf(S[r][j], k[r], sk[j]);
-                sq[j] = fmaf(S[r][j], q[r], sq[j]);
+            for (int r = 0; r < RK; ++r) {
+                kk = fmaf(k[r], k[r], kk);
+                qq = fmaf(q[r], q[r], qq);
+                kq = fmaf(k[r], q[r], kq);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    sk[j] = fmaf(S[r][j], k[r], sk[j]);
+                    sq[j] = fmaf(S[r][j], q[r], sq[j]);
+                }
             }
-        }
-        const auto sum8 = [](float x) { return add_xor32(add_xor16(add_xor8(x))); };
+            const auto sum8 = [](float x) { return add_xor32(add_xor16(add_xor8(x))); };
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sk[j] = sum8(sk[j]), sq[j] = sum8(sq[j]);
-        kq = sum8(kq);
+            for (int j = 0; j < 4; ++j) sk[j] = sum8(sk[j]), sq[j] = sum8(sq[j]);
+            kq = sum8(kq);
+            if (a.l2norm) kk = sum8(kk), qq = sum8(qq);
+        };
+        sums();
         float rk = 1.0f, rq = 1.0f;
         if (a.l2norm) {
-            rk = 1.0f / sqrtf(sum8(kk) + a.eps);
-            rq = 1.0f / sqrtf(sum8(qq) + a.eps);
+            float ek = a.eps, eq = a.eps;
+            // squares that left 32 bits (the same in all lanes): the row at another scale, which its norm takes out again
+            const auto outside = [](float x) { return !(x > 0x1p-100f && x < 0x1p100f); };
+            if (outside(kk + ek) || outside(qq + eq)) {
+                const float fk = kk > 1.0f ? 0x1p-80f : 0x1p60f, fq = qq > 1.0f ? 0x1p-80f : 0x1p60f;
+                const bool ok = outside(kk + ek), oq = outside(qq + eq);
+                ek = ok ? ek * fk * fk : ek;
+                eq = oq ? eq * fq * fq : eq;
+#pragma unroll
+                for (int r = 0; r < RK; ++r) k[r] = ok ? k[r] * fk : k[r], q[r] = oq ? q[r] * fq : q[r];
+                sums();
+            }
+            rk = 1.0f / sqrtf(kk + ek);
+            rq = 1.0f / sqrtf(qq + eq);
         }
         float u[4], o[4];
 #pragma unroll

@@ -303,6 +303,80 @@ def test_delta_keys_of_zeros_and_of_all_lengths(T):
         close(so, rs, "f32", T, 64, "state")
 
 
+@pytest.mark.parametrize("l2norm,qe,ke", [(True, -80, 0), (True, 0, -80), (True, 75, 75), (False, -75, 0), (False, 75, -75),
+                                          (False, -75, 75)])
+@pytest.mark.parametrize("T", [5, 40, 100])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_delta_rows_whose_squares_leave_32_bits(dtype, T, l2norm, qe, ke):
+    """Queries and keys so faint or loud that their squares are 0 or infinite in 32 bits."""
+    d = make(2, T, 1, 2, 64, 48, dtype, seed=T, l2norm=l2norm)
+    d["q"], d["k"] = (d["q"].float() * 2.0 ** qe).to(DT[dtype]), (d["k"].float() * 2.0 ** ke).to(DT[dtype])
+    if (l2norm, ke) == (False, 75):
+        d["k"][:, 1:] = 0  # one key per stream: with more, the rule itself leaves 32 bits
+    out, so = run_delta(d, 1, dtype, l2norm=l2norm, state=False)
+    ro, rs = delta_ref(d["q"], d["k"], d["v"], d["g"], d["beta"], None, None, l2norm, 64 ** -0.5)
+    close(out, ro, dtype, T, 64, "out")
+    close(so, rs, "f32", T, 64, "state")
+
+
+@pytest.mark.parametrize("T", [5, 40, 150])
+@pytest.mark.parametrize("what", ["v", "state"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_delta_infinity_is_seen(dtype, what, T):
+    """An infinite value never turns its neighbours' columns into finite wrong ones; earlier chunks are as without it."""
+    d = make(2, T, 1, 2, 64, 64, dtype, seed=T)
+    ro, rs = delta_ref(d["q"], d["k"], d["v"], d["g"], d["beta"], d["state"], None, True, 64 ** -0.5)
+    t, hit = T - 3, torch.zeros(2, 2, dtype=torch.bool)
+    hit[1, 1] = True
+    if what == "v":
+        d["v"][1, t, 1, 5] = float("inf")
+    else:
+        d["state"][1, 1, 7, 5], t = float("-inf"), 0
+    out, so = run_delta(d, 1, dtype)
+    for s, h in ((0, 0), (0, 1), (1, 0)):
+        close(out[s, :, h], ro[s, :, h], dtype, T, 64, "another head")
+        close(so[s, h], rs[s, h], "f32", T, 64, "another head's state")
+    mine, ref = out[1, :, 1].double().cpu(), ro[1, :, 1]
+    close(out[1, :t // 64 * 64, 1], ref[:t // 64 * 64], dtype, T, 64, "before")
+    assert not bool(torch.isfinite(mine[t:, 5]).any()) and not bool(torch.isfinite(so[1, 1, :, 5]).any())
+    fin = torch.isfinite(mine)
+    close(torch.where(fin, mine, ref), ref, dtype, T, 64, "finite values")
+    st = so[1, 1].double().cpu()
+    close(torch.where(torch.isfinite(st), st, rs[1, 1]), rs[1, 1], "f32", T, 64, "finite states")
+
+
+@pytest.mark.parametrize("S,T,h,d_", [(2, 5, 2, 64), (2, 130, 2, 64), (8, 330, 32, 128), (300, 70, 1, 32)])
+def test_delta_final_state_dropped(S, T, h, d_):
+    """Frame by frame, in two passes (of one slab and of two) and in chunks, without state_out."""
+    d = make(S, T, h, h, d_, d_, "bf16", seed=S)
+    ref, _ = run_delta(d, h, "bf16")
+    p = gated_delta()(S, T, h, h, d_, d_)
+    out = torch.zeros_like(ref)
+    ws = torch.empty(max(16, p.workspace_bytes), dtype=torch.uint8, device="cuda")
+    p.exec_device(ptr(d["q"]), ptr(d["k"]), ptr(d["v"]), ptr(d["g"]), ptr(d["beta"]), ptr(out), state_in=ptr(d["state"]),
+                  workspace=ptr(ws), stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(out, ref)
+
+
+def test_delta_two_calls_at_once():
+    """Two calls in two passes on two streams, each with its own workspace, and one more behind the first."""
+    T = 700
+    d = [make(2, T, 2, 4, 128, 128, "bf16", seed=i) for i in range(2)]
+    ref = [run_delta(x, 2, "bf16") for x in d]
+    p = gated_delta()(2, T, 2, 4, 128, 128)
+    st = [torch.cuda.Stream() for _ in d]
+    ws = [torch.empty(p.workspace_bytes, dtype=torch.uint8, device="cuda") for _ in d]
+    out, so = [torch.zeros_like(r[0]) for r in ref], [torch.zeros_like(r[1]) for r in ref]
+    torch.cuda.synchronize()
+    for i in (0, 1, 0):
+        p.exec_device(ptr(d[i]["q"]), ptr(d[i]["k"]), ptr(d[i]["v"]), ptr(d[i]["g"]), ptr(d[i]["beta"]), ptr(out[i]),
+                      state_in=ptr(d[i]["state"]), state_out=ptr(so[i]), workspace=ptr(ws[i]), stream=st[i].cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(out[i], ref[i][0]) and torch.equal(so[i], ref[i][1])
+
+
 def test_delta_same_bits_every_time_and_by_stream():
     """Results do not depend on the run, nor on the other streams of the call."""
     d = make(40, 130, 2, 4, 64, 64, "bf16", seed=6)
