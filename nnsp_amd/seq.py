@@ -8,6 +8,7 @@ are made, and every call takes device buffers as raw pointers (e.g.
 ``torch.Tensor.data_ptr()``) and queues its kernels on ``stream`` (a raw
 ``hipStream_t``, e.g. ``torch.cuda.current_stream().cuda_stream``; 0 or None:
 the default stream).  The buffers have to live until the stream has passed them.
+A plan is for one thread at a time; threads that call at once make one each.
 """
 from __future__ import annotations
 
@@ -26,11 +27,22 @@ def _one_of(table: dict, name: str, what: str) -> int:
     return table[name]
 
 
+def _set(args, **numbers) -> None:
+    """Integer fields of a struct, which ctypes alone would cut to their width."""
+    for name, x in numbers.items():
+        setattr(args, name, x)
+        if getattr(args, name) != x:
+            raise ValueError(f"{name} {x} is out of range")
+
+
 def _set_strides(args, strides: dict | None, names: tuple, dims: int) -> None:
     for name, st in (strides or {}).items():
         if name not in names or len(st) != dims:
             raise ValueError(f"strides of {name!r}: {dims} numbers for one of {', '.join(names)}")
-        getattr(args, name + "_stride")[:] = [int(x) for x in st]
+        st = [int(x) for x in st]
+        getattr(args, name + "_stride")[:] = st
+        if getattr(args, name + "_stride")[:] != st:
+            raise ValueError(f"strides of {name!r} {st} are out of range")
 
 
 def _fields(args, first: str, last: str):
@@ -51,8 +63,7 @@ class GatedDelta:
                  strides: dict | None = None):
         a = self.args = _lib.DeltaArgs()
         a.dtype = _one_of(DTYPES, dtype, "dtype")
-        a.n_streams, a.n_frames, a.key_heads, a.value_heads, a.dk, a.dv = (n_streams, n_frames, key_heads, value_heads,
-                                                                           dk, dv)
+        _set(a, n_streams=n_streams, n_frames=n_frames, key_heads=key_heads, value_heads=value_heads, dk=dk, dv=dv)
         a.l2norm, a.eps = int(bool(l2norm)), eps
         L = _lib.lib()
         self._ref, self._call = C.byref(a), L.nnsp_delta_exec_device
@@ -89,7 +100,7 @@ class BlockNorm:
         a.res_dtype = a.dtype if res_dtype is None else _one_of(DTYPES, res_dtype, "res_dtype")
         a.post, a.pre = _one_of(NORMS, post, "post"), _one_of(NORMS, pre, "pre")
         a.act = _one_of(GATES, act, "act")
-        a.rows, a.groups, a.dim = rows, groups, dim
+        _set(a, rows=rows, groups=groups, dim=dim)
         a.eps_pre, a.eps_post, a.res_scale = eps, eps if eps_post is None else eps_post, res_scale
         L = _lib.lib()
         self._ref, self._call = C.byref(a), L.nnsp_norm_exec_device

@@ -51,6 +51,17 @@ def test_delta_sizes_refused(sizes, message, code):
     refused(lambda: GatedDelta(*sizes), message, code)
 
 
+@pytest.mark.parametrize("make", [
+    lambda: GatedDelta((1 << 32) + 1, 1, 1, 1, 8, 8), lambda: GatedDelta(1, (1 << 32) + 3, 1, 1, 8, 8),
+    lambda: GatedDelta(1, 1, 1, 1, 8, (1 << 32) + 8), lambda: BlockNorm(1, (1 << 32) + 8), lambda: BlockNorm((1 << 64) + 1, 8),
+    lambda: BlockNorm(1, 8, groups=(1 << 32) + 1), lambda: BlockNorm(1, 8, strides={"x": ((1 << 64) + 8, 8)}),
+    lambda: GatedDelta(1, 1, 1, 1, 8, 8, strides={"v": (8, 8, 1 << 64)}),
+])
+def test_sizes_beyond_their_fields_are_refused(make):
+    with pytest.raises(ValueError, match="out of range"):
+        make()
+
+
 def test_delta_unknown_dtype():
     with pytest.raises(ValueError, match="one of"):
         GatedDelta(1, 1, 1, 1, 8, 8, dtype="f64")
