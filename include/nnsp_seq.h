@@ -67,7 +67,9 @@ extern "C" {
  * A value that is not finite in frame t spreads, as the recurrence has it, to
  * the later frames of its stream and head; where a call has more than
  * NNSP_DELTA_STEP_FRAMES frames it may reach the other frames of the same 64
- * (64 n .. 64 n + 63), earlier ones too.
+ * (64 n .. 64 n + 63), earlier ones too.  In such calls a column of v or of the
+ * state is as exact as 2^-38 of the largest among the 16 or 32 columns beside
+ * it, and decays above 1 (g > 0) cost precision by their product over 64 frames.
  *
  * workspace: nnsp_delta_workspace() bytes of device memory, 16-byte aligned,
  * used by this call only while its kernels run (one workspace per call in
@@ -77,7 +79,7 @@ extern "C" {
  * Limits: dk, dv 1 .. 256; value_heads a multiple of key_heads;
  * n_frames at most 2^30; n_streams * value_heads * ceil(dv / 16) below 2^31.
  */
-#define NNSP_DELTA_STEP_FRAMES 8
+#define NNSP_DELTA_STEP_FRAMES 2
 typedef struct {
     int32_t dtype;
     int32_t n_streams, n_frames;      /* S, T (0: nothing but the state's copy) */

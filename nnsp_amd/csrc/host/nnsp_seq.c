@@ -155,15 +155,30 @@ int nnsp_delta_contiguous(nnsp_delta_args *a)
     return 0;
 }
 
-/* How a call runs: frame by frame (few frames, or heads too wide for the matrix
- * kernels' LDS), in chunks, or in chunks in two passes.  */
+/* How a call runs: frame by frame, in chunks, or in chunks in two passes. */
 enum { DELTA_STEP, DELTA_CHUNK, DELTA_SPLIT };
 
 static int delta_way(const nnsp_delta_args *a)
 {
-    if (a->n_frames <= NNSP_DELTA_STEP_FRAMES || a->dk > NNSP_DELTA_CHUNK_DK) return DELTA_STEP;
-    const long long rows = (long long)a->n_streams * a->value_heads * ((a->dv + 127) / 128);
-    return rows <= 128 && a->n_frames > 64 ? DELTA_SPLIT : DELTA_CHUNK;
+    /* A frame costs 0.8 to 3.3 us by itself, a chunk 7 to 13 us whatever it
+     * holds, and rows of 32 little more by frames.  bf16, 4096 rows, frames
+     * against a chunk in us: dk = dv = 32, 8 frames 28 against 38, 12 frames 37
+     * against 38; 64, 4 frames 43 against 45, 6 frames 54 against 44; 128, 2
+     * frames 126 against 120, 4 frames 168 against 118.  One row, 4 frames: 8.6
+     * against 7.0, 9.6 against 7.7, 12.3 against 8.7. */
+    if (a->n_frames <= (a->dk <= 32 ? 8 : a->dk <= 96 ? 4 : NNSP_DELTA_STEP_FRAMES)) return DELTA_STEP;
+    /* Two passes shorten the chain of a call whose few rows leave CUs idle, and
+     * move twice the bytes.  bf16, dk = dv = 128, chunks against two passes in
+     * us: 64 rows (512 workgroups of 16 columns) 130 frames 29 against 30, 260
+     * frames 48 against 38, 1000 frames 156 against 71; 128 rows 260 frames 50
+     * against 58, 1000 frames 158 against 133; 192 rows 1000 frames 188 against
+     * 224.  fp32: 64 rows 1000 frames 182 against 106, 96 rows 184 against 183.
+     * LDS has no room for the first pass's 64 frames of fp32 wider than 128. */
+    const long long groups = (long long)a->n_streams * a->value_heads * ((a->dv + 15) / 16);
+    const int wide = a->dtype == NNSP_F32;
+    if (wide && a->dk > 128) return DELTA_CHUNK;
+    return (groups <= 512 && a->n_frames > 192) || (groups <= 1024 && a->n_frames > 512 && !wide) ? DELTA_SPLIT
+                                                                                                  : DELTA_CHUNK;
 }
 
 int nnsp_delta_workspace(const nnsp_delta_args *a, size_t *bytes)

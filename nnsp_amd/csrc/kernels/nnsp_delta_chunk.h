@@ -460,7 +460,7 @@ __device__ __forceinline__ void invert_diagonal(const TriA<C>& A, Diag<C>& D, in
 template <class T, int NKT>
 __device__ __forceinline__ void make_tp(const KQ<T, NKT, 64>& X, TP<T, 64>& Y, Make<64>& M, Diag<64>& D, TriA<64>& A, int wave,
                                         int lane) {
-    constexpr int KP = KQ<T, NKT, 64>::KP, OP = TP<T, 64>::OP;
+    constexpr int KP = KQ<T, NKT, 64>::KP;
     const int l15 = lane & 15, g = lane >> 4;
     f32x4 acc[4];
 #pragma unroll
@@ -708,10 +708,24 @@ struct Chunk {
     }
 };
 
-// f(t, j, r, base, at, in) for element r of accumulator tile (t, j): its place base
-// + at in the head's state (base the same for all lanes), kept inside it, and
-// whether it is one of it
-template <int NKT, int NB, class F>
+// Where element r of accumulator tile t, j lies in the head's state: base + at,
+// base the same for all lanes, `at` kept inside the state, `in` if it is one of it.
+// live: the tile has any.  FAST: dk and dv are multiples of 8.
+struct Spot {
+    int base;
+    unsigned at;
+    bool in, live;
+};
+template <bool FAST>
+__device__ __forceinline__ Spot spot(const nnsp_delta_args& a, int c0, int t, int j, int r, int lane) {
+    const int l15 = lane & 15, g = lane >> 4, r0 = 32 * (t >> 1), row = r0 + 4 * (t & 1) + r, col = c0 + 16 * j;
+    if (FAST)
+        return {row * a.dv + col, (unsigned)(min(8 * g, a.dk - 8 - r0) * a.dv + min(l15, a.dv - 1 - col)),
+                r0 + 8 * g < a.dk && col + l15 < a.dv, r0 < a.dk && col < a.dv};
+    return {0, (unsigned)(min(row + 8 * g, a.dk - 1) * a.dv + min(col + l15, a.dv - 1)), row + 8 * g < a.dk && col + l15 < a.dv, true};
+}
+// f(t, j, r, base, at, in) for all a wave has that are live
+template <int NKT, int NB, bool FAST, class F>
 __device__ __forceinline__ void each_state(const nnsp_delta_args& a, int c0, int lane, const F& f) {
     const int l15 = lane & 15, g = lane >> 4;
     if (a.dk == 32 * NKT && c0 + 16 * NB <= a.dv) {
@@ -726,12 +740,14 @@ __device__ __forceinline__ void each_state(const nnsp_delta_args& a, int c0, int
 #pragma unroll
         for (int j = 0; j < NB; ++j)
 #pragma unroll
-            for (int t = 0; t < 2 * NKT; ++t)
+            for (int t = 0; t < 2 * NKT; ++t) {
+                if (!spot<FAST>(a, c0, t, j, 0, lane).live) continue;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int row = 32 * (t >> 1) + 4 * (t & 1) + r + 8 * g, col = c0 + 16 * j + l15;
-                    f(t, j, r, 0, (unsigned)(min(row, a.dk - 1) * a.dv + min(col, a.dv - 1)), row < a.dk && col < a.dv);
+                    const Spot p = spot<FAST>(a, c0, t, j, r, lane);
+                    f(t, j, r, p.base, p.at, p.in);
                 }
+            }
     }
 }
 
@@ -877,11 +893,17 @@ __device__ __forceinline__ int frames_of(const nnsp_delta_args& a, int s) {
     return a.lens ? max(0, min(a.lens[s], a.n_frames)) : a.n_frames;
 }
 
+// waves per SIMD that the state and the operands leave registers and LDS for
+template <class T, int NKT, int NB, int NW>
+constexpr int fused_waves() {
+    return Geo<T, NKT, NB>::WIDE && NKT > 4 && NW == 4 ? 1 : Geo<T, NKT, NB>::WIDE || NB == 2 || NKT > 4 ? 2 : 3;
+}
+
 // Many streams: a workgroup per stream, head and 16 NB NW columns goes through its
 // chunks of 32 alone, and the workgroups of a CU fill each other's waits.
 // FAST: dk and dv are multiples of 8.
 template <class T, int NKT, int NB, int NW, bool FAST>
-__global__ __launch_bounds__(64 * NW, (Geo<T, NKT, NB>::WIDE || NB == 2 ? 2 : 3)) void delta_chunk_kernel(const nnsp_delta_args a) {
+__global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delta_chunk_kernel(const nnsp_delta_args a) {
     using G = Geo<T, NKT, NB>;
     struct Lds {
         KQ<T, NKT, CF> X;
@@ -901,11 +923,17 @@ __global__ __launch_bounds__(64 * NW, (Geo<T, NKT, NB>::WIDE || NB == 2 ? 2 : 3)
 
     f32x4 S[2 * NKT][NB];
     float sinv = 1.0f;
-    const float* sp = a.state_in + so;
-    each_state<NKT, NB>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
-        const float x = a.state_in ? (sp + base)[at] : 0.0f;
-        S[t][j][r] = in ? x : 0.0f;
-    });
+#pragma unroll
+    for (int t = 0; t < 2 * NKT; ++t)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) S[t][j] = f32x4{0, 0, 0, 0};
+    if (a.state_in) {
+        const float* sp = a.state_in + so;
+        each_state<NKT, NB, FAST>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
+            const float x = (sp + base)[at];
+            S[t][j][r] = in ? x : 0.0f;
+        });
+    }
     Rows<T, NKT, CF, 2 * NW, FAST> rows(a, s, h, 0, tid, wave);
     Cols<T, NKT, NB, FAST, CF, CF> cols(a, s, h, 0, c0, lane);
     if (n > 0) {
@@ -946,7 +974,7 @@ __global__ __launch_bounds__(64 * NW, (Geo<T, NKT, NB>::WIDE || NB == 2 ? 2 : 3)
     }
     if (a.state_out) {
         float* sq = a.state_out + so;
-        each_state<NKT, NB>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
+        each_state<NKT, NB, FAST>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
             if (in) (sq + base)[at] = S[t][j][r] * sinv;
         });
     }
@@ -972,7 +1000,7 @@ __device__ __forceinline__ void copy_out(char* dst, const X& src, int tid) {
 
 // One workgroup per stream, key head and chunk, for all the key head's value heads.
 template <class T, int NKT, bool FAST>
-__global__ __launch_bounds__(256, 2) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
+__global__ __launch_bounds__(256, (sizeof(KQ<T, NKT, C>) > 48 * 1024 ? 1 : 2)) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
     struct Lds {
         KQ<T, NKT, C> X;
         Make<C> M;
@@ -1098,26 +1126,30 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
     const f32x4 zero = {0, 0, 0, 0};
     f32x4 S[TPW][NB];
     float sinv = 1.0f, m = 0.0f;
-    // f(i, j, r, at, in) for element r of tile (i, j), as each_state
+    // f(i, j, r, place, in) for element r of this wave's tile (i, j), as each_state
     const auto own_state = [&](int lane, const auto& f) {
-        const int l15 = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int i = 0; i < TPW; ++i) {
-            const int t = wave * TPW + i;
+        for (int i = 0; i < TPW; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
+            for (int j = 0; j < NB; ++j) {
+                if (!spot<FAST>(a, c0, wave * TPW + i, j, 0, lane).live) continue;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int rw = 32 * (t >> 1) + 4 * (t & 1) + r + 8 * g, col = c0 + 16 * j + l15;
-                    f(i, j, r, min(rw, a.dk - 1) * a.dv + min(col, a.dv - 1), rw < a.dk && col < a.dv);
+                    const Spot p = spot<FAST>(a, c0, wave * TPW + i, j, r, lane);
+                    f(i, j, r, so + p.base + p.at, p.in);
                 }
-        }
+            }
     };
-    own_state(lane_, [&](int i, int j, int r, int at, bool in) {
-        const float x = b.state_in ? (b.state_in + so)[at] : 0.0f;
-        S[i][j][r] = in ? x : 0.0f;
-        m = fmaxf(m, fabsf(S[i][j][r]));
-    });
+#pragma unroll
+    for (int i = 0; i < TPW; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) S[i][j] = zero;
+    if (b.state_in)
+        own_state(lane_, [&](int i, int j, int r, long long at, bool in) {
+            const float x = b.state_in[at];
+            S[i][j][r] = in ? x : 0.0f;
+            m = fmaxf(m, fabsf(S[i][j][r]));
+        });
     m = wave_max(m);
     if (lane_ == 0) L.E.smax[wave] = m;
     __syncthreads();
@@ -1288,8 +1320,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
         if (BUFS == 1) __syncthreads();
     }
     if (b.state_out)
-        own_state(here(lane_), [&](int i, int j, int r, int at, bool in) {
-            if (in) (b.state_out + so)[at] = S[i][j][r] * sinv;
+        own_state(here(lane_), [&](int i, int j, int r, long long at, bool in) {
+            if (in) b.state_out[at] = S[i][j][r] * sinv;
         });
 }
 
@@ -1349,11 +1381,14 @@ auto with_sizes(const nnsp_delta_args& a, const F& f) {
     typedef std::integral_constant<int, 2> I2;
     typedef std::integral_constant<int, 3> I3;
     typedef std::integral_constant<int, 4> I4;
-    if ((a.dk | a.dv) & 7) return a.dk <= 64 ? f(I2(), std::false_type()) : f(I4(), std::false_type());
+    typedef std::integral_constant<int, 8> I8;
+    if ((a.dk | a.dv) & 7)
+        return a.dk <= 64 ? f(I2(), std::false_type()) : a.dk <= 128 ? f(I4(), std::false_type()) : f(I8(), std::false_type());
     if (a.dk <= 32) return f(I1(), std::true_type());
     if (a.dk <= 64) return f(I2(), std::true_type());
     if (a.dk <= 96) return f(I3(), std::true_type());
-    return f(I4(), std::true_type());
+    if (a.dk <= 128) return f(I4(), std::true_type());
+    return f(I8(), std::true_type());
 }
 
 template <class T>
@@ -1366,9 +1401,18 @@ int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
     with_sizes(a, [&](auto nkt, auto fast) {
         constexpr int NKT = decltype(nkt)::value;
         constexpr bool FAST = decltype(fast)::value;
-        if (split) launch_split<T, NKT, FAST>(a, st);
-        else if (a.dv <= 64) launch_fused<T, NKT, 1, 4, FAST>(a, st);
-        else launch_fused<T, NKT, Geo<T, NKT, 1>::WIDE ? 1 : 2, Geo<T, NKT, 1>::WIDE ? 8 : 4, FAST>(a, st);
+        constexpr bool WIDE = Geo<T, NKT, 1>::WIDE;
+        // the first pass has no room in LDS for an image of 64 fp32 frames wider than 128
+        if constexpr (!WIDE || NKT <= 4) {
+            if (split) {
+                launch_split<T, NKT, FAST>(a, st);
+                return 0;
+            }
+        }
+        const bool narrow = a.dv <= 64 || (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64) <= 256;
+        if constexpr (WIDE) narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 1, 8, FAST>(a, st);
+        else if constexpr (NKT > 4) launch_fused<T, NKT, 1, 4, FAST>(a, st);
+        else narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 2, 4, FAST>(a, st);
         return 0;
     });
     return (int)hipGetLastError();

@@ -11,12 +11,11 @@ extern "C" {
 
 /* largest head width of the delta rule and row length of the norms */
 #define NNSP_DELTA_MAX_D 256
-#define NNSP_DELTA_CHUNK_DK 128
 #define NNSP_NORM_MAX_DIM 16384
 
 int nnspk_launch_delta_step(const nnsp_delta_args *a, void *stream);
-/* dk <= NNSP_DELTA_CHUNK_DK; split: in two passes over the workspace, of
- * nnspk_delta_split_bytes_*() bytes */
+/* split: in two passes over the workspace, of nnspk_delta_split_bytes_*() bytes
+ * (not of fp32 with dk > 128) */
 int nnspk_launch_delta_chunk_f32(const nnsp_delta_args *a, int split, void *stream);
 int nnspk_launch_delta_chunk_bf16(const nnsp_delta_args *a, int split, void *stream);
 int nnspk_launch_delta_chunk_f16(const nnsp_delta_args *a, int split, void *stream);

@@ -272,6 +272,37 @@ def test_delta_many_streams_and_slabs(S, T, hk, hv, dk, dv, dtype):
     close(so, rs, "f32", T, dk, "state")
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("S,T,hk,hv,dk,dv", [
+    (3, 3, 1, 2, 136, 24), (2, 40, 1, 2, 256, 256), (1, 33, 2, 2, 144, 200), (2, 64, 1, 1, 129, 100), (1, 31, 1, 1, 250, 7),
+    (600, 37, 1, 1, 160, 128), (1100, 66, 1, 1, 200, 64), (3, 300, 1, 2, 256, 72), (2, 560, 4, 8, 192, 144), (1, 200, 1, 3, 133, 61),
+])
+def test_delta_wide_keys(S, T, hk, hv, dk, dv, dtype):
+    d = make(S, T, hk, hv, dk, dv, dtype, seed=S + T)
+    out, so = run_delta(d, hk, dtype)
+    ro, rs = delta_ref_all(d, True, dk ** -0.5)
+    close(out, ro, dtype, T, dk, "out")
+    close(so, rs, "f32", T, dk, "state")
+
+
+@pytest.mark.parametrize("S,T,hk,hv,dk,dv,dtype", [
+    (2, 1800, 32, 32, 128, 128, "bf16"), (2, 1100, 32, 32, 128, 128, "f32"), (1, 1700, 16, 32, 256, 144, "f16"),
+    (12, 1300, 8, 8, 128, 104, "bf16"),
+])
+def test_delta_two_passes_over_several_slabs(S, T, hk, hv, dk, dv, dtype):
+    d = make(S, T, hk, hv, dk, dv, dtype, seed=S)
+    lens = [max(0, T - 700 * i) for i in range(S)]
+    out, so = run_delta(d, hk, dtype, lens=lens)
+    whole = {k: d[k] for k in d}
+    for s, n in enumerate(lens):  # frames that change nothing take the place of those behind a stream's end
+        whole["g"][s, n:], whole["beta"][s, n:] = 0, 0
+    ro, rs = delta_ref_all(whole, True, dk ** -0.5)
+    for s, n in enumerate(lens):
+        assert bool((out[s, n:] == 7).all())
+        close(out[s, :n], ro[s, :n], dtype, T, dk, f"out {s}")
+    close(so, rs, "f32", T, dk, "state")
+
+
 @pytest.mark.parametrize("state", [True, False])
 def test_delta_slabs_ragged(state):
     """Streams that end in the first slab, in the middle and in the last; the final state dropped or kept."""
