@@ -6,12 +6,12 @@
 namespace {
 
 // ---- gated delta rule, one frame after another ------------------------------
-// Columns of the state are independent, so a wave takes 32 columns of one
-// stream and head and keeps them in registers for all the call's frames: lane
-// (rg, cl) = (lane / 8, lane % 8) holds rows rg * RK .. rg * RK + RK - 1 of
-// columns 4 cl .. 4 cl + 3.  The state's read and write (8 dk dv bytes per
-// stream and head) are what a single frame costs; a wave issues its RK 16-byte
-// loads per lane (128-byte lines) before anything else.
+// Columns of the state are independent, so a wave takes 4 CL columns of one
+// stream and head and keeps them in registers for all the call's frames: CL
+// lanes side by side hold 4 columns each, and 64 / CL groups of them RK rows
+// each.  The state's read and write (8 dk dv bytes per stream and head) are what
+// a single frame costs; a wave issues its RK 16-byte loads per lane before
+// anything else.
 //
 // With S the state before the frame, o = scale (d S^T q + (k . q) u): both
 // products with S and the three scalar products are summed over the row groups
@@ -22,45 +22,84 @@ struct FrameRaw {
     float g, beta;
 };
 
+// x[j + sh], 0 beyond x[3]
+template <class T>
+__device__ __forceinline__ void shifted(T (&x)[4], int sh) {
+    if constexpr (sizeof(T) == 2) {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        const t4 v = {x[0], x[1], x[2], x[3]};
+        const t4 r = __builtin_bit_cast(t4, sh < 4 ? __builtin_bit_cast(unsigned long long, v) >> (16 * (sh & 3)) : 0ull);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = r[j];
+    } else {
+#pragma unroll
+        for (int b = 1; b <= 4; b *= 2)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (sh & b || sh > 4) x[j] = j + b < 4 ? x[j + b] : (T)0.0f;
+    }
+}
+
+// elements r0 .. r0 + RK - 1 of n, zeros beyond them
 template <class T, int RK>
-__device__ __forceinline__ void load_rows(T (&d)[RK], const T* p, int r0, int n, bool vec) {
-    if (vec) {
+__device__ __forceinline__ void load_rows(T (&d)[RK], const T* p, int r0, int n) {
+    if (RK % 4 == 0 && (n & 3) == 0) {
 #pragma unroll
         for (int c = 0; c < RK; c += 4) {
             T x[4];
-            load_raw(x, p + min(r0 + c, n - 4));
+            load_raw(x, p + (unsigned)min(r0 + c, n - 4));
 #pragma unroll
             for (int j = 0; j < 4; ++j) d[c + j] = r0 + c < n ? x[j] : (T)0.0f;
+        }
+    } else if (n >= 4) {
+#pragma unroll
+        for (int c = 0; c < RK; c += 4) {
+            T x[4];
+            const int at = min(r0 + c, n - 4);
+            load_raw(x, p + (unsigned)at);
+            shifted(x, r0 + c - at);
+#pragma unroll
+            for (int j = 0; j < 4 && c + j < RK; ++j) d[c + j] = x[j];
         }
     } else {
 #pragma unroll
         for (int c = 0; c < RK; ++c) {
-            const T x = p[min(r0 + c, n - 1)];
+            const T x = p[(unsigned)min(r0 + c, n - 1)];
             d[c] = r0 + c < n ? x : (T)0.0f;
         }
     }
 }
 
+// columns c0 .. c0 + 3 of n of the row at p + row (p the same for all lanes)
 template <class T>
-__device__ __forceinline__ void load_cols(T (&d)[4], const T* p, int c0, int n, bool vec) {
+__device__ __forceinline__ void load_cols(T (&d)[4], const T* p, unsigned row, int c0, int n, bool vec) {
     if (vec) {
-        load_raw(d, p + min(c0, n - 4));
+        load_raw(d, p + (row + c0));
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[j] = p[min(c0 + j, n - 1)];
+        for (int j = 0; j < 4; ++j) d[j] = p[row + min(c0 + j, n - 1)];
     }
 }
 
-template <class T, int RK>
+// FULL: dk is 64 / CL RK and dv a multiple of 4
+template <class T, int RK, int CL, bool FULL>
 __global__ __launch_bounds__(256) void delta_step_kernel(const nnsp_delta_args a) {
+    static_assert(CL == 8 || CL == 4, "");
     const int lane = threadIdx.x & 63;
-    const int ncb = (a.dv + 31) >> 5;
-    const unsigned unit = blockIdx.x * 4u + (threadIdx.x >> 6);
+    const int ncb = (a.dv + 4 * CL - 1) / (4 * CL);
+    // where the waves of a head share 128-byte lines of its state, a range of its own for each of the 8 XCDs, so that
+    // they share an L2 as well (dk = dv = 72: 3.6 -> 4.0 TB/s; without such lines it costs 2 %)
+    const bool ranges = a.dv > 4 * CL && a.dv % 32;
+    const unsigned block = ranges ? (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x;
+    const unsigned unit = block * 4u + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (unit >= (unsigned)a.n_streams * a.value_heads * ncb) return;
     const int cb = unit % ncb, h = (unit / ncb) % a.value_heads, s = unit / ncb / a.value_heads;
     const int hk = h / (a.value_heads / a.key_heads);
-    const int r0 = (lane >> 3) * RK, c0 = cb * 32 + (lane & 7) * 4;
-    const bool vk = (a.dk & 3) == 0, vv = (a.dv & 3) == 0;
+    const int rg = CL == 8 ? lane >> 3 : (lane & 3) | (lane >> 4) << 2, cl = CL == 8 ? lane & 7 : (lane >> 2) & 3;
+    const int r0 = rg * RK, own = cb * 4 * CL + cl * 4;
+    // a wave that has 4 columns: lanes whose 4 go past the last take the last 4, the same as others of the wave
+    const bool vv = FULL || a.dv - cb * 4 * CL >= 4;
+    const int c0 = vv ? min(own, a.dv - 4) : own;
 
     const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
     float S[RK][4];
@@ -69,9 +108,9 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const nnsp_delta_args a
 #pragma unroll
         for (int r = 0; r < RK; ++r) {
             float x[4];
-            load_cols(x, p + (long long)min(r0 + r, a.dk - 1) * a.dv, c0, a.dv, vv);
+            load_cols(x, FULL ? p + r * a.dv : p, (FULL ? r0 : min(r0 + r, a.dk - 1)) * a.dv, c0, a.dv, vv);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) S[r][j] = r0 + r < a.dk ? x[j] : 0.0f;
+            for (int j = 0; j < 4; ++j) S[r][j] = FULL || r0 + r < a.dk ? x[j] : 0.0f;
         }
     } else {
 #pragma unroll
@@ -86,13 +125,13 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const nnsp_delta_args a
     const T* vp = (const T*)a.v + s * a.v_stride[0] + h * a.v_stride[2];
     const float* gp = a.g ? a.g + s * a.g_stride[0] + h * a.g_stride[2] : nullptr;
     const float* bp = a.beta + s * a.beta_stride[0] + h * a.beta_stride[2];
-    T* op = (T*)a.out + s * a.out_stride[0] + h * a.out_stride[2] + c0;
+    T* op = (T*)a.out + s * a.out_stride[0] + h * a.out_stride[2];
 
     FrameRaw<T, RK> raw;
     const auto fetch = [&](long long t) {
-        load_rows(raw.k, kp + t * a.k_stride[1], r0, a.dk, vk);
-        load_rows(raw.q, qp + t * a.q_stride[1], r0, a.dk, vk);
-        load_cols(raw.v, vp + t * a.v_stride[1], c0, a.dv, vv);
+        load_rows(raw.k, kp + t * a.k_stride[1], r0, a.dk);
+        load_rows(raw.q, qp + t * a.q_stride[1], r0, a.dk);
+        load_cols(raw.v, vp + t * a.v_stride[1], 0, c0, a.dv, vv);
         raw.g = gp ? gp[t * a.g_stride[1]] : 0.0f;
         raw.beta = bp[t * a.beta_stride[1]];
     };
@@ -122,11 +161,11 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const nnsp_delta_args a
                     sq[j] = fmaf(S[r][j], q[r], sq[j]);
                 }
             }
-            const auto sum8 = [](float x) { return add_xor32(add_xor16(add_xor8(x))); };
+            const auto rows_sum = [](float x) { return add_xor32(add_xor16(CL == 8 ? add_xor8(x) : add_xor2(add_xor1(x)))); };
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sk[j] = sum8(sk[j]), sq[j] = sum8(sq[j]);
-            kq = sum8(kq);
-            if (a.l2norm) kk = sum8(kk), qq = sum8(qq);
+            for (int j = 0; j < 4; ++j) sk[j] = rows_sum(sk[j]), sq[j] = rows_sum(sq[j]);
+            kq = rows_sum(kq);
+            if (a.l2norm) kk = rows_sum(kk), qq = rows_sum(qq);
         };
         sums();
         float rk = 1.0f, rq = 1.0f;
@@ -157,45 +196,60 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const nnsp_delta_args a
         for (int r = 0; r < RK; ++r)
 #pragma unroll
             for (int j = 0; j < 4; ++j) S[r][j] = fmaf(k[r], u[j], dec * S[r][j]);
-        if (lane < 8) {
+        if (rg == 0) {
             T* p = op + t * a.out_stride[1];
             if (vv) {
-                if (c0 < a.dv) store_vec(p, o);
+                if (own < a.dv) store_vec(p + (unsigned)c0, o);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (c0 + j < a.dv) p[j] = (T)o[j];
+                    if (c0 + j < a.dv) p[(unsigned)(c0 + j)] = (T)o[j];
             }
         }
     }
     if (a.state_out) {
-        float* p = a.state_out + so + c0;
+        float* p = a.state_out + so;
 #pragma unroll
         for (int r = 0; r < RK; ++r) {
-            if (r0 + r >= a.dk) continue;
-            float* row = p + (long long)(r0 + r) * a.dv;
+            if (!FULL && r0 + r >= a.dk) continue;
+            float* base = FULL ? p + r * a.dv : p;
+            const unsigned row = (FULL ? r0 : r0 + r) * a.dv;
             if (vv) {
-                if (c0 < a.dv) store_vec(row, S[r]);
+                if (own < a.dv) store_vec(base + (row + c0), S[r]);
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (c0 + j < a.dv) row[j] = S[r][j];
+                    if (c0 + j < a.dv) base[row + c0 + j] = S[r][j];
             }
         }
     }
 }
 
+// N rows a lane at least, of the few counts there are kernels for
+template <class T, int CL, int N>
+bool launch_step_rows(const nnsp_delta_args& a, hipStream_t st) {
+    if (a.dk > 64 / CL * N) return false;
+    const long long units = (long long)a.n_streams * a.value_heads * ((a.dv + 4 * CL - 1) / (4 * CL));
+    const dim3 grid((unsigned)((units + 31) / 32 * 8)), block(256);  // a multiple of the 8 XCDs
+    if constexpr (N % 4 == 0 || N > 8)
+        if (a.dk == 64 / CL * N && a.dv % 4 == 0) {
+            delta_step_kernel<T, N, CL, true><<<grid, block, 0, st>>>(a);
+            return true;
+        }
+    delta_step_kernel<T, N, CL, false><<<grid, block, 0, st>>>(a);
+    return true;
+}
+// Groups of 8 lanes read a row of the state by whole 128-byte lines (dk = dv =
+// 64: 4.6 TB/s, with groups of 4 4.1); above 128 rows groups of 4 halve the
+// registers a lane holds (144: 3.9 TB/s, with groups of 8 2.9).
+template <class T, int CL, int... N>
+void launch_step_of(const nnsp_delta_args& a, hipStream_t st) {
+    (void)(launch_step_rows<T, CL, N>(a, st) || ...);
+}
 template <class T>
 void launch_step(const nnsp_delta_args& a, hipStream_t st) {
-    const long long units = (long long)a.n_streams * a.value_heads * ((a.dv + 31) / 32);
-    const dim3 grid((unsigned)((units + 3) / 4)), block(256);
-    const int rk = (a.dk + 7) / 8;
-    if (rk <= 4) delta_step_kernel<T, 4><<<grid, block, 0, st>>>(a);
-    else if (rk <= 8) delta_step_kernel<T, 8><<<grid, block, 0, st>>>(a);
-    else if (rk <= 12) delta_step_kernel<T, 12><<<grid, block, 0, st>>>(a);
-    else if (rk <= 16) delta_step_kernel<T, 16><<<grid, block, 0, st>>>(a);
-    else if (rk <= 24) delta_step_kernel<T, 24><<<grid, block, 0, st>>>(a);
-    else delta_step_kernel<T, 32><<<grid, block, 0, st>>>(a);
+    if (a.dk <= 128) launch_step_of<T, 8, 1, 2, 3, 4, 5, 6, 8, 9, 10, 12, 14, 16>(a, st);
+    else launch_step_of<T, 4, 9, 10, 12, 14, 16>(a, st);
 }
 
 // ---- norms around a block ---------------------------------------------------
