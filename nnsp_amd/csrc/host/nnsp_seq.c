@@ -169,16 +169,16 @@ static int delta_way(const nnsp_delta_args *a)
     if (a->n_frames <= (a->dk <= 32 ? 8 : a->dk <= 96 ? 4 : NNSP_DELTA_STEP_FRAMES)) return DELTA_STEP;
     /* Two passes shorten the chain of a call whose few rows leave CUs idle, and
      * move twice the bytes.  bf16, dk = dv = 128, chunks against two passes in
-     * us: 64 rows (512 workgroups of 16 columns) 130 frames 29 against 30, 260
-     * frames 48 against 38, 1000 frames 156 against 71; 128 rows 260 frames 50
+     * us: 32 rows (256 workgroups of 16 columns) 130 frames 28 against 25; 64 rows
+     * 130 frames 29 against 30, 260 frames 48 against 38, 1000 frames 156 against 71; 128 rows 260 frames 50
      * against 58, 1000 frames 158 against 133; 192 rows 1000 frames 188 against
      * 224.  fp32: 64 rows 1000 frames 182 against 106, 96 rows 184 against 183.
      * LDS has no room for the first pass's 64 frames of fp32 wider than 128. */
     const long long groups = (long long)a->n_streams * a->value_heads * ((a->dv + 15) / 16);
     const int wide = a->dtype == NNSP_F32;
     if (wide && a->dk > 128) return DELTA_CHUNK;
-    return (groups <= 512 && a->n_frames > 192) || (groups <= 1024 && a->n_frames > 512 && !wide) ? DELTA_SPLIT
-                                                                                                  : DELTA_CHUNK;
+    const int from = groups <= 256 ? 128 : groups <= 512 ? 193 : groups <= 1024 && !wide ? 513 : INT32_MAX;
+    return a->n_frames >= from ? DELTA_SPLIT : DELTA_CHUNK;
 }
 
 int nnsp_delta_workspace(const nnsp_delta_args *a, size_t *bytes)

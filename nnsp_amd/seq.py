@@ -13,6 +13,7 @@ A plan is for one thread at a time; threads that call at once make one each.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import _lib
 
@@ -45,10 +46,11 @@ def _set_strides(args, strides: dict | None, names: tuple, dims: int) -> None:
             raise ValueError(f"strides of {name!r} {st} are out of range")
 
 
-def _fields(args, first: str, last: str):
-    """The 8-byte fields first .. last of a struct as one array (a call sets them all, in one go)."""
+def _packer(args, first: str, last: str):
+    """pack(buffer, 0, ...) and the buffer of a struct's 8-byte fields first .. last: a call sets them all in one go."""
     begin, end = getattr(type(args), first).offset, getattr(type(args), last).offset + 8
-    return (C.c_uint64 * ((end - begin) // 8)).from_buffer(args, begin)
+    return (struct.Struct(f"{(end - begin) // 8}Q").pack_into,
+            memoryview((C.c_char * (end - begin)).from_buffer(args, begin)))
 
 
 class GatedDelta:
@@ -67,7 +69,7 @@ class GatedDelta:
         a.l2norm, a.eps = int(bool(l2norm)), eps
         L = _lib.lib()
         self._ref, self._call = C.byref(a), L.nnsp_delta_exec_device
-        self._ptrs = _fields(a, "q", "workspace_bytes")
+        self._pack, self._ptrs = _packer(a, "q", "workspace_bytes")
         _lib.check(L.nnsp_delta_contiguous(self._ref), "nnsp_delta_contiguous")
         a.scale = dk ** -0.5 if scale is None else scale
         _set_strides(a, strides, ("q", "k", "v", "g", "beta", "out"), 3)
@@ -79,8 +81,8 @@ class GatedDelta:
                     state_out: int | None = None, lens: int | None = None, workspace: int | None = None,
                     stream: int | None = None) -> None:
         """One call; ``workspace``: workspace_bytes bytes of device memory."""
-        self._ptrs[:] = (q or 0, k or 0, v or 0, g or 0, beta or 0, lens or 0, state_in or 0, out or 0, state_out or 0,
-                         workspace or 0, self.workspace_bytes if workspace else 0)
+        self._pack(self._ptrs, 0, q or 0, k or 0, v or 0, g or 0, beta or 0, lens or 0, state_in or 0, out or 0,
+                   state_out or 0, workspace or 0, self.workspace_bytes if workspace else 0)
         rc = self._call(self._ref, stream)
         if rc:
             _lib.check(rc, "nnsp_delta_exec_device")
@@ -104,7 +106,7 @@ class BlockNorm:
         a.eps_pre, a.eps_post, a.res_scale = eps, eps if eps_post is None else eps_post, res_scale
         L = _lib.lib()
         self._ref, self._call = C.byref(a), L.nnsp_norm_exec_device
-        self._ptrs = _fields(a, "x", "y")
+        self._pack, self._ptrs = _packer(a, "x", "y")
         _lib.check(L.nnsp_norm_contiguous(self._ref), "nnsp_norm_contiguous")
         _set_strides(a, strides, ("x", "gate", "res_in", "res_out", "y"), 2)
 
@@ -112,8 +114,8 @@ class BlockNorm:
                     b_post: int | None = None, col_scale: int | None = None, w_pre: int | None = None,
                     b_pre: int | None = None, res_in: int | None = None, res_out: int | None = None,
                     stream: int | None = None) -> None:
-        self._ptrs[:] = (x or 0, gate or 0, res_in or 0, w_post or 0, b_post or 0, col_scale or 0, w_pre or 0, b_pre or 0,
-                         res_out or 0, y or 0)
+        self._pack(self._ptrs, 0, x or 0, gate or 0, res_in or 0, w_post or 0, b_post or 0, col_scale or 0, w_pre or 0,
+                   b_pre or 0, res_out or 0, y or 0)
         rc = self._call(self._ref, stream)
         if rc:
             _lib.check(rc, "nnsp_norm_exec_device")
