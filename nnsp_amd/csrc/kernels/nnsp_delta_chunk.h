@@ -130,8 +130,10 @@ __device__ __forceinline__ float scan_min(float x, int lane) {
     return lane < 16 ? x : fminf(x, lane < 32 ? a : lane < 48 ? m : fminf(m, b));
 }
 
-// keeps the operands of later products out of the registers until theirs are done
-__device__ __forceinline__ void no_hoist() { __builtin_amdgcn_sched_barrier(0); }
+// Everything this wave has asked of global memory is there.  Put before a loop
+// and before its stores, whose completion would otherwise be waited for together
+// with the loads that came before them.
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 // a copy the compiler knows nothing about: LDS addresses made of it are not
 // kept in registers from chunk to chunk
@@ -940,6 +942,7 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
         rows.fetch(a.dk, n);
         cols.fetch(n);
     }
+    wait_loads();
     for (int t0 = 0; t0 < n; t0 += CF) {
         const int left = n - t0, nt = left > 16 ? 2 : 1, ln = here(lane), l15 = ln & 15, g = ln >> 4;
         rows.stage(a, L.X, L.Y, L.M);
@@ -969,6 +972,7 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
         }
         __syncthreads();
         c.second(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
+        wait_loads();
         cols.store(L.V[wave], left);
         __syncthreads();
     }
@@ -1035,14 +1039,19 @@ __global__ __launch_bounds__(256, (sizeof(KQ<T, NKT, C>) > 48 * 1024 ? 1 : 2)) v
     }
 }
 
-// an image into LDS, past the registers: waves `wave` of `waves`, 1 KB an instruction
-template <class X>
-__device__ __forceinline__ void copy_in(X& dst, const char* src, int wave, int waves, int lane) {
-    constexpr int N = sizeof(X) / 16;
-    for (int i = wave * 64; i < N; i += waves * 64)
-        if (i + lane < N)
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (long long)(i + lane) * 16),
-                                             (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(&dst) + i * 16), 16, 0, 0);
+// A chunk's two images, from `from` thirds of them to `to`, into LDS past the
+// registers: by waves `wave` of 4, 1 KB an instruction.
+template <class X, class Y>
+__device__ __forceinline__ void copy_in(X& x, const char* sx, Y& y, const char* sy, int from, int to, int wave, int lane) {
+    constexpr int NX = sizeof(X) / 16, NY = sizeof(Y) / 16, BX = (NX + 63) / 64, BLOCKS = BX + (NY + 63) / 64;
+    for (int b = BLOCKS * from / 3 + wave; b < BLOCKS * to / 3; b += 4) {
+        const bool first = b < BX;
+        const int i = (first ? b : b - BX) * 64;
+        if (i + lane < (first ? NX : NY))
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)((first ? sx : sy) + (long long)(i + lane) * 16),
+                (__attribute__((address_space(3))) void*)((first ? (char*)&x : (char*)&y) + i * 16), 16, 0, 0);
+    }
 }
 
 // a tile times its rows' factors, as half of the high and low B operand that it is part of
@@ -1080,7 +1089,10 @@ struct ScanLds {
 // each of waves 0 .. 3 does a quarter of every product: a tile of 16 frames in
 // K S0, T R, Q S0 and P U, a quarter of the state's rows in K^T U, handing its
 // results on through LDS (three barriers a chunk).  Waves 4 .. 7 bring the next
-// chunk's images meanwhile (BUFS 2; where LDS has room for one, all wait).
+// chunk's images meanwhile, a third after each barrier: all at once they hold up
+// the products' own reads of LDS (64 chunks of 128 x 128 bf16: 127 us, all after
+// the first barrier 148, none 121).  Where LDS has room for one chunk only (BUFS
+// 1) they come after the third barrier, when the images have been read.
 // Scales have to be the same for all four before anybody has seen all values:
 // they come from bounds (|R| <= bmax |v| + xmax |S|, |u| <= 64 2^30,
 // |S1| <= all |S0| + 64 2^15 |U fk|) over the magnitudes exchanged at the
@@ -1100,24 +1112,28 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
     if (wave >= 4) {
         const char* kq = b.kq + ((long long)s * a.key_heads + hk) * b.chunks * sizeof(KQ<T, NKT, C>);
         const char* tp = b.tp + ((long long)s * a.value_heads + h) * b.chunks * sizeof(TP<T, C>);
-        const auto load = [&](int i) {
-            copy_in(L.X[i], kq, wave - 4, 4, lane_);
-            copy_in(L.Y[i], tp, wave - 4, 4, lane_);
-            kq += sizeof(KQ<T, NKT, C>);
-            tp += sizeof(TP<T, C>);
+        const auto load = [&](int i, int from, int to) {
+            copy_in(L.X[i], kq, L.Y[i], tp, from, to, wave - 4, lane_);
+            if (to == 3) kq += sizeof(KQ<T, NKT, C>), tp += sizeof(TP<T, C>);
         };
-        if (n > 0) load(0);
-        __syncthreads();
+        // bare barriers: __syncthreads() would wait for the copies, which only the next chunk's first barrier has to
+        const auto barrier = [] {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+        };
+        if (n > 0) load(0, 0, 3);
+        barrier();
         for (int t0 = 0, i = 0; t0 < n; t0 += C) {
-            __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-            __syncthreads();                     // this chunk is here, and the one before done with its buffer (BUFS 2)
-            if (BUFS == 2 && n - t0 > C) load(i ^= 1);
-            __syncthreads();
-            __syncthreads();
-            if (BUFS == 1) {
-                __syncthreads();  // this chunk is done with the buffer
-                if (n - t0 > C) load(0);
-            }
+            wait_loads();
+            barrier();  // this chunk is here, and the one before done with its buffer (BUFS 2)
+            const bool more = n - t0 > C;
+            if (more) i ^= BUFS - 1;
+            if (BUFS == 2 && more) load(i, 0, 1);
+            barrier();
+            if (BUFS == 2 && more) load(i, 1, 2);
+            barrier();  // nothing reads this chunk's images any more (BUFS 1)
+            if (more) load(i, BUFS == 2 ? 2 : 0, 3);
         }
         return;
     }
@@ -1161,6 +1177,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
 
     Cols<T, NKT, NB, FAST, 16, C> cols(a, s, h, (long long)b.first * C + 16 * wave, c0, lane_);
     if (n > 0) cols.fetch(n - 16 * wave);
+    wait_loads();
     for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= BUFS - 1) {
         const int lane = here(lane_), l15 = lane & 15, g = lane >> 4, left = n - t0;
         const KQ<T, NKT, C>& X = L.X[i];
@@ -1316,8 +1333,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
 #pragma unroll
                 for (int r = 0; r < 4; ++r) L.V[wave][4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], O[n][r]);
         }
+        wait_loads();
         cols.store(L.V[wave], left - 16 * wave);
-        if (BUFS == 1) __syncthreads();
     }
     if (b.state_out)
         own_state(here(lane_), [&](int i, int j, int r, long long at, bool in) {
