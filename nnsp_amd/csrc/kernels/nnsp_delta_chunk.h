@@ -1039,12 +1039,14 @@ __global__ __launch_bounds__(256, (sizeof(KQ<T, NKT, C>) > 48 * 1024 ? 1 : 2)) v
     }
 }
 
-// A chunk's two images, from `from` thirds of them to `to`, into LDS past the
-// registers: by waves `wave` of 4, 1 KB an instruction.
-template <class X, class Y>
-__device__ __forceinline__ void copy_in(X& x, const char* sx, Y& y, const char* sy, int from, int to, int wave, int lane) {
+// Part `part` (0, 1, 2) of a chunk's two images into LDS past the registers, by
+// waves `wave` of 4, 1 KB an instruction: a third each; of one buffer only for Y,
+// half of X twice and then Y; of one buffer for both, all at the end.
+template <int XB, int YB, class X, class Y>
+__device__ __forceinline__ void copy_in(X& x, const char* sx, Y& y, const char* sy, int part, int wave, int lane) {
     constexpr int NX = sizeof(X) / 16, NY = sizeof(Y) / 16, BX = (NX + 63) / 64, BLOCKS = BX + (NY + 63) / 64;
-    for (int b = BLOCKS * from / 3 + wave; b < BLOCKS * to / 3; b += 4) {
+    const auto bound = [](int p) { return p == 3 ? BLOCKS : YB == 2 ? BLOCKS * p / 3 : XB == 2 ? BX * p / 2 : 0; };
+    for (int b = bound(part) + wave; b < bound(part + 1); b += 4) {
         const bool first = b < BX;
         const int i = (first ? b : b - BX) * 64;
         if (i + lane < (first ? NX : NY))
@@ -1077,10 +1079,11 @@ struct Exchange {
     float smax[4], vmax[4], fmax[4];
 };
 
-template <class T, int NKT, int NB, int BUFS>
+// XB, YB: buffers of the two images
+template <class T, int NKT, int NB, int XB, int YB>
 struct ScanLds {
-    KQ<T, NKT, C> X[BUFS];
-    TP<T, C> Y[BUFS];
+    KQ<T, NKT, C> X[XB];
+    TP<T, C> Y[YB];
     Exchange<NKT, NB> E;
     alignas(16) T V[4][16][Geo<T, NKT, NB>::VS];
 };
@@ -1091,18 +1094,18 @@ struct ScanLds {
 // results on through LDS (three barriers a chunk).  Waves 4 .. 7 bring the next
 // chunk's images meanwhile, a third after each barrier: all at once they hold up
 // the products' own reads of LDS (64 chunks of 128 x 128 bf16: 127 us, all after
-// the first barrier 148, none 121).  Where LDS has room for one chunk only (BUFS
-// 1) they come after the third barrier, when the images have been read.
+// the first barrier 148, none 121).  Where LDS has no room for two of an image, it
+// comes after the third barrier, when the one before has been read.
 // Scales have to be the same for all four before anybody has seen all values:
 // they come from bounds (|R| <= bmax |v| + xmax |S|, |u| <= 64 2^30,
 // |S1| <= all |S0| + 64 2^15 |U fk|) over the magnitudes exchanged at the
 // barriers, looser than the largest value by 2^4 to 2^8.
-template <class T, int NKT, int NB, bool FAST, int BUFS>
+template <class T, int NKT, int NB, bool FAST, int XB, int YB>
 __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a, const Slab b) {
     using G = Geo<T, NKT, NB>;
     constexpr bool LOW = G::OP == 2;
     constexpr int TPW = (2 * NKT + 3) / 4;  // state tiles of a wave
-    __shared__ ScanLds<T, NKT, NB, BUFS> L;
+    __shared__ ScanLds<T, NKT, NB, XB, YB> L;
     const int lane_ = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // streams and key heads vary fastest: with a multiple of 8 of them, all workgroups that read an image are on one XCD
     const unsigned keys = (unsigned)a.n_streams * a.key_heads;
@@ -1112,9 +1115,9 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
     if (wave >= 4) {
         const char* kq = b.kq + ((long long)s * a.key_heads + hk) * b.chunks * sizeof(KQ<T, NKT, C>);
         const char* tp = b.tp + ((long long)s * a.value_heads + h) * b.chunks * sizeof(TP<T, C>);
-        const auto load = [&](int i, int from, int to) {
-            copy_in(L.X[i], kq, L.Y[i], tp, from, to, wave - 4, lane_);
-            if (to == 3) kq += sizeof(KQ<T, NKT, C>), tp += sizeof(TP<T, C>);
+        const auto load = [&](int i, int part) {
+            copy_in<XB, YB>(L.X[i & (XB - 1)], kq, L.Y[i & (YB - 1)], tp, part, wave - 4, lane_);
+            if (part == 2) kq += sizeof(KQ<T, NKT, C>), tp += sizeof(TP<T, C>);
         };
         // bare barriers: __syncthreads() would wait for the copies, which only the next chunk's first barrier has to
         const auto barrier = [] {
@@ -1122,18 +1125,17 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
         };
-        if (n > 0) load(0, 0, 3);
+        if (n > 0) load(0, 0), load(0, 1), load(0, 2);
         barrier();
-        for (int t0 = 0, i = 0; t0 < n; t0 += C) {
-            wait_loads();
-            barrier();  // this chunk is here, and the one before done with its buffer (BUFS 2)
+        for (int t0 = 0, i = 1; t0 < n; t0 += C, i ^= 1) {
             const bool more = n - t0 > C;
-            if (more) i ^= BUFS - 1;
-            if (BUFS == 2 && more) load(i, 0, 1);
+            wait_loads();
+            barrier();  // this chunk is here, and the one before done with its buffers
+            if (more) load(i, 0);
             barrier();
-            if (BUFS == 2 && more) load(i, 1, 2);
-            barrier();  // nothing reads this chunk's images any more (BUFS 1)
-            if (more) load(i, BUFS == 2 ? 2 : 0, 3);
+            if (more) load(i, 1);
+            barrier();  // nothing reads this chunk's images any more
+            if (more) load(i, 2);
         }
         return;
     }
@@ -1178,10 +1180,10 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
     Cols<T, NKT, NB, FAST, 16, C> cols(a, s, h, (long long)b.first * C + 16 * wave, c0, lane_);
     if (n > 0) cols.fetch(n - 16 * wave);
     wait_loads();
-    for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= BUFS - 1) {
+    for (int t0 = 0, i = 0; t0 < n; t0 += C, i ^= 1) {
         const int lane = here(lane_), l15 = lane & 15, g = lane >> 4, left = n - t0;
-        const KQ<T, NKT, C>& X = L.X[i];
-        const TP<T, C>& Y = L.Y[i];
+        const KQ<T, NKT, C>& X = L.X[i & (XB - 1)];
+        const TP<T, C>& Y = L.Y[i & (YB - 1)];
         Exchange<NKT, NB>& E = L.E;
         // 1: the state's parts, and what bounds R
         float inv;
@@ -1366,9 +1368,10 @@ DeltaSplit plan_split(const nnsp_delta_args& a) {
 
 template <class T, int NKT, int NB, bool FAST>
 void launch_scan(const nnsp_delta_args& a, const Slab& b, hipStream_t st) {
-    constexpr int BUFS = sizeof(ScanLds<T, NKT, NB, 2>) <= 160 * 1024 ? 2 : 1;
+    constexpr int LDS = 160 * 1024, YB = sizeof(ScanLds<T, NKT, NB, 2, 2>) <= LDS ? 2 : 1,
+                  XB = sizeof(ScanLds<T, NKT, NB, 2, YB>) <= LDS ? 2 : 1;
     const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 16 * NB - 1) / (16 * NB));
-    delta_scan_kernel<T, NKT, NB, FAST, BUFS><<<dim3((unsigned)grid), dim3(512), 0, st>>>(a, b);
+    delta_scan_kernel<T, NKT, NB, FAST, XB, YB><<<dim3((unsigned)grid), dim3(512), 0, st>>>(a, b);
 }
 
 template <class T, int NKT, bool FAST>
