@@ -160,24 +160,27 @@ enum { DELTA_STEP, DELTA_CHUNK, DELTA_SPLIT };
 
 static int delta_way(const nnsp_delta_args *a)
 {
-    /* A frame costs 0.8 to 3.3 us by itself, a chunk 7 to 13 us whatever it
-     * holds, and rows of 32 little more by frames.  bf16, 4096 rows, frames
-     * against a chunk in us: dk = dv = 32, 8 frames 28 against 38, 12 frames 37
-     * against 38; 64, 4 frames 43 against 45, 6 frames 54 against 44; 128, 2
-     * frames 126 against 120, 4 frames 168 against 118.  One row, 4 frames: 8.6
-     * against 7.0, 9.6 against 7.7, 12.3 against 8.7. */
+    /* A frame by itself costs 0.9 to 2 us after the first, a chunk of up to 32
+     * about 7 to 13 us whatever it holds; rows of dk = 32 cost little more frame
+     * by frame.  Frames against a chunk, bf16, us, 4096 rows: dk = dv = 32, 8
+     * frames 27 against 39; 64, 4 frames 42 against 45, 6 frames 50 against 45;
+     * 96, 4 frames 82 against 87, 6 frames 102 against 87; 128, 2 frames 121
+     * against 118, 4 frames 156 against 120.  One row, 4 frames: 32 8.4 against
+     * 6.9, 64 8.5 against 7.2, 128 10.9 against 8.6. */
     if (a->n_frames <= (a->dk <= 32 ? 8 : a->dk <= 96 ? 4 : NNSP_DELTA_STEP_FRAMES)) return DELTA_STEP;
     /* Two passes shorten the chain of a call whose few rows leave CUs idle, and
-     * move twice the bytes.  bf16, dk = dv = 128, chunks against two passes in
-     * us: 32 rows (256 workgroups of 16 columns) 130 frames 28 against 25; 64 rows
-     * 130 frames 29 against 30, 260 frames 48 against 38, 1000 frames 156 against 71; 128 rows 260 frames 50
-     * against 58, 1000 frames 158 against 133; 192 rows 1000 frames 188 against
-     * 224.  fp32: 64 rows 1000 frames 182 against 106, 96 rows 184 against 183.
-     * LDS has no room for the first pass's 64 frames of fp32 wider than 128. */
+     * move twice the bytes.  What counts is how many workgroups of 16 columns
+     * the second pass has for 256 CUs.  Chunks against two passes, dk = dv = 128,
+     * us.  bf16, 256 workgroups: 65 frames 19 against 22, 100 frames 24 against
+     * 22, 1000 frames 157 against 54; 512: 130 frames 29 against 30, 193 frames
+     * 38 against 33, 1000 frames 156 against 66; 1024: 260 frames 50 against 55,
+     * 500 frames 83 against 69; 1536: 2000 frames 365 against 408.  fp32, 512:
+     * 193 frames 44 against 43, 1000 frames 186 against 110; 768: 2000 frames
+     * 362 against 383.  LDS has no room for 64 frames of fp32 wider than 128. */
     const long long groups = (long long)a->n_streams * a->value_heads * ((a->dv + 15) / 16);
-    const int wide = a->dtype == NNSP_F32;
-    if (wide && a->dk > 128) return DELTA_CHUNK;
-    const int from = groups <= 256 ? 128 : groups <= 512 ? 193 : groups <= 1024 && !wide ? 513 : INT32_MAX;
+    const int fp32 = a->dtype == NNSP_F32;
+    if (fp32 && a->dk > 128) return DELTA_CHUNK;
+    const int from = groups <= 256 ? 100 : groups <= 512 ? 193 : groups <= 1024 && !fp32 ? 400 : INT32_MAX;
     return a->n_frames >= from ? DELTA_SPLIT : DELTA_CHUNK;
 }
 

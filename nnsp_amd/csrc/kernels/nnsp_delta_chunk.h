@@ -19,8 +19,9 @@
 // absolute terms, 2^-38 of the bound, so neither a loose bound nor a column much
 // smaller than its neighbours costs precision.  q and k go in with
 // their rows scaled too: fp16 and bf16 in one part (exact down to 2^-19 and
-// 2^-28 of a row's largest, to 2^-30 and 2^-39 of it below), fp32 in two.  All other factors (norms, decays, beta) multiply
-// in 32 bits outside the products.  For bf16 outputs the products that reach
+// 2^-28 of a row's largest, to 2^-30 and 2^-39 of it below), fp32 in two.  All
+// other factors (norms, decays, beta) multiply in 32 bits outside the products.
+// For bf16 outputs the products that reach
 // only the output (Q S0, P U) use one part of S0, P and U, 11 bits, below the
 // output's own 8.
 //
@@ -44,8 +45,11 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 
 // frames of a chunk: 64 where a chain of chunks is what takes time, 32 where
-// many streams fill the device and registers and LDS decide how well
+// many streams fill the device and registers and LDS decide how well (100 frames
+// of 8192 streams, 2 heads of 64 x 64: chunks of 64 667 us, of 32 607 us then)
 constexpr int C = 64, CF = 32;
+// images of a slab, inside the 256 MB cache behind the L2s (16384 frames of 32
+// heads of 128 x 128, us: 32 MB 703, 96 MB 633, 200 MB 619; fp32 932, 870, 892)
 constexpr long long DELTA_SLAB_BYTES = 96ll << 20;
 
 // sizes of a call in two passes
@@ -333,8 +337,8 @@ __device__ __forceinline__ f32x4 dot_tile(const _Float16 (*X)[C][KS], const _Flo
 }
 __device__ __forceinline__ f32x4 ld4(const float* p) { return *reinterpret_cast<const f32x4*>(p); }
 
-// Factors of the staged frames (of C / 64 waves' lanes each): part 0 those of A, part
-// 1 those of P, part 2 those of the products with the state.
+// Factors of the staged frames, a frame a lane (of a chunk of 32 twice): part 0
+// those of A, part 1 those of P, part 2 those of the products with the state.
 //
 // A decay between two frames of different 16s is a product of three that are
 // each at most 1 (to the end of the column's 16, between, from the start of
@@ -904,6 +908,13 @@ constexpr int fused_waves() {
 // Many streams: a workgroup per stream, head and 16 NB NW columns goes through its
 // chunks of 32 alone, and the workgroups of a CU fill each other's waits.
 // FAST: dk and dv are multiples of 8.
+//
+// 100 frames of 8192 streams, 2 heads of 64 x 64, fp16: 505 us, of which the bytes
+// alone would take 280; the vector units issue 68 % of the time (splits, factors,
+// addresses: some 680 instructions a wave and chunk, 38 of them matrix ones), at
+// three waves a SIMD.  512 streams of 4 heads of 128 x 128, bf16: 159 us, bytes
+// 98.  Where rows are few a chunk takes 4 to 6 us, most of it the chain staging
+// -> products -> inverse -> products.
 template <class T, int NKT, int NB, int NW, bool FAST>
 __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delta_chunk_kernel(const nnsp_delta_args a) {
     using G = Geo<T, NKT, NB>;
@@ -1002,7 +1013,10 @@ __device__ __forceinline__ void copy_out(char* dst, const X& src, int tid) {
         reinterpret_cast<f32x4*>(dst)[i] = reinterpret_cast<const f32x4*>(&src)[i];
 }
 
-// One workgroup per stream, key head and chunk, for all the key head's value heads.
+// One workgroup per stream, key head and chunk, for all the key head's value heads
+// (64 chunks of 16 key heads and 32 value heads, 128 wide, bf16: 40 us for 34 MB
+// in and 83 MB out; two workgroups a CU is what LDS has room for, and each waits
+// for the inverse's chain most of the time).
 template <class T, int NKT, bool FAST>
 __global__ __launch_bounds__(256, (sizeof(KQ<T, NKT, C>) > 48 * 1024 ? 1 : 2)) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
     struct Lds {
@@ -1088,7 +1102,8 @@ struct ScanLds {
     alignas(16) T V[4][16][Geo<T, NKT, NB>::VS];
 };
 
-// The chain through the chunks for 16 NB columns.  Its length is what counts, so
+// The chain through the chunks for 16 NB columns: about 2 us a chunk (128 x 128,
+// bf16), bound by the latency of its three exchanges.  Its length counts, so
 // each of waves 0 .. 3 does a quarter of every product: a tile of 16 frames in
 // K S0, T R, Q S0 and P U, a quarter of the state's rows in K^T U, handing its
 // results on through LDS (three barriers a chunk).  Waves 4 .. 7 bring the next
@@ -1389,6 +1404,8 @@ void launch_split(const nnsp_delta_args& a, hipStream_t st) {
         b.state_out = b.first + b.chunks < p.chunks ? carry : a.state_out;
         delta_prepare_kernel<T, NKT, FAST>
             <<<dim3((unsigned)((long long)a.n_streams * a.key_heads * b.chunks)), dim3(256), 0, st>>>(a, b);
+        // 16 columns a workgroup while each still has a CU to itself, else 32 (LDS has room for one workgroup): 1000
+        // frames of 128 x 128, bf16, us, 32 rows 55 and 65, 40 rows 83 and 66
         if (rows * ((a.dv + 15) / 16) <= 256) launch_scan<T, NKT, 1, FAST>(a, b, st);
         else launch_scan<T, NKT, 2, FAST>(a, b, st);
     }
@@ -1429,6 +1446,10 @@ int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
                 return 0;
             }
         }
+        // Columns of a workgroup: 64 where there are no more or where CUs are left over, else 128.  500 frames of 16 heads
+        // of 128 x 128, bf16, us: 128 rows by 64 columns 82, by 128 97; 192 rows 108, 99; 512 rows 190, 141; fp32: 128
+        // rows 96, 111; 192 rows 130, 114.  Keys over 128 leave registers for 64 in 16 bits (512 rows of 256 x 256, 200
+        // frames: 258 us, 128 by 8 waves 276).
         const bool narrow = a.dv <= 64 || (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64) <= 256;
         if constexpr (WIDE) narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 1, 8, FAST>(a, st);
         else if constexpr (NKT > 4) launch_fused<T, NKT, 1, 4, FAST>(a, st);

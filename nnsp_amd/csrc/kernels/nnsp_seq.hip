@@ -16,6 +16,11 @@ namespace {
 // With S the state before the frame, o = scale (d S^T q + (k . q) u): both
 // products with S and the three scalar products are summed over the row groups
 // together, one cross-lane reduction per frame.
+//
+// One frame of 8192 streams, 2 heads of 64 x 64: 102 us, 5.4 TB/s of states, q, k,
+// v and out, what a large copy reaches; of 128 streams, 32 heads of 128 x 128: 103
+// us, 5.2 TB/s.  A frame of one stream takes 6 us on the device, a launch's and
+// three dependent loads' latency.
 template <class T, int RK>
 struct FrameRaw {
     T k[RK], q[RK], v[4];
@@ -257,9 +262,16 @@ void launch_step(const nnsp_delta_args& a, hipStream_t st) {
 // thread), so each input is read once and each output written once; the call
 // is bound by those bytes, provided that a gate's exponential and reciprocal
 // are the hardware's (with their exact forms the vector units were the bound).
-// Rows up to 1024 elements take 8 .. 64 lanes of a wave, U rows each so that
-// more is in flight, and sum by lane permutes; longer ones a whole workgroup
-// and one LDS exchange per sum.
+// Rows up to 1024 elements take 8 .. 64 lanes of a wave and sum by lane permutes;
+// longer ones a whole workgroup and one LDS exchange per sum.  (Several short rows
+// a thread, for more loads in flight, were no faster: 262144 gated rows of 64
+// 17 us, four a thread 20.)
+//
+// 1638400 rows of 64, gated, bf16: 107 us, 5.9 TB/s; 8192 of 4096 with an fp32
+// residual: 79 us, 5.1 TB/s; 16384 of 2048 in fp32, gated: 119 us, 5.6 TB/s; a
+// large copy 4.9 to 5.4.  5000 layer norms of 1001 with gate, residual and
+// biases, fp16: 12 us, 4.1 TB/s; one row of 1024 3 us, a launch's and its loads'
+// latency.
 //
 // ROW_FULL: the row is 8 TPR NCH elements.  ROW_TAIL: the row ends within a
 // thread's chunk; that chunk then starts at n - 8, and what it has of the
@@ -369,31 +381,28 @@ __device__ __forceinline__ float sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-template <class T, class R, int TPR, int NCH, int U, int MODE>
+template <class T, class R, int TPR, int NCH, int MODE>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(const nnsp_norm_args a) {
     constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;  // rows of a workgroup at a time
     __shared__ float red[4 * (TPR > 64 ? TPR / 64 : 1)];
     RowSum<TPR> sum{red};
     const int tid = threadIdx.x % TPR, n = a.dim;
     const unsigned rows = (unsigned)a.rows * (unsigned)a.groups;
-    const unsigned row0 = blockIdx.x * (unsigned)(RPB * U) + threadIdx.x / TPR;  // < 2^31 + 2^10
+    const unsigned row = blockIdx.x * (unsigned)RPB + threadIdx.x / TPR;  // < 2^31 + 2^8
     Place<MODE> at[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) at[i] = Place<MODE>(i * TPR + tid, n);
-    typename Vec<T, 8>::raw x[U][NCH], z[U][NCH];
-    typename Vec<R, 8>::raw q[U][NCH];
+    typename Vec<T, 8>::raw x[NCH], z[NCH];
+    typename Vec<R, 8>::raw q[NCH];
+    // rows past the last read the last again (and store nothing)
+    const unsigned live = min(row, rows - 1);
+    long long ro = live, ri = 0;
+    if (a.groups > 1) ro = live / (unsigned)a.groups, ri = live % (unsigned)a.groups;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        // rows past the last read the last again (and store nothing)
-        const unsigned row = min(row0 + u * RPB, rows - 1);
-        long long ro = row, ri = 0;
-        if (a.groups > 1) ro = row / (unsigned)a.groups, ri = row % (unsigned)a.groups;
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            x[u][i] = at[i].load((const T*)a.x + ro * a.x_stride[0] + ri * a.x_stride[1]);
-            if (a.act != NNSP_GATE_NONE) z[u][i] = at[i].load((const T*)a.gate + ro * a.gate_stride[0] + ri * a.gate_stride[1]);
-            if (a.res_in) q[u][i] = at[i].load((const R*)a.res_in + ro * a.res_in_stride[0] + ri * a.res_in_stride[1]);
-        }
+    for (int i = 0; i < NCH; ++i) {
+        x[i] = at[i].load((const T*)a.x + ro * a.x_stride[0] + ri * a.x_stride[1]);
+        if (a.act != NNSP_GATE_NONE) z[i] = at[i].load((const T*)a.gate + ro * a.gate_stride[0] + ri * a.gate_stride[1]);
+        if (a.res_in) q[i] = at[i].load((const R*)a.res_in + ro * a.res_in_stride[0] + ri * a.res_in_stride[1]);
     }
     float wp[NCH][8], wn[NCH][8];
     const auto weights = [&](float (&w)[NCH][8], const float* p) {
@@ -414,69 +423,55 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(const nnsp_
     // in place and without a norm, nothing else keeps a wave's stores behind the others' loads of the same tail
     if (TPR > 64 && MODE == ROW_TAIL && a.post == NNSP_NORM_NONE) __syncthreads();
 
+    float h[NCH][8];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const unsigned row = row0 + u * RPB;
-        float h[NCH][8];
+    for (int i = 0; i < NCH; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i][j] = (float)x[i][j];
+    if (a.post != NNSP_NORM_NONE) norm_row<TPR, NCH, MODE>(h, a.post, a.eps_post, wp, a.b_post, at, n, sum);
+    if (a.act != NNSP_GATE_NONE)
 #pragma unroll
         for (int i = 0; i < NCH; ++i)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = (float)x[u][i][j];
-        if (a.post != NNSP_NORM_NONE) norm_row<TPR, NCH, MODE>(h, a.post, a.eps_post, wp, a.b_post, at, n, sum);
-        if (a.act != NNSP_GATE_NONE)
-#pragma unroll
-            for (int i = 0; i < NCH; ++i)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float g = (float)z[u][i][j], s = sigmoid<sizeof(T) == 4>(g);
-                    h[i][j] *= a.act == NNSP_GATE_SILU ? g * s : s;
-                }
-#pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            if (a.col_scale) {
-                const auto c = at[i].load(a.col_scale);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) h[i][j] *= c[j];
+            for (int j = 0; j < 8; ++j) {
+                const float g = (float)z[i][j], s = sigmoid<sizeof(T) == 4>(g);
+                h[i][j] *= a.act == NNSP_GATE_SILU ? g * s : s;
             }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) h[i][j] = a.res_in ? fmaf(a.res_scale, h[i][j], (float)q[u][i][j]) : a.res_scale * h[i][j];
+    for (int i = 0; i < NCH; ++i) {
+        if (a.col_scale) {
+            const auto c = at[i].load(a.col_scale);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] *= c[j];
         }
-        long long ro = row, ri = 0;
-        if (a.groups > 1) ro = row / (unsigned)a.groups, ri = row % (unsigned)a.groups;
-        if (a.res_out && row < rows) {
-            R* p = (R*)a.res_out + ro * a.res_out_stride[0] + ri * a.res_out_stride[1];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) h[i][j] = a.res_in ? fmaf(a.res_scale, h[i][j], (float)q[i][j]) : a.res_scale * h[i][j];
+    }
+    if (a.res_out && row < rows) {
+        R* p = (R*)a.res_out + ro * a.res_out_stride[0] + ri * a.res_out_stride[1];
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) at[i].store(p, h[i]);
+    }
+    if (a.y) {
+        if (a.pre != NNSP_NORM_NONE) norm_row<TPR, NCH, MODE>(h, a.pre, a.eps_pre, wn, a.b_pre, at, n, sum);
+        if (row < rows) {
+            T* p = (T*)a.y + ro * a.y_stride[0] + ri * a.y_stride[1];
 #pragma unroll
             for (int i = 0; i < NCH; ++i) at[i].store(p, h[i]);
         }
-        if (a.y) {
-            if (a.pre != NNSP_NORM_NONE) norm_row<TPR, NCH, MODE>(h, a.pre, a.eps_pre, wn, a.b_pre, at, n, sum);
-            if (row < rows) {
-                T* p = (T*)a.y + ro * a.y_stride[0] + ri * a.y_stride[1];
-#pragma unroll
-                for (int i = 0; i < NCH; ++i) at[i].store(p, h[i]);
-            }
-        }
     }
 }
 
-template <class T, class R, int TPR, int NCH, int U, int MODE>
-void launch_norm_as(const nnsp_norm_args& a, hipStream_t st) {
-    constexpr int PER = (TPR > 256 ? 1 : 256 / TPR) * U;
+template <class T, class R, int TPR, int NCH, int MODE>
+void launch_norm_mode(const nnsp_norm_args& a, hipStream_t st) {
+    constexpr int PER = TPR > 256 ? 1 : 256 / TPR;
     const long long rows = a.rows * a.groups;
-    norm_kernel<T, R, TPR, NCH, U, MODE><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(TPR > 256 ? TPR : 256), 0, st>>>(a);
+    norm_kernel<T, R, TPR, NCH, MODE><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(TPR > 256 ? TPR : 256), 0, st>>>(a);
 }
-
-// U rows a thread once that still leaves every CU its workgroups
-template <class T, class R, int TPR, int NCH, int U>
-void launch_norm_u(const nnsp_norm_args& a, hipStream_t st) {
-    const bool full = a.dim == 8 * TPR * NCH;
-    if (U > 1 && a.rows * a.groups >= 2048ll * (256 / TPR) * U) {
-        if (full) launch_norm_as<T, R, TPR, NCH, U, ROW_FULL>(a, st);
-        else launch_norm_as<T, R, TPR, NCH, U, ROW_TAIL>(a, st);
-    } else {
-        if (full) launch_norm_as<T, R, TPR, NCH, 1, ROW_FULL>(a, st);
-        else launch_norm_as<T, R, TPR, NCH, 1, ROW_TAIL>(a, st);
-    }
+template <class T, class R, int TPR, int NCH>
+void launch_norm_as(const nnsp_norm_args& a, hipStream_t st) {
+    if (a.dim == 8 * TPR * NCH) launch_norm_mode<T, R, TPR, NCH, ROW_FULL>(a, st);
+    else launch_norm_mode<T, R, TPR, NCH, ROW_TAIL>(a, st);
 }
 
 template <class T, class R>
@@ -490,16 +485,16 @@ void launch_norm_t(nnsp_norm_args a, hipStream_t st) {
         a.groups = 1;
     }
     const int nc = (a.dim + 7) / 8;  // chunks of 8 elements
-    if (a.dim < 8) launch_norm_as<T, R, 8, 1, 1, ROW_TINY>(a, st);
-    else if (nc <= 8) launch_norm_u<T, R, 8, 1, 4>(a, st);
-    else if (nc <= 16) launch_norm_u<T, R, 16, 1, 4>(a, st);
-    else if (nc <= 32) launch_norm_u<T, R, 32, 1, 4>(a, st);
-    else if (nc <= 64) launch_norm_u<T, R, 64, 1, 4>(a, st);
-    else if (nc <= 128) launch_norm_u<T, R, 64, 2, 2>(a, st);
-    else if (nc <= 256) launch_norm_u<T, R, 256, 1, 1>(a, st);
-    else if (nc <= 512) launch_norm_u<T, R, 256, 2, 1>(a, st);
-    else if (nc <= 1024) launch_norm_u<T, R, 512, 2, 1>(a, st);
-    else launch_norm_u<T, R, 1024, 2, 1>(a, st);
+    if (a.dim < 8) launch_norm_mode<T, R, 8, 1, ROW_TINY>(a, st);
+    else if (nc <= 8) launch_norm_as<T, R, 8, 1>(a, st);
+    else if (nc <= 16) launch_norm_as<T, R, 16, 1>(a, st);
+    else if (nc <= 32) launch_norm_as<T, R, 32, 1>(a, st);
+    else if (nc <= 64) launch_norm_as<T, R, 64, 1>(a, st);
+    else if (nc <= 128) launch_norm_as<T, R, 64, 2>(a, st);
+    else if (nc <= 256) launch_norm_as<T, R, 256, 1>(a, st);
+    else if (nc <= 512) launch_norm_as<T, R, 256, 2>(a, st);
+    else if (nc <= 1024) launch_norm_as<T, R, 512, 2>(a, st);
+    else launch_norm_as<T, R, 1024, 2>(a, st);
 }
 
 int ok(hipError_t e) { return e == hipSuccess ? 0 : (int)e; }
