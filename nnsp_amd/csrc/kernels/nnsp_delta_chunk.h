@@ -1013,10 +1013,10 @@ __device__ __forceinline__ void copy_out(char* dst, const X& src, int tid) {
         reinterpret_cast<f32x4*>(dst)[i] = reinterpret_cast<const f32x4*>(&src)[i];
 }
 
-// One workgroup per stream, key head and chunk, for all the key head's value heads
-// (64 chunks of 16 key heads and 32 value heads, 128 wide, bf16: 40 us for 34 MB
-// in and 83 MB out; two workgroups a CU is what LDS has room for, and each waits
-// for the inverse's chain most of the time).
+// One workgroup per stream, key head and chunk, for all the key head's value heads.
+// 64 chunks of 16 key heads and 32 value heads, 128 wide, bf16: 40 us for 34 MB in
+// and 83 MB out, that is 2.1 TB/s of stores, where a large copy's are 2.5 (workgroups
+// that stay and fetch their next chunk beside the work on one took as long).
 template <class T, int NKT, bool FAST>
 __global__ __launch_bounds__(256, (sizeof(KQ<T, NKT, C>) > 48 * 1024 ? 1 : 2)) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
     struct Lds {
