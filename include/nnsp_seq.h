@@ -42,7 +42,8 @@ extern "C" {
  * Gated delta rule.  Per stream and value head h, with the key head
  * h / (value_heads / key_heads), state S [dk][dv]:
  *
- *   k^_t = k_t / sqrt(|k_t|^2 + eps), q^_t the same    (l2norm != 0; else as given)
+ *   k^_t = k_t / sqrt(|k_t|^2 + eps), q^_t the same    (l2norm != 0; else as given;
+ *                                                       a row of zeros stays zeros)
  *   S'   = exp(g_t) S_{t-1}
  *   u_t  = beta_t (v_t - S'^T k^_t)
  *   S_t  = S' + k^_t u_t^T
@@ -77,7 +78,7 @@ extern "C" {
  * time, need one each).
  *
  * Limits: dk, dv 1 .. 256; value_heads a multiple of key_heads;
- * n_frames at most 2^30; n_streams * value_heads * ceil(dv / 16) below 2^31.
+ * n_frames at most 2^30; n_streams * value_heads * ceil(dv / 16) below 2^24.
  */
 #define NNSP_DELTA_STEP_FRAMES 2
 typedef struct {

@@ -129,8 +129,8 @@ static int delta_sizes(const nnsp_delta_args *a, const char *who)
         nnsp_set_error("%s: n_frames must be at most 2^30", who);
         return NNSP_EUNSUPPORTED;
     }
-    if ((double)a->n_streams * a->value_heads * ((a->dv + 15) / 16) >= 2147483648.0) {
-        nnsp_set_error("%s: n_streams * value_heads * ceil(dv / 16) must stay below 2^31", who);
+    if ((double)a->n_streams * a->value_heads * ((a->dv + 15) / 16) >= 16777216.0) { /* 256 threads each, 2^32 in all */
+        nnsp_set_error("%s: n_streams * value_heads * ceil(dv / 16) must stay below 2^24", who);
         return NNSP_EUNSUPPORTED;
     }
     return 0;

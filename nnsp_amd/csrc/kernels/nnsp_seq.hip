@@ -187,8 +187,9 @@ __global__ __launch_bounds__(256) void delta_step_kernel(const nnsp_delta_args a
                 for (int r = 0; r < RK; ++r) k[r] = ok ? k[r] * fk : k[r], q[r] = oq ? q[r] * fq : q[r];
                 sums();
             }
-            rk = 1.0f / sqrtf(kk + ek);
-            rq = 1.0f / sqrtf(qq + eq);
+            // a row of zeros stays one, also with eps 0
+            rk = kk + ek == 0.0f ? 0.0f : 1.0f / sqrtf(kk + ek);
+            rq = qq + eq == 0.0f ? 0.0f : 1.0f / sqrtf(qq + eq);
         }
         float u[4], o[4];
 #pragma unroll
@@ -388,7 +389,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(const nnsp_
     RowSum<TPR> sum{red};
     const int tid = threadIdx.x % TPR, n = a.dim;
     const unsigned rows = (unsigned)a.rows * (unsigned)a.groups;
-    const unsigned row = blockIdx.x * (unsigned)RPB + threadIdx.x / TPR;  // < 2^31 + 2^8
+    const unsigned row = (blockIdx.y * gridDim.x + blockIdx.x) * (unsigned)RPB + threadIdx.x / TPR;  // < 2^31 + 2^28
     Place<MODE> at[NCH];
 #pragma unroll
     for (int i = 0; i < NCH; ++i) at[i] = Place<MODE>(i * TPR + tid, n);
@@ -465,8 +466,10 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(const nnsp_
 template <class T, class R, int TPR, int NCH, int MODE>
 void launch_norm_mode(const nnsp_norm_args& a, hipStream_t st) {
     constexpr int PER = TPR > 256 ? 1 : 256 / TPR;
-    const long long rows = a.rows * a.groups;
-    norm_kernel<T, R, TPR, NCH, MODE><<<dim3((unsigned)((rows + PER - 1) / PER)), dim3(TPR > 256 ? TPR : 256), 0, st>>>(a);
+    // a grid has at most 2^32 - 1 threads along x
+    const long long groups = (a.rows * a.groups + PER - 1) / PER, x = groups < (1 << 21) ? groups : 1 << 21;
+    const dim3 grid((unsigned)x, (unsigned)((groups + x - 1) / x));
+    norm_kernel<T, R, TPR, NCH, MODE><<<grid, dim3(TPR > 256 ? TPR : 256), 0, st>>>(a);
 }
 template <class T, class R, int TPR, int NCH>
 void launch_norm_as(const nnsp_norm_args& a, hipStream_t st) {

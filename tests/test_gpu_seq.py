@@ -81,10 +81,10 @@ def close(got, ref, dtype, T, dk, what):
     assert bool((off <= bound).all()), f"{what}: off {float((off - bound).max()):.3g} beyond the bound, largest {big:.3g}"
 
 
-def run_delta(d, hk, dtype, l2norm=True, lens=None, state=True, out=None, state_out=None, stream=None, strides=None):
+def run_delta(d, hk, dtype, l2norm=True, lens=None, state=True, out=None, state_out=None, stream=None, strides=None, eps=1e-6):
     S, T, hv, dv = d["v"].shape
     dk = d["q"].shape[-1]
-    p = gated_delta()(S, T, hk, hv, dk, dv, dtype=dtype, l2norm=l2norm, strides=strides)
+    p = gated_delta()(S, T, hk, hv, dk, dv, dtype=dtype, l2norm=l2norm, strides=strides, eps=eps)
     out = torch.full((S, T, hv, dv), 7.0, dtype=DT[dtype], device="cuda") if out is None else out
     so = torch.full((S, hv, dk, dv), 7.0, device="cuda") if state_out is None else state_out
     ln = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
@@ -408,6 +408,35 @@ def test_delta_two_calls_at_once():
         assert torch.equal(out[i], ref[i][0]) and torch.equal(so[i], ref[i][1])
 
 
+@pytest.mark.parametrize("T", [1, 7, 40, 130])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_delta_rows_of_zeros_without_eps(dtype, T):
+    """Nothing is divided by the length of a row that has none."""
+    d = make(2, T, 1, 2, 64, 40, dtype, seed=T)
+    d["k"][0, ::3], d["q"][1, ::2] = 0, 0
+    d["k"][1, -1:], d["q"][0, -1:] = 0, 0
+    out, so = run_delta(d, 1, dtype, eps=0.0)
+    # the oracle's 1e-60 changes no other length
+    ro, rs = delta_ref(d["q"], d["k"], d["v"], d["g"], d["beta"], d["state"], None, True, 64 ** -0.5, eps=1e-60)
+    close(out, ro, dtype, T, 64, "out")
+    close(so, rs, "f32", T, 64, "state")
+
+
+@pytest.mark.parametrize("T", [6, 40, 150])
+def test_delta_growth(T):
+    """Decays above 1 now and then, as a learned gate may give: what a state gains over 64 frames stays small."""
+    d = make(2, T, 1, 2, 64, 40, "f32", seed=T)
+    d["g"] = 0.05 * torch.randn(2, T, 2, generator=torch.Generator().manual_seed(T)).cuda()
+    out, so = run_delta(d, 1, "f32")
+    ro, rs = delta_ref(d["q"], d["k"], d["v"], d["g"], d["beta"], d["state"], None, True, 64 ** -0.5)
+    # the largest product of decays over 64 frames is the factor that precision may cost
+    s = torch.cumsum(d["g"].double().cpu(), 1)
+    s = torch.cat([torch.zeros(2, 1, 2, dtype=torch.float64), s], 1)
+    grow = max(float((s[:, i + 1:i + 65] - s[:, i:i + 1]).max()) for i in range(T))
+    close(out, ro, "f32", T * np.exp(2 * grow), 64, "out")
+    close(so, rs, "f32", T * np.exp(2 * grow), 64, "state")
+
+
 def test_delta_same_bits_every_time_and_by_stream():
     """Results do not depend on the run, nor on the other streams of the call."""
     d = make(40, 130, 2, 4, 64, 64, "bf16", seed=6)
@@ -626,6 +655,16 @@ def test_norm_in_a_graph():
         call()
         torch.cuda.synchronize()
         assert torch.equal(got, y) and torch.equal(gr, ro)
+
+
+def test_norm_more_rows_than_a_grid_has_threads_along_x():
+    """2^29 + 33 rows by 8 lanes each."""
+    rows = (1 << 29) + 33
+    x = torch.arange(rows, device="cuda", dtype=torch.int32).remainder_(251).to(torch.bfloat16)
+    y = torch.zeros_like(x)
+    block_norm()(rows, 1, post="none", pre="none", res_scale=2.0).exec_device(ptr(x), ptr(y))
+    torch.cuda.synchronize()
+    assert torch.equal(y, x.mul_(2))
 
 
 # ---- together ----------------------------------------------------------------

@@ -45,7 +45,8 @@ def refused(call, message, code=_lib.NNSP_EINVAL):
     ((1, 1, 0, 1, 8, 8), "multiple of key_heads", -1), ((1, 1, 2, 3, 8, 8), "multiple of key_heads", -1),
     ((1, 1, 1, 0, 8, 8), "multiple of key_heads", -1),
     ((1, 1, 1, 1, 0, 8), "dk, dv", -2), ((1, 1, 1, 1, 257, 8), "dk, dv", -2), ((1, 1, 1, 1, 8, 257), "dk, dv", -2),
-    ((1 << 30, 1, 1, 2, 8, 8), "below 2", -2), ((1, (1 << 30) + 1, 1, 1, 8, 8), "n_frames", -2),
+    ((1 << 30, 1, 1, 2, 8, 8), "below 2", -2),
+    ((1 << 23, 1, 1, 1, 8, 17), "below 2", -2), ((1, (1 << 30) + 1, 1, 1, 8, 8), "n_frames", -2),
 ])
 def test_delta_sizes_refused(sizes, message, code):
     refused(lambda: GatedDelta(*sizes), message, code)
