@@ -171,16 +171,16 @@ static int delta_way(const nnsp_delta_args *a)
     /* Two passes shorten the chain of a call whose few rows leave CUs idle, and
      * move twice the bytes.  What counts is how many workgroups of 16 columns
      * the second pass has for 256 CUs.  Chunks against two passes, dk = dv = 128,
-     * us.  bf16, 256 workgroups: 65 frames 19 against 22, 100 frames 24 against
-     * 22, 1000 frames 157 against 54; 512: 130 frames 29 against 30, 193 frames
-     * 38 against 33, 1000 frames 156 against 66; 1024: 260 frames 50 against 55,
-     * 500 frames 83 against 69; 1536: 2000 frames 365 against 408.  fp32, 512:
-     * 193 frames 44 against 43, 1000 frames 186 against 110; 768: 2000 frames
-     * 362 against 383.  LDS has no room for 64 frames of fp32 wider than 128. */
+     * us.  bf16, 256 workgroups: 64 frames 14 against 20, 130 frames 24.3 against
+     * 24.4, 260 frames 40 against 30; 512: 130 frames 25 against 29, 260 frames 40
+     * against 37; 1024: 260 frames 43 against 55, 500 frames 69 against 69, 1000
+     * frames 133 against 122; 1536: 2000 frames 365 against 408.  fp32, 512: 260
+     * frames 50 against 48, 1000 frames 160 against 110; 768: 2000 frames 362
+     * against 383.  LDS has no room for 64 frames of fp32 wider than 128. */
     const long long groups = (long long)a->n_streams * a->value_heads * ((a->dv + 15) / 16);
     const int fp32 = a->dtype == NNSP_F32;
     if (fp32 && a->dk > 128) return DELTA_CHUNK;
-    const int from = groups <= 256 ? 100 : groups <= 512 ? 193 : groups <= 1024 && !fp32 ? 400 : INT32_MAX;
+    const int from = groups <= 256 ? 128 : groups <= 512 ? 256 : groups <= 1024 && !fp32 ? 512 : INT32_MAX;
     return a->n_frames >= from ? DELTA_SPLIT : DELTA_CHUNK;
 }
 

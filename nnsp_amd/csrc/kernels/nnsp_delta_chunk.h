@@ -578,8 +578,10 @@ struct Chunk {
     h8 shi[NKT][NB];
     float smax, rmax, sout;
 
+    // mid() is called once on the way, and so in second()
+    template <class F>
     __device__ __forceinline__ void first(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], const f32x4 (&S)[2 * NKT][NB],
-                                          float sinv, int lane, int nt) {
+                                          float sinv, int lane, int nt, const F& mid) {
         const int l15 = lane & 15, g = lane >> 4;
         const f32x4 zero = {0, 0, 0, 0};
         h8 lo[NKT][NB];
@@ -599,6 +601,7 @@ struct Chunk {
             for (int t = 0; t < NKT; ++t) split<true>(S[2 * t][n], S[2 * t + 1][n], all4(sc), all4(sc), shi[t][n], lo[t][n]);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
+            if (m == 1) mid();
             if (m >= nt) {
 #pragma unroll
                 for (int n = 0; n < NB; ++n) R[m][n] = zero;
@@ -638,8 +641,9 @@ struct Chunk {
     }
 
     // U, the output (into V) and the state after the chunk
+    template <class F>
     __device__ __forceinline__ void second(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], f32x4 (&S)[2 * NKT][NB],
-                                           float& sinv, int lane, int nt) {
+                                           float& sinv, int lane, int nt, const F& mid) {
         const int l15 = lane & 15, g = lane >> 4;
         const f32x4 zero = {0, 0, 0, 0};
         f32x4 u[2][NB];  // U = u ti rinv, where |u| is at most 32 products of 2^30
@@ -682,6 +686,7 @@ struct Chunk {
                 for (int r = 0; r < 4; ++r)
                     V[16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], LOW ? O[LOW ? m : 0][n][r] : fq[r] * qs[n][r]);
         }
+        mid();
         // S1, accumulated onto the decayed state in the scale s of U fk; where U is next to nothing, in 2^13 of the
         // decayed state's own, so that neither leaves its range (2^100 at most: the state's factor stays finite)
         const float all = Y.all;
@@ -899,6 +904,34 @@ __device__ __forceinline__ int frames_of(const nnsp_delta_args& a, int s) {
     return a.lens ? max(0, min(a.lens[s], a.n_frames)) : a.n_frames;
 }
 
+// What a chunk of 32 needs no state for, before its inverse, by NW waves: the tiles
+// of A ((0,0), (1,0), (1,1)) and of P, and the factors, which the tiles take in
+// put(), with all waves together in between.
+template <class T, int NKT, int NW>
+struct Tiles {
+    f32x4 ta, tp;
+    // the wave's tile of A and of P; 3 and above: none
+    static __device__ __forceinline__ int at(int role) { return role; }
+    static __device__ __forceinline__ int pt(int role) {
+        return NW == 4 ? (role == 3 ? 1 : role == 1 ? 3 : role) : role >= 3 ? role - 3 : 3;
+    }
+    __device__ __forceinline__ void dots(const KQ<T, NKT, CF>& X, TP<T, CF>& Y, Make<CF>& M, int role, int lane) {
+        constexpr int KP = KQ<T, NKT, CF>::KP;
+        const int l15 = lane & 15, g = lane >> 4, i = at(role), p = pt(role);
+        if (i < 3) ta = dot_tile<NKT, KP>(X.K, X.K, i > 0, i > 1, l15, g);
+        if (p < 3) tp = dot_tile<NKT, KP>(X.K, X.Q, p > 1, p > 0, l15, g);
+        if (role == 1) make_factors<NKT>(X, Y, M, 0, lane);
+        if (role == NW - 1) make_factors<NKT>(X, Y, M, 1, lane);
+        if (role == (NW == 4 ? 1 : 6)) make_factors<NKT>(X, Y, M, 2, lane);
+    }
+    __device__ __forceinline__ void put(TP<T, CF>& Y, const Make<CF>& M, TriA<CF>& A, int role, int lane) const {
+        const int l15 = lane & 15, g = lane >> 4, i = at(role), p = pt(role);
+        if (i < 3) put_a(M, A, ta, i > 0, i > 1, l15, g);
+        if (p < 3) put_p(Y, M, tp, p > 0, p > 1, l15, g);
+        if (p == 0) put_p(Y, M, tp, 0, 1, l15, g);
+    }
+};
+
 // waves per SIMD that the state and the operands leave registers and LDS for
 template <class T, int NKT, int NB, int NW>
 constexpr int fused_waves() {
@@ -955,37 +988,115 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
     }
     wait_loads();
     for (int t0 = 0; t0 < n; t0 += CF) {
-        const int left = n - t0, nt = left > 16 ? 2 : 1, ln = here(lane), l15 = ln & 15, g = ln >> 4;
+        const int left = n - t0, nt = left > 16 ? 2 : 1, ln = here(lane);
         rows.stage(a, L.X, L.Y, L.M);
         cols.stage(L.V[wave]);
         __syncthreads();
-        // the tiles of A ((0,0), (1,0), (1,1)) and of P, and the factors, which the tiles take afterwards
-        constexpr int KP = KQ<T, NKT, CF>::KP;
-        const int at = role, pt = NW == 4 ? (role == 3 ? 1 : role == 1 ? 3 : role) : role - 3;
-        f32x4 ta, tp;
-        if (at < 3) ta = dot_tile<NKT, KP>(L.X.K, L.X.K, at > 0, at > 1, l15, g);
-        if (pt >= 0 && pt < 3) tp = dot_tile<NKT, KP>(L.X.K, L.X.Q, pt > 1, pt > 0, l15, g);
-        if (role == 1) make_factors<NKT>(L.X, L.Y, L.M, 0, ln);
-        if (role == NW - 1) make_factors<NKT>(L.X, L.Y, L.M, 1, ln);
-        if (role == (NW == 4 ? 1 : 6)) make_factors<NKT>(L.X, L.Y, L.M, 2, ln);
+        Tiles<T, NKT, NW> tiles;
+        tiles.dots(L.X, L.Y, L.M, role, ln);
         __syncthreads();
-        if (at < 3) put_a(L.M, L.A, ta, at > 0, at > 1, l15, g);
-        if (pt >= 0 && pt < 3) put_p(L.Y, L.M, tp, pt > 0, pt > 1, l15, g);
-        if (pt == 0) put_p(L.Y, L.M, tp, 0, 1, l15, g);
+        tiles.put(L.Y, L.M, L.A, role, ln);
         __syncthreads();
         if (role == 0) make_t(L.Y, L.A, ln);
         Chunk<T, NKT, NB> c;
-        c.first(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
+        c.first(L.X, L.Y, L.V[wave], S, sinv, ln, nt, [] {});
         if (left > CF) {
             rows.next();
             rows.fetch(a.dk, left - CF);
             cols.fetch(left - CF);
         }
         __syncthreads();
-        c.second(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
+        c.second(L.X, L.Y, L.V[wave], S, sinv, ln, nt, [] {});
         wait_loads();
         cols.store(L.V[wave], left);
         __syncthreads();
+    }
+    if (a.state_out) {
+        float* sq = a.state_out + so;
+        each_state<NKT, NB, FAST>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
+            if (in) (sq + base)[at] = S[t][j][r] * sinv;
+        });
+    }
+}
+
+// Few rows, some chunks: the same with the two halves of a chunk's work beside each
+// other.  Waves 4 .. 7 make chunk c + 1 ready (its rows, tiles, inverse) while
+// waves 0 .. 3, 16 columns each, take chunk c through the state.  The latter need
+// no barrier of their own and meet the former's four on the way.  A chunk takes
+// 3.9 to 4.5 us, bound by the chain that makes it ready (one after the other: 5.2).
+template <class T, int NKT>
+struct PairLds {
+    KQ<T, NKT, CF> X[2];
+    TP<T, CF> Y[2];
+    Make<CF> M;
+    TriA<CF> A;
+    alignas(16) T V[4][CF][Geo<T, NKT, 1>::VS];
+};
+template <class T, int NKT, bool FAST>
+__global__ __launch_bounds__(512) void delta_pair_kernel(const nnsp_delta_args a) {
+    constexpr int NB = 1;
+    __shared__ PairLds<T, NKT> L;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int ncb = (a.dv + 64 * NB - 1) / (64 * NB);
+    const int cb = blockIdx.x % ncb, h = (blockIdx.x / ncb) % a.value_heads, s = blockIdx.x / ncb / a.value_heads;
+    const int n = frames_of(a, s);
+    if (wave >= 4) {
+        const int role = wave - 4;
+        Rows<T, NKT, CF, 8, FAST> rows(a, s, h, 0, threadIdx.x & 255, role);
+        if (n > 0) rows.fetch(a.dk, n);
+        for (int t0 = 0, i = 0; t0 < n; t0 += CF, i ^= 1) {
+            const int left = n - t0, ln = here(lane);
+            rows.stage(a, L.X[i], L.Y[i], L.M);
+            if (left > CF) {
+                rows.next();
+                rows.fetch(a.dk, left - CF);
+            }
+            __syncthreads();
+            Tiles<T, NKT, 4> tiles;
+            tiles.dots(L.X[i], L.Y[i], L.M, role, ln);
+            __syncthreads();
+            tiles.put(L.Y[i], L.M, L.A, role, ln);
+            __syncthreads();
+            if (role == 0) make_t(L.Y[i], L.A, ln);
+            __syncthreads();  // this chunk is ready, and the one before done with
+        }
+        return;
+    }
+    const int c0 = (cb * 4 + wave) * 16 * NB;
+    const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
+    f32x4 S[2 * NKT][NB];
+    float sinv = 1.0f;
+#pragma unroll
+    for (int t = 0; t < 2 * NKT; ++t)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) S[t][j] = f32x4{0, 0, 0, 0};
+    Cols<T, NKT, NB, FAST, CF, CF> cols(a, s, h, 0, c0, lane);
+    if (a.state_in) {
+        const float* sp = a.state_in + so;
+        each_state<NKT, NB, FAST>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
+            const float x = (sp + base)[at];
+            S[t][j][r] = in ? x : 0.0f;
+        });
+    }
+    if (n > 0) {
+        cols.fetch(n);
+        for (int i = 0; i < 4; ++i) __syncthreads();
+    }
+    wait_loads();
+    for (int t0 = 0, i = 0; t0 < n; t0 += CF, i ^= 1) {
+        const int left = n - t0, nt = left > 16 ? 2 : 1, ln = here(lane);
+        const auto meet = [&] {
+            if (left > CF) __syncthreads();
+        };
+        cols.stage(L.V[wave]);
+        Chunk<T, NKT, NB> c;
+        c.first(L.X[i], L.Y[i], L.V[wave], S, sinv, ln, nt, meet);
+        if (left > CF) cols.fetch(left - CF);
+        meet();
+        c.second(L.X[i], L.Y[i], L.V[wave], S, sinv, ln, nt, meet);
+        wait_loads();
+        cols.store(L.V[wave], left);
+        meet();
     }
     if (a.state_out) {
         float* sq = a.state_out + so;
@@ -1366,6 +1477,12 @@ void launch_fused(const nnsp_delta_args& a, hipStream_t st) {
     delta_chunk_kernel<T, NKT, NB, NW, FAST><<<dim3((unsigned)grid), dim3(64 * NW), 0, st>>>(a);
 }
 
+template <class T, int NKT, bool FAST>
+void launch_pair(const nnsp_delta_args& a, hipStream_t st) {
+    const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64);
+    delta_pair_kernel<T, NKT, FAST><<<dim3((unsigned)grid), dim3(512), 0, st>>>(a);
+}
+
 template <class T, int NKT>
 DeltaSplit plan_split(const nnsp_delta_args& a) {
     DeltaSplit p;
@@ -1446,14 +1563,26 @@ int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
                 return 0;
             }
         }
-        // Columns of a workgroup: 64 where there are no more or where CUs are left over, else 128.  500 frames of 16 heads
-        // of 128 x 128, bf16, us: 128 rows by 64 columns 82, by 128 97; 192 rows 108, 99; 512 rows 190, 141; fp32: 128
-        // rows 96, 111; 192 rows 130, 114.  Keys over 128 leave registers for 64 in 16 bits (512 rows of 256 x 256, 200
-        // frames: 258 us, 128 by 8 waves 276).
-        const bool narrow = a.dv <= 64 || (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64) <= 256;
-        if constexpr (WIDE) narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 1, 8, FAST>(a, st);
+        // Workgroups of 64 columns, the halves of a chunk's work beside each other (pair), or one after the other (fused;
+        // of 128 columns where there are so many).  260 frames, dk = dv, us, pair against fused: bf16, 64 columns a
+        // workgroup, 256 workgroups 36 against 42, 512 48 against 53, 1024 88 against 90, 4096 326 against 319; of 128
+        // columns, 64 rows (128 workgroups by 64) 40 against 51 (by 64 columns) and 48 (by 128), 128 rows 43 against 52
+        // and 50, 256 rows 60 against 62, 512 rows 113 against 88.  fp32, 64 columns, 64 workgroups 38 against 44, 4096 417
+        // against 453; 128 columns, 128 rows 51 against 58, 256 rows 98 against 69.
+        const long long groups = (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64);
+        const bool one = a.dv <= 64;
+        if constexpr (sizeof(PairLds<T, NKT>) <= 160 * 1024) {
+            if (groups <= (one ? 512 : 256) || (WIDE && one)) {
+                launch_pair<T, NKT, FAST>(a, st);
+                return 0;
+            }
+        }
+        // Keys over 128 leave registers for 64 columns in 16 bits (512 rows of 256 x 256, 200 frames: 258 us, 128 columns
+        // by 8 waves 276)
+        if constexpr (WIDE && NKT > 4) one || groups <= 256 ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 1, 8, FAST>(a, st);
+        else if constexpr (WIDE) launch_fused<T, NKT, 1, 8, FAST>(a, st);
         else if constexpr (NKT > 4) launch_fused<T, NKT, 1, 4, FAST>(a, st);
-        else narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 2, 4, FAST>(a, st);
+        else one ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 2, 4, FAST>(a, st);
         return 0;
     });
     return (int)hipGetLastError();
