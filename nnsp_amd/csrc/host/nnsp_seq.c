@@ -170,18 +170,17 @@ static int delta_way(const nnsp_delta_args *a)
     if (a->n_frames <= (a->dk <= 32 ? 8 : a->dk <= 96 ? 4 : NNSP_DELTA_STEP_FRAMES)) return DELTA_STEP;
     /* Two passes shorten the chain of a call whose few rows leave CUs idle, and
      * move twice the bytes.  What counts is how many workgroups of 16 columns
-     * the second pass has for 256 CUs.  Chunks against two passes, dk = dv = 128,
-     * us.  bf16, 256 workgroups: 64 frames 14 against 20, 130 frames 24.3 against
-     * 24.4, 260 frames 40 against 30; 512: 130 frames 25 against 29, 260 frames 40
-     * against 37; 1024: 260 frames 43 against 55, 500 frames 69 against 69, 1000
-     * frames 133 against 122; 1536: 2000 frames 365 against 408.  fp32, 512: 260
-     * frames 50 against 48, 1000 frames 160 against 110; 768: 2000 frames 362
-     * against 383.  LDS has no room for 64 frames of fp32 wider than 128. */
+     * the second pass has for 256 CUs.  Chunks against two passes, us.  bf16, dk =
+     * dv = 64: 256 workgroups, 260 frames 28 against 28, 500 frames 45 against 36;
+     * 512: 260 frames 29 against 35, 500 frames 46 against 42; 768: 1000 frames 84
+     * against 107.  128: 256, 130 frames 21 against 24, 260 frames 33 against 29;
+     * 512: 260 frames 34 against 37, 500 frames 55 against 46, 1000 frames 103
+     * against 67; 1024: 1000 frames 109 against 126.  fp32, 128: 256, 260 frames
+     * 40 against 41, 500 frames 65 against 56; 512: 500 frames 70 against 60.
+     * LDS has no room for 64 frames of fp32 wider than 128. */
     const long long groups = (long long)a->n_streams * a->value_heads * ((a->dv + 15) / 16);
-    const int fp32 = a->dtype == NNSP_F32;
-    if (fp32 && a->dk > 128) return DELTA_CHUNK;
-    const int from = groups <= 256 ? 128 : groups <= 512 ? 256 : groups <= 1024 && !fp32 ? 512 : INT32_MAX;
-    return a->n_frames >= from ? DELTA_SPLIT : DELTA_CHUNK;
+    if (a->dtype == NNSP_F32 && a->dk > 128) return DELTA_CHUNK;
+    return groups <= 512 && a->n_frames >= (groups <= 256 ? 256 : 400) ? DELTA_SPLIT : DELTA_CHUNK;
 }
 
 int nnsp_delta_workspace(const nnsp_delta_args *a, size_t *bytes)

@@ -528,11 +528,12 @@ __device__ __forceinline__ void make_tp(const KQ<T, NKT, 64>& X, TP<T, 64>& Y, M
 }
 
 // T of a chunk of 32 by one wave: both diagonal inverses, then N_10 = -T_00^T A_10^T T_11^T
-template <class T>
-__device__ __forceinline__ void make_t(TP<T, 32>& Y, const TriA<32>& A, int lane) {
+template <class T, class F>
+__device__ __forceinline__ void make_t(TP<T, 32>& Y, const TriA<32>& A, int lane, const F& mid) {
     const int l15 = lane & 15, g = lane >> 4;
     Diag<32>& D = *reinterpret_cast<Diag<32>*>(Y.T_);
     invert_diagonal(A, D, g, l15);
+    mid();
     asm volatile("" ::: "memory");  // LDS keeps its order within a wave, the compiler has to
     f32x4 t0, t1, y = {0, 0, 0, 0}, t = {0, 0, 0, 0};
 #pragma unroll
@@ -578,10 +579,8 @@ struct Chunk {
     h8 shi[NKT][NB];
     float smax, rmax, sout;
 
-    // mid() is called once on the way, and so in second()
-    template <class F>
     __device__ __forceinline__ void first(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], const f32x4 (&S)[2 * NKT][NB],
-                                          float sinv, int lane, int nt, const F& mid) {
+                                          float sinv, int lane, int nt) {
         const int l15 = lane & 15, g = lane >> 4;
         const f32x4 zero = {0, 0, 0, 0};
         h8 lo[NKT][NB];
@@ -601,7 +600,6 @@ struct Chunk {
             for (int t = 0; t < NKT; ++t) split<true>(S[2 * t][n], S[2 * t + 1][n], all4(sc), all4(sc), shi[t][n], lo[t][n]);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-            if (m == 1) mid();
             if (m >= nt) {
 #pragma unroll
                 for (int n = 0; n < NB; ++n) R[m][n] = zero;
@@ -640,7 +638,7 @@ struct Chunk {
         }
     }
 
-    // U, the output (into V) and the state after the chunk
+    // U, the output (into V) and the state after the chunk; mid() is called once on the way
     template <class F>
     __device__ __forceinline__ void second(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], f32x4 (&S)[2 * NKT][NB],
                                            float& sinv, int lane, int nt, const F& mid) {
@@ -946,8 +944,7 @@ constexpr int fused_waves() {
 // alone would take 280; the vector units issue 68 % of the time (splits, factors,
 // addresses: some 680 instructions a wave and chunk, 38 of them matrix ones), at
 // three waves a SIMD.  512 streams of 4 heads of 128 x 128, bf16: 159 us, bytes
-// 98.  Where rows are few a chunk takes 4 to 6 us, most of it the chain staging
-// -> products -> inverse -> products.
+// 98.
 template <class T, int NKT, int NB, int NW, bool FAST>
 __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delta_chunk_kernel(const nnsp_delta_args a) {
     using G = Geo<T, NKT, NB>;
@@ -997,9 +994,9 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
         __syncthreads();
         tiles.put(L.Y, L.M, L.A, role, ln);
         __syncthreads();
-        if (role == 0) make_t(L.Y, L.A, ln);
+        if (role == 0) make_t(L.Y, L.A, ln, [] {});
         Chunk<T, NKT, NB> c;
-        c.first(L.X, L.Y, L.V[wave], S, sinv, ln, nt, [] {});
+        c.first(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
         if (left > CF) {
             rows.next();
             rows.fetch(a.dk, left - CF);
@@ -1019,78 +1016,87 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
     }
 }
 
-// Few rows, some chunks: the same with the two halves of a chunk's work beside each
-// other.  Waves 4 .. 7 make chunk c + 1 ready (its rows, tiles, inverse) while
-// waves 0 .. 3, 16 columns each, take chunk c through the state.  The latter need
-// no barrier of their own and meet the former's four on the way.  A chunk takes
-// 3.9 to 4.5 us, bound by the chain that makes it ready (one after the other: 5.2).
+// Few rows, some chunks: the same with the parts of a chunk's work beside each
+// other.  While waves 0 .. 3, 16 columns each, take chunk c through the state,
+// wave 8 inverts chunk c + 1 and waves 4 .. 7 stage chunk c + 2 and make its
+// tiles.  All meet three times a period; only 4 .. 7 need that.  A chunk takes
+// the 6000 cycles of 4 .. 7 (the others' parts 4900 and 3200), one after the
+// other 13000.
 template <class T, int NKT>
-struct PairLds {
-    KQ<T, NKT, CF> X[2];
-    TP<T, CF> Y[2];
+struct PipeLds {
+    KQ<T, NKT, CF> X[3];
+    TP<T, CF> Y[3];
     Make<CF> M;
-    TriA<CF> A;
+    TriA<CF> A[2];
     alignas(16) T V[4][CF][Geo<T, NKT, 1>::VS];
 };
 template <class T, int NKT, bool FAST>
-__global__ __launch_bounds__(512) void delta_pair_kernel(const nnsp_delta_args a) {
-    constexpr int NB = 1;
-    __shared__ PairLds<T, NKT> L;
+__global__ __launch_bounds__(576) void delta_pipe_kernel(const nnsp_delta_args a) {
+    __shared__ PipeLds<T, NKT> L;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int ncb = (a.dv + 64 * NB - 1) / (64 * NB);
+    const int ncb = (a.dv + 63) / 64;
     const int cb = blockIdx.x % ncb, h = (blockIdx.x / ncb) % a.value_heads, s = blockIdx.x / ncb / a.value_heads;
-    const int n = frames_of(a, s);
+    const int n = frames_of(a, s), periods = n > 0 ? (n + CF - 1) / CF + 2 : 0;
+    const auto meet = [] { __syncthreads(); };
+    if (wave == 8) {
+        for (int p = 0, i = 2; p < periods; ++p, i = i < 2 ? i + 1 : 0) {
+            if (p >= 1 && p + 1 < periods) make_t(L.Y[i], L.A[(p + 1) & 1], here(lane), meet);
+            else meet();
+            meet();
+            meet();
+        }
+        return;
+    }
     if (wave >= 4) {
         const int role = wave - 4;
         Rows<T, NKT, CF, 8, FAST> rows(a, s, h, 0, threadIdx.x & 255, role);
         if (n > 0) rows.fetch(a.dk, n);
-        for (int t0 = 0, i = 0; t0 < n; t0 += CF, i ^= 1) {
-            const int left = n - t0, ln = here(lane);
+        for (int p = 0, i = 0; p < periods; ++p, i = i < 2 ? i + 1 : 0) {
+            const int left = n - p * CF, ln = here(lane);
+            if (left <= 0) {
+                meet();
+                meet();
+                meet();
+                continue;
+            }
             rows.stage(a, L.X[i], L.Y[i], L.M);
             if (left > CF) {
                 rows.next();
                 rows.fetch(a.dk, left - CF);
             }
-            __syncthreads();
+            meet();
             Tiles<T, NKT, 4> tiles;
             tiles.dots(L.X[i], L.Y[i], L.M, role, ln);
-            __syncthreads();
-            tiles.put(L.Y[i], L.M, L.A, role, ln);
-            __syncthreads();
-            if (role == 0) make_t(L.Y[i], L.A, ln);
-            __syncthreads();  // this chunk is ready, and the one before done with
+            meet();
+            tiles.put(L.Y[i], L.M, L.A[p & 1], role, ln);
+            meet();
         }
         return;
     }
-    const int c0 = (cb * 4 + wave) * 16 * NB;
+    const int c0 = (cb * 4 + wave) * 16;
     const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
-    f32x4 S[2 * NKT][NB];
+    f32x4 S[2 * NKT][1];
     float sinv = 1.0f;
 #pragma unroll
-    for (int t = 0; t < 2 * NKT; ++t)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) S[t][j] = f32x4{0, 0, 0, 0};
-    Cols<T, NKT, NB, FAST, CF, CF> cols(a, s, h, 0, c0, lane);
+    for (int t = 0; t < 2 * NKT; ++t) S[t][0] = f32x4{0, 0, 0, 0};
+    Cols<T, NKT, 1, FAST, CF, CF> cols(a, s, h, 0, c0, lane);
     if (a.state_in) {
         const float* sp = a.state_in + so;
-        each_state<NKT, NB, FAST>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
+        each_state<NKT, 1, FAST>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
             const float x = (sp + base)[at];
             S[t][j][r] = in ? x : 0.0f;
         });
     }
     if (n > 0) {
         cols.fetch(n);
-        for (int i = 0; i < 4; ++i) __syncthreads();
+        for (int i = 0; i < 6; ++i) meet();  // two periods
     }
     wait_loads();
-    for (int t0 = 0, i = 0; t0 < n; t0 += CF, i ^= 1) {
-        const int left = n - t0, nt = left > 16 ? 2 : 1, ln = here(lane);
-        const auto meet = [&] {
-            if (left > CF) __syncthreads();
-        };
+    for (int p = 2, i = 0; p < periods; ++p, i = i < 2 ? i + 1 : 0) {
+        const int left = n - (p - 2) * CF, nt = left > 16 ? 2 : 1, ln = here(lane);
         cols.stage(L.V[wave]);
-        Chunk<T, NKT, NB> c;
-        c.first(L.X[i], L.Y[i], L.V[wave], S, sinv, ln, nt, meet);
+        Chunk<T, NKT, 1> c;
+        c.first(L.X[i], L.Y[i], L.V[wave], S, sinv, ln, nt);
         if (left > CF) cols.fetch(left - CF);
         meet();
         c.second(L.X[i], L.Y[i], L.V[wave], S, sinv, ln, nt, meet);
@@ -1100,7 +1106,7 @@ __global__ __launch_bounds__(512) void delta_pair_kernel(const nnsp_delta_args a
     }
     if (a.state_out) {
         float* sq = a.state_out + so;
-        each_state<NKT, NB, FAST>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
+        each_state<NKT, 1, FAST>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
             if (in) (sq + base)[at] = S[t][j][r] * sinv;
         });
     }
@@ -1478,9 +1484,9 @@ void launch_fused(const nnsp_delta_args& a, hipStream_t st) {
 }
 
 template <class T, int NKT, bool FAST>
-void launch_pair(const nnsp_delta_args& a, hipStream_t st) {
+void launch_pipe(const nnsp_delta_args& a, hipStream_t st) {
     const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64);
-    delta_pair_kernel<T, NKT, FAST><<<dim3((unsigned)grid), dim3(512), 0, st>>>(a);
+    delta_pipe_kernel<T, NKT, FAST><<<dim3((unsigned)grid), dim3(576), 0, st>>>(a);
 }
 
 template <class T, int NKT>
@@ -1563,26 +1569,25 @@ int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
                 return 0;
             }
         }
-        // Workgroups of 64 columns, the halves of a chunk's work beside each other (pair), or one after the other (fused;
-        // of 128 columns where there are so many).  260 frames, dk = dv, us, pair against fused: bf16, 64 columns a
-        // workgroup, 256 workgroups 36 against 42, 512 48 against 53, 1024 88 against 90, 4096 326 against 319; of 128
-        // columns, 64 rows (128 workgroups by 64) 40 against 51 (by 64 columns) and 48 (by 128), 128 rows 43 against 52
-        // and 50, 256 rows 60 against 62, 512 rows 113 against 88.  fp32, 64 columns, 64 workgroups 38 against 44, 4096 417
-        // against 453; 128 columns, 128 rows 51 against 58, 256 rows 98 against 69.
+        // Workgroups of 64 columns that work on three chunks at once (pipe, keys up to 128 wide) while each has a CU to
+        // itself, else such as share a CU, of 128 columns where there are so many (fused).  260 frames, dk = dv, us, pipe
+        // against fused, bf16: 64, 32 rows 28 and 41, 256 rows 30 and 42, 384 rows 53 and 51; 128, 32 rows 33 and 47 (by 64
+        // columns), 128 rows 37 and 50, 192 rows 66 and 59; fp32: 64, 256 rows 35 and 46, 384 rows 62 and 57; 128, 128
+        // rows 45 and 58, 192 rows 80 and 66.  20 frames, 64: 9 and 9; 128, 128 rows 11 and 12.
         const long long groups = (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64);
-        const bool one = a.dv <= 64;
-        if constexpr (sizeof(PairLds<T, NKT>) <= 160 * 1024) {
-            if (groups <= (one ? 512 : 256) || (WIDE && one)) {
-                launch_pair<T, NKT, FAST>(a, st);
+        if constexpr (NKT <= 4) {
+            if (groups <= 256) {
+                launch_pipe<T, NKT, FAST>(a, st);
                 return 0;
             }
         }
         // Keys over 128 leave registers for 64 columns in 16 bits (512 rows of 256 x 256, 200 frames: 258 us, 128 columns
-        // by 8 waves 276)
-        if constexpr (WIDE && NKT > 4) one || groups <= 256 ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 1, 8, FAST>(a, st);
-        else if constexpr (WIDE) launch_fused<T, NKT, 1, 8, FAST>(a, st);
+        // by 8 waves 276), and fp32 is faster by 64 while CUs are left over (64 streams of 8 frames, 8
+        // heads of 256 x 256: 114 us by 64, by 128 85; one stream, 2000 frames 521 and 624)
+        const bool narrow = a.dv <= 64 || (NKT > 4 && groups <= 256);
+        if constexpr (WIDE) narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 1, 8, FAST>(a, st);
         else if constexpr (NKT > 4) launch_fused<T, NKT, 1, 4, FAST>(a, st);
-        else one ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 2, 4, FAST>(a, st);
+        else narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 2, 4, FAST>(a, st);
         return 0;
     });
     return (int)hipGetLastError();

@@ -113,7 +113,7 @@ def test_delta(S, T, hk, hv, dk, dv, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-@pytest.mark.parametrize("T", [3, 64, 150])
+@pytest.mark.parametrize("T", [3, 64, 150, 300])
 def test_delta_given_keys_no_decay_no_state(T, dtype):
     d = make(2, T, 1, 2, 64, 48, dtype, seed=T, l2norm=False)
     d["g"] = None
@@ -123,7 +123,7 @@ def test_delta_given_keys_no_decay_no_state(T, dtype):
     close(so, rs, "f32", T, 64, "state")
 
 
-@pytest.mark.parametrize("T", [5, 150])
+@pytest.mark.parametrize("T", [5, 150, 300])
 def test_delta_equal_keys_and_full_beta(T):
     """The hardest triangular system: every key the same, beta 1, no decay."""
     d = make(1, T, 1, 1, 64, 64, "f32", seed=9)
@@ -136,7 +136,7 @@ def test_delta_equal_keys_and_full_beta(T):
     close(so, rs, "f32", T, 64, "state")
 
 
-@pytest.mark.parametrize("T", [4, 140])
+@pytest.mark.parametrize("T", [4, 140, 300])
 def test_delta_decays_from_nothing_to_everything(T):
     """g of 0, tiny, large and -inf: frames after a cleared state see nothing of it."""
     d = make(2, T, 1, 3, 64, 64, "bf16", seed=3)
@@ -150,7 +150,7 @@ def test_delta_decays_from_nothing_to_everything(T):
 
 
 @pytest.mark.parametrize("exponent", [-40, 40])
-@pytest.mark.parametrize("T", [2, 80])
+@pytest.mark.parametrize("T", [2, 80, 280])
 def test_delta_scales(T, exponent):
     """Values far from 1 (bf16 has the range): nothing is lost to a narrower one on the way."""
     d = make(1, T, 1, 1, 64, 64, "bf16", seed=5)
@@ -163,7 +163,7 @@ def test_delta_scales(T, exponent):
     close(so, rs, "f32", T, 64, "state")
 
 
-@pytest.mark.parametrize("T,lens", [(6, [0, 6, 1, 5]), (100, [0, 100, 64, 65]), (200, [129, 1, 200, 63]), (70, [-3, 1000, 8, 16])])
+@pytest.mark.parametrize("T,lens", [(6, [0, 6, 1, 5]), (100, [0, 100, 64, 65]), (200, [129, 1, 200, 63]), (70, [-3, 1000, 8, 16]), (500, [257, 1, 500, 0])])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_delta_ragged(T, lens, dtype):
     """Padding holds NaN and infinity; rows behind a stream's length keep what they held; length 0 keeps the state."""
@@ -182,7 +182,7 @@ def test_delta_ragged(T, lens, dtype):
             assert torch.equal(so[s], d["state"][s])
 
 
-@pytest.mark.parametrize("T", [1, 3, 66])
+@pytest.mark.parametrize("T", [1, 3, 66, 300])
 def test_delta_strides_and_offsets(T):
     """q, k, v as slices of one projection that starts at odd addresses, heads before frames in out, repeated beta."""
     S, hk, hv, dk, dv = 3, 1, 2, 24, 20
@@ -208,7 +208,7 @@ def test_delta_strides_and_offsets(T):
     close(so, rs, "f32", T, dk, "state")
 
 
-@pytest.mark.parametrize("T", [1, 90])
+@pytest.mark.parametrize("T", [1, 90, 600])
 def test_delta_state_in_place(T):
     d = make(3, T, 2, 2, 64, 64, "bf16", seed=4)
     ref_out, ref_state = run_delta(d, 2, "bf16")
@@ -319,7 +319,7 @@ def test_delta_slabs_ragged(state):
         close(so[s:s + 1], rs, "f32", T, d_, f"state {s}")
 
 
-@pytest.mark.parametrize("T", [5, 60, 140])
+@pytest.mark.parametrize("T", [5, 60, 140, 300])
 def test_delta_keys_of_zeros_and_of_all_lengths(T):
     """Silence (keys and queries of zeros, also with eps 0) and frames far quieter than their neighbours."""
     for dtype in ("bf16", "f16", "f32"):
@@ -336,7 +336,7 @@ def test_delta_keys_of_zeros_and_of_all_lengths(T):
 
 @pytest.mark.parametrize("l2norm,qe,ke", [(True, -80, 0), (True, 0, -80), (True, 75, 75), (False, -75, 0), (False, 75, -75),
                                           (False, -75, 75)])
-@pytest.mark.parametrize("T", [5, 40, 100])
+@pytest.mark.parametrize("T", [5, 40, 300])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_delta_rows_whose_squares_leave_32_bits(dtype, T, l2norm, qe, ke):
     """Queries and keys so faint or loud that their squares are 0 or infinite in 32 bits."""
@@ -350,7 +350,7 @@ def test_delta_rows_whose_squares_leave_32_bits(dtype, T, l2norm, qe, ke):
     close(so, rs, "f32", T, 64, "state")
 
 
-@pytest.mark.parametrize("T", [5, 40, 150])
+@pytest.mark.parametrize("T", [5, 40, 150, 300])
 @pytest.mark.parametrize("what", ["v", "state"])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_delta_infinity_is_seen(dtype, what, T):
@@ -376,9 +376,9 @@ def test_delta_infinity_is_seen(dtype, what, T):
     close(torch.where(torch.isfinite(st), st, rs[1, 1]), rs[1, 1], "f32", T, 64, "finite states")
 
 
-@pytest.mark.parametrize("S,T,h,d_", [(2, 5, 2, 64), (2, 130, 2, 64), (8, 330, 32, 128), (300, 70, 1, 32)])
+@pytest.mark.parametrize("S,T,h,d_", [(2, 5, 2, 64), (2, 130, 2, 64), (2, 500, 2, 64), (2, 1800, 32, 128), (300, 70, 1, 32)])
 def test_delta_final_state_dropped(S, T, h, d_):
-    """Frame by frame, in two passes (of one slab and of two) and in chunks, without state_out."""
+    """Frame by frame, in chunks (few rows and many) and in two passes (of one slab and of several), without state_out."""
     d = make(S, T, h, h, d_, d_, "bf16", seed=S)
     ref, _ = run_delta(d, h, "bf16")
     p = gated_delta()(S, T, h, h, d_, d_)
@@ -408,7 +408,7 @@ def test_delta_two_calls_at_once():
         assert torch.equal(out[i], ref[i][0]) and torch.equal(so[i], ref[i][1])
 
 
-@pytest.mark.parametrize("T", [1, 7, 40, 130])
+@pytest.mark.parametrize("T", [1, 7, 40, 300])
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 def test_delta_rows_of_zeros_without_eps(dtype, T):
     """Nothing is divided by the length of a row that has none."""
@@ -422,7 +422,7 @@ def test_delta_rows_of_zeros_without_eps(dtype, T):
     close(so, rs, "f32", T, 64, "state")
 
 
-@pytest.mark.parametrize("T", [6, 40, 150])
+@pytest.mark.parametrize("T", [6, 40, 150, 300])
 def test_delta_growth(T):
     """Decays above 1 now and then, as a learned gate may give: what a state gains over 64 frames stays small."""
     d = make(2, T, 1, 2, 64, 40, "f32", seed=T)
@@ -445,7 +445,7 @@ def test_delta_same_bits_every_time_and_by_stream():
     assert torch.equal(a, b) and torch.equal(sa, sb)
 
 
-@pytest.mark.parametrize("T", [1, 130])
+@pytest.mark.parametrize("T", [1, 130, 600])
 def test_delta_other_stream(T):
     d = make(2, T, 1, 2, 64, 64, "bf16", seed=7)
     ref, rs = run_delta(d, 1, "bf16")
@@ -454,7 +454,7 @@ def test_delta_other_stream(T):
     assert torch.equal(out, ref) and torch.equal(so, rs)
 
 
-@pytest.mark.parametrize("T", [1, 130])
+@pytest.mark.parametrize("T", [1, 130, 600])
 def test_delta_in_a_graph(T):
     """Captured once, replayed on new inputs, with the same call made eagerly in between."""
     S, hk, hv, dk, dv = 2, 1, 2, 64, 64

@@ -127,7 +127,7 @@ def test_delta_workspace():
     assert GatedDelta(1, 8, 1, 1, 64, 64).workspace_bytes == 0
     assert GatedDelta(8192, 100, 2, 2, 64, 64).workspace_bytes == 0
     assert GatedDelta(0, 1000, 2, 2, 64, 64).workspace_bytes == 0
-    n = [GatedDelta(1, T, 16, 32, 128, 128).workspace_bytes for T in (128, 16384, 1 << 30)]
+    n = [GatedDelta(1, T, 16, 32, 128, 128).workspace_bytes for T in (256, 16384, 1 << 30)]
     assert 0 < n[0] < n[1] <= n[2] < 128 << 20
     refused(delta(sizes=(2, 1000, 1, 2, 64, 64)), "workspace of 0 bytes")
     refused(delta({"workspace": BAD + 8}, sizes=(2, 1000, 1, 2, 64, 64)), "workspace is not aligned")
