@@ -938,14 +938,17 @@ constexpr int fused_waves() {
 
 // Many streams: a workgroup per stream, head and 16 NB NW columns goes through its
 // chunks of 32 alone, and the workgroups of a CU fill each other's waits.
-// FAST: dk and dv are multiples of 8.
+// FAST: dk and dv are multiples of 8.  SPARE: dv leaves the last of them waves
+// without columns, which only help with the tiles and the inverse (512 streams of
+// 100 frames, 4 heads of 72 x 72, bf16: 134 -> 118 us; asking costs registers: 128
+// x 128, which has none, 168 -> 176).
 //
 // 100 frames of 8192 streams, 2 heads of 64 x 64, fp16: 505 us, of which the bytes
 // alone would take 280; the vector units issue 68 % of the time (splits, factors,
 // addresses: some 680 instructions a wave and chunk, 38 of them matrix ones), at
 // three waves a SIMD.  512 streams of 4 heads of 128 x 128, bf16: 159 us, bytes
 // 98.
-template <class T, int NKT, int NB, int NW, bool FAST>
+template <class T, int NKT, int NB, int NW, bool FAST, bool SPARE>
 __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delta_chunk_kernel(const nnsp_delta_args a) {
     using G = Geo<T, NKT, NB>;
     struct Lds {
@@ -962,7 +965,9 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
     const int n = frames_of(a, s);
     const int c0 = (cb * NW + wave) * 16 * NB;  // first column of this wave
     const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
-    const int role = (wave + blockIdx.x) & (NW - 1);  // who does what of the tiles: another SIMD each workgroup
+    const bool live = !SPARE || c0 < a.dv, spare = SPARE && (cb + 1) * 16 * NB * NW - 16 * NB >= a.dv;  // the last wave has none
+    // who does what of the tiles: another SIMD each workgroup, or a wave without columns the longest part
+    const int role = (wave + (spare ? 1 : blockIdx.x)) & (NW - 1);
 
     f32x4 S[2 * NKT][NB];
     float sinv = 1.0f;
@@ -970,7 +975,7 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
     for (int t = 0; t < 2 * NKT; ++t)
 #pragma unroll
         for (int j = 0; j < NB; ++j) S[t][j] = f32x4{0, 0, 0, 0};
-    if (a.state_in) {
+    if (a.state_in && live) {
         const float* sp = a.state_in + so;
         each_state<NKT, NB, FAST>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
             const float x = (sp + base)[at];
@@ -981,13 +986,13 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
     Cols<T, NKT, NB, FAST, CF, CF> cols(a, s, h, 0, c0, lane);
     if (n > 0) {
         rows.fetch(a.dk, n);
-        cols.fetch(n);
+        if (live) cols.fetch(n);
     }
     wait_loads();
     for (int t0 = 0; t0 < n; t0 += CF) {
         const int left = n - t0, nt = left > 16 ? 2 : 1, ln = here(lane);
         rows.stage(a, L.X, L.Y, L.M);
-        cols.stage(L.V[wave]);
+        if (live) cols.stage(L.V[wave]);
         __syncthreads();
         Tiles<T, NKT, NW> tiles;
         tiles.dots(L.X, L.Y, L.M, role, ln);
@@ -996,19 +1001,19 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
         __syncthreads();
         if (role == 0) make_t(L.Y, L.A, ln, [] {});
         Chunk<T, NKT, NB> c;
-        c.first(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
+        if (live) c.first(L.X, L.Y, L.V[wave], S, sinv, ln, nt);
         if (left > CF) {
             rows.next();
             rows.fetch(a.dk, left - CF);
-            cols.fetch(left - CF);
+            if (live) cols.fetch(left - CF);
         }
         __syncthreads();
-        c.second(L.X, L.Y, L.V[wave], S, sinv, ln, nt, [] {});
+        if (live) c.second(L.X, L.Y, L.V[wave], S, sinv, ln, nt, [] {});
         wait_loads();
-        cols.store(L.V[wave], left);
+        if (live) cols.store(L.V[wave], left);
         __syncthreads();
     }
-    if (a.state_out) {
+    if (a.state_out && live) {
         float* sq = a.state_out + so;
         each_state<NKT, NB, FAST>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
             if (in) (sq + base)[at] = S[t][j][r] * sinv;
@@ -1479,8 +1484,16 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
 // ---- launches ----
 template <class T, int NKT, int NB, int NW, bool FAST>
 void launch_fused(const nnsp_delta_args& a, hipStream_t st) {
-    const long long grid = (long long)a.n_streams * a.value_heads * ((a.dv + 16 * NB * NW - 1) / (16 * NB * NW));
-    delta_chunk_kernel<T, NKT, NB, NW, FAST><<<dim3((unsigned)grid), dim3(64 * NW), 0, st>>>(a);
+    constexpr int COLS = 16 * NB * NW;
+    const int blocks = (a.dv + COLS - 1) / COLS;
+    const dim3 grid((unsigned)((long long)a.n_streams * a.value_heads * blocks)), block(64 * NW);
+    if constexpr (NKT <= 4) {  // wider keys leave no registers to ask
+        if (blocks * COLS - 16 * NB >= a.dv) {
+            delta_chunk_kernel<T, NKT, NB, NW, FAST, true><<<grid, block, 0, st>>>(a);
+            return;
+        }
+    }
+    delta_chunk_kernel<T, NKT, NB, NW, FAST, false><<<grid, block, 0, st>>>(a);
 }
 
 template <class T, int NKT, bool FAST>
