@@ -263,10 +263,12 @@ void launch_step(const nnsp_delta_args& a, hipStream_t st) {
 // thread), so each input is read once and each output written once; the call
 // is bound by those bytes, provided that a gate's exponential and reciprocal
 // are the hardware's (with their exact forms the vector units were the bound).
-// Rows up to 1024 elements take 8 .. 64 lanes of a wave and sum by lane permutes;
-// longer ones a whole workgroup and one LDS exchange per sum.  (Several short rows
-// a thread, for more loads in flight, were no faster: 262144 gated rows of 64
-// 17 us, four a thread 20.)
+// Rows up to 1536 elements take 8 .. 64 lanes of a wave and sum by lane permutes;
+// longer ones a whole workgroup and one LDS exchange per sum (32768 rows, two
+// layer norms, bf16, by waves against workgroups: 1383 elements 75 us against 89,
+// 1664 101 against 99, 2048 110 against 101).  Several short rows a thread, for
+// more loads in flight, were no faster: 262144 gated rows of 64 17 us, four a
+// thread 20.
 //
 // 1638400 rows of 64, gated, bf16: 107 us, 5.9 TB/s; 8192 of 4096 with an fp32
 // residual: 79 us, 5.1 TB/s; 16384 of 2048 in fp32, gated: 119 us, 5.6 TB/s; a
@@ -494,6 +496,7 @@ void launch_norm_t(nnsp_norm_args a, hipStream_t st) {
     else if (nc <= 32) launch_norm_as<T, R, 32, 1>(a, st);
     else if (nc <= 64) launch_norm_as<T, R, 64, 1>(a, st);
     else if (nc <= 128) launch_norm_as<T, R, 64, 2>(a, st);
+    else if (nc <= 192) launch_norm_as<T, R, 64, 3>(a, st);
     else if (nc <= 256) launch_norm_as<T, R, 256, 1>(a, st);
     else if (nc <= 512) launch_norm_as<T, R, 256, 2>(a, st);
     else if (nc <= 1024) launch_norm_as<T, R, 512, 2>(a, st);

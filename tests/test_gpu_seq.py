@@ -553,7 +553,7 @@ def norm_inputs(rows, groups, dim, dtype, res, seed):
 
 @pytest.mark.parametrize("dtype,res", [("bf16", None), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f32", "f32")])
 @pytest.mark.parametrize("rows,groups,dim", [(1, 1, 1), (3, 2, 7), (5, 1, 64), (33, 3, 65), (2, 1, 129), (9, 1, 256), (3, 1, 1000),
-                                             (2, 2, 1025), (2, 1, 2048), (3, 1, 4097), (1, 1, 8192), (2, 1, 16384), (1, 1, 16383)])
+                                             (2, 2, 1025), (5, 1, 1383), (7, 1, 1536), (2, 1, 1537), (2, 1, 2048), (3, 1, 4097), (1, 1, 8192), (2, 1, 16384), (1, 1, 16383)])
 @pytest.mark.parametrize("post,act,pre", [("rms", "sigmoid", "rms"), ("layer", "silu", "layer"), ("none", "none", "rms"),
                                           ("rms", "silu", "none")])
 def test_norm(rows, groups, dim, dtype, res, post, act, pre):
