@@ -482,21 +482,34 @@ def test_delta_in_a_graph(T):
         assert torch.equal(got, out) and torch.equal(gs, so)
 
 
-def test_delta_far_offsets():
-    """Frames more than 2^31 elements apart from the first."""
-    T, dk, dv, far = 3, 16, 16, 1 << 31
-    buf = torch.zeros(far + 64, dtype=torch.bfloat16, device="cuda")
+@pytest.mark.parametrize("T", [3, 40, 300])
+def test_delta_far_offsets(T):
+    """Streams more than 2^31 elements apart, one frame at a time, in chunks and in two passes."""
+    dk, dv, far = 16, 16, 1 << 31
     d = make(2, T, 1, 1, dk, dv, "bf16", seed=14)
+    buf = torch.zeros(far + T * dv, dtype=torch.bfloat16, device="cuda")
     v = torch.as_strided(buf, (2, T, 1, dv), (far, dv, dv, 1), 0)
     v.copy_(d["v"])
     out, so = torch.zeros(2, T, 1, dv, dtype=torch.bfloat16, device="cuda"), torch.zeros_like(d["state"])
     p = gated_delta()(2, T, 1, 1, dk, dv, strides={"v": (far, dv, dv)})
+    ws = torch.empty(max(16, p.workspace_bytes), dtype=torch.uint8, device="cuda")
     p.exec_device(ptr(d["q"]), ptr(d["k"]), buf.data_ptr(), ptr(d["g"]), ptr(d["beta"]), ptr(out), state_in=ptr(d["state"]),
-                  state_out=ptr(so))
+                  state_out=ptr(so), workspace=ptr(ws))
     torch.cuda.synchronize()
     ro, rs = delta_ref(d["q"], d["k"], d["v"], d["g"], d["beta"], d["state"], None, True, dk ** -0.5)
     close(out, ro, "bf16", T, dk, "out")
     close(so, rs, "f32", T, dk, "state")
+
+
+@pytest.mark.parametrize("T", [2, 50])
+def test_delta_pinned_host_memory(T):
+    """Inputs and the state in pinned host memory, which the device reads and writes in place."""
+    d = make(2, T, 1, 2, 64, 40, "bf16", seed=T)
+    ref, rs = run_delta(d, 1, "bf16")
+    pinned = {n: torch.empty(x.shape, dtype=x.dtype, pin_memory=True).copy_(x) for n, x in d.items()}
+    so = torch.zeros(rs.shape, pin_memory=True)
+    out, _ = run_delta(pinned, 1, "bf16", state_out=so)
+    assert torch.equal(out, ref) and torch.equal(so, rs.cpu())
 
 
 def test_delta_host_memory_is_refused():
