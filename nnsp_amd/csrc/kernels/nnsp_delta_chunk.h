@@ -1487,7 +1487,7 @@ void launch_fused(const nnsp_delta_args& a, hipStream_t st) {
     constexpr int COLS = 16 * NB * NW;
     const int blocks = (a.dv + COLS - 1) / COLS;
     const dim3 grid((unsigned)((long long)a.n_streams * a.value_heads * blocks)), block(64 * NW);
-    if constexpr (NKT <= 4) {  // wider keys leave no registers to ask
+    if constexpr (NKT <= 6) {  // wider keys leave no registers to ask
         if (blocks * COLS - 16 * NB >= a.dv) {
             delta_chunk_kernel<T, NKT, NB, NW, FAST, true><<<grid, block, 0, st>>>(a);
             return;
@@ -1547,13 +1547,17 @@ void launch_split(const nnsp_delta_args& a, hipStream_t st) {
     }
 }
 
-// f<NKT, FAST>() of this call's sizes
+// f<NKT, FAST>() of this call's sizes: keys go in by 32 columns, padded to one of
+// a few widths (512 streams of 100 frames, 4 heads of 192 x 128, bf16: padded to
+// 192 310 us, to 256 355; one stream of 4000 frames, 8 heads of 160 x 128, in two
+// passes 146 and 226)
 template <class F>
 auto with_sizes(const nnsp_delta_args& a, const F& f) {
     typedef std::integral_constant<int, 1> I1;
     typedef std::integral_constant<int, 2> I2;
     typedef std::integral_constant<int, 3> I3;
     typedef std::integral_constant<int, 4> I4;
+    typedef std::integral_constant<int, 6> I6;
     typedef std::integral_constant<int, 8> I8;
     if ((a.dk | a.dv) & 7)
         return a.dk <= 64 ? f(I2(), std::false_type()) : a.dk <= 128 ? f(I4(), std::false_type()) : f(I8(), std::false_type());
@@ -1561,6 +1565,7 @@ auto with_sizes(const nnsp_delta_args& a, const F& f) {
     if (a.dk <= 64) return f(I2(), std::true_type());
     if (a.dk <= 96) return f(I3(), std::true_type());
     if (a.dk <= 128) return f(I4(), std::true_type());
+    if (a.dk <= 192) return f(I6(), std::true_type());
     return f(I8(), std::true_type());
 }
 
