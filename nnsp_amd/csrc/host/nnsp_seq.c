@@ -177,10 +177,13 @@ static int delta_way(const nnsp_delta_args *a)
      * 512: 260 frames 34 against 37, 500 frames 55 against 46, 1000 frames 103
      * against 67; 1024: 1000 frames 109 against 126.  fp32, 128: 256, 260 frames
      * 40 against 41, 500 frames 65 against 56; 512: 500 frames 70 against 60.
-     * LDS has no room for 64 frames of fp32 wider than 128. */
+     * Wider keys, whose chunks go one after the other, 160 x 128, bf16: 256, 130
+     * frames 32 against 27; 512, 260 frames 56 against 44.  LDS has no room for 64
+     * frames of fp32 wider than 128. */
     const long long groups = (long long)a->n_streams * a->value_heads * ((a->dv + 15) / 16);
     if (a->dtype == NNSP_F32 && a->dk > 128) return DELTA_CHUNK;
-    return groups <= 512 && a->n_frames >= (groups <= 256 ? 256 : 400) ? DELTA_SPLIT : DELTA_CHUNK;
+    const int wide = a->dk > 128, from = groups <= 256 ? (wide ? 128 : 256) : wide ? 256 : 400;
+    return groups <= 512 && a->n_frames >= from ? DELTA_SPLIT : DELTA_CHUNK;
 }
 
 int nnsp_delta_workspace(const nnsp_delta_args *a, size_t *bytes)
