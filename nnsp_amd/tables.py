@@ -1,13 +1,13 @@
 """Constant-table generator for the ns-nnsp hot path.
 
 Every constant table the fixed-point path needs is regenerated here from a
-closed-form rule; nothing is copied from the reference.  Each rule was pinned
-against the reference's own table bytes in the build container (see
-tests/test_tables.py, which re-checks all of them whenever /root/reference is
-present):
+closed-form rule; nothing is copied from the reference.  The rules of the
+tables that the reference has as source are checked word for word against it
+(tests/test_tables.py, whenever /root/reference is present); the last three are
+the library's inside arm_rfft_q31, which the reference has no source of:
 
 =========================  ==========================================  ==========================================
-table                      reference location                          rule (exact, all entries)
+table                      reference location                          rule
 =========================  ==========================================  ==========================================
 stft window (480 x i16)    ns-nnsp/src/window_stft_coef.c:6            floor(sqrt(hop/win*(1-cos(2*pi*n/win)))*2^15)
                            (generator python/nnsp_pack/gen_stft_win.py:14-19)
@@ -15,13 +15,16 @@ mel banks (534 x i16)      ns-nnsp/src/melSpec_coeff.c:5               packed [s
                            (generator python/nnsp_pack/mel.py:10-50)   coef = floor(tri * 2^15)
 log10 interp (256 x i16)   ns-nnsp/src/fixlog10.c:6                    [floor(ln(1+k/128)*2^15), min(floor(2^15/(1+k/128)),32767)]
 tanh interp (384 x i16)    ns-nnsp/src/activation.c:5                  c=(512+1024k)/2^15: [floor(tanh c*2^15), floor((1-tanh^2 c)*2^15)]
-cfft twiddles (384 x q31)  CMSIS-DSP 1.10.0 twiddleCoef_256_q31         floor(x*2^31 + 0.05), x = cos/sin(2*pi*i/256)
+cfft twiddles (384 x q31)  CMSIS-DSP 1.10.0 twiddleCoef_256_q31         round(x*2^31), x = cos/sin(2*pi*i/256), i < 192
 rfft split A/B (q31)       CMSIS-DSP 1.10.0 realCoefAQ31/realCoefBQ31   round(0.5*(1-+sin t)*2^31), round(-+0.5*cos t*2^31)
 bit reversal               CMSIS-DSP armBitRevIndexTable_fixed_256      8-bit bit reversal of the 256 complex slots
 =========================  ==========================================  ==========================================
 
-The CMSIS-DSP tables have no source in the reference: their rules are held by
-the tests of the float DFT alone.
+Those three follow from the mathematics of the transform: cos and sin to the
+nearest q31 value (1 saturates) and the order of a radix-2 bit reversal.
+Whether the shipped library's words are the same is not known: parity unpinned.
+tests/test_tables.py holds them to half a step of the exact values, and
+tests/test_fft_oracle.py the transform to a float DFT.
 
 ``write_header`` emits ``nnsp_amd/csrc/gen/nnsp_tables.h`` used by both the
 HIP kernels / host library and the test oracle.
@@ -130,23 +133,23 @@ def act_affine_table() -> np.ndarray:
     return (out & 0xFFFFFFFF).astype(np.uint32).view(np.int32)
 
 
+def _q31(x: np.ndarray) -> np.ndarray:
+    """The nearest q31 value; 1 saturates."""
+    return np.clip(np.round(x * 2.0 ** 31), -2 ** 31, 2 ** 31 - 1).astype(np.int32)
+
+
 def cfft256_twiddles() -> np.ndarray:
-    i = np.arange(192)
-    v = np.stack([np.cos(2 * np.pi * i / 256), np.sin(2 * np.pi * i / 256)], 1).reshape(-1) * 2.0 ** 31
-    return np.clip(np.floor(v + 0.05), -2 ** 31, 2 ** 31 - 1).astype(np.int32)
+    th = 2 * np.pi * np.arange(192) / 256
+    return _q31(np.stack([np.cos(th), np.sin(th)], 1).reshape(-1))
 
 
 def rfft_split_full(n: int = 4096) -> tuple[np.ndarray, np.ndarray]:
     """Full CMSIS realCoefAQ31 / realCoefBQ31 (n complex entries each)."""
     i = np.arange(n)
     th = 2 * np.pi * i / (2 * n)
-
-    def q31(x):
-        return np.clip(np.round(x * 2.0 ** 31), -2 ** 31, 2 ** 31 - 1).astype(np.int64)
-
-    a = np.stack([q31(0.5 * (1 - np.sin(th))), q31(-0.5 * np.cos(th))], 1).reshape(-1)
-    b = np.stack([q31(0.5 * (1 + np.sin(th))), q31(0.5 * np.cos(th))], 1).reshape(-1)
-    return a.astype(np.int32), b.astype(np.int32)
+    a = np.stack([_q31(0.5 * (1 - np.sin(th))), _q31(-0.5 * np.cos(th))], 1).reshape(-1)
+    b = np.stack([_q31(0.5 * (1 + np.sin(th))), _q31(0.5 * np.cos(th))], 1).reshape(-1)
+    return a, b
 
 
 def rfft512_split_coefs() -> np.ndarray:
@@ -227,8 +230,8 @@ def header_text() -> str:
     mel = mel_bank_packed()
     parts = [
         "/* GENERATED by nnsp_amd/tables.py -- do not edit.\n"
-        " * Closed-form regenerations of the ns-nnsp / CMSIS-DSP constant tables;\n"
-        " * exactness vs the reference is checked by tests/test_tables.py. */\n",
+        " * Closed-form regenerations of the constant tables of ns-nnsp (checked\n"
+        " * against its source tables by tests/test_tables.py) and of its FFT. */\n",
         "#ifndef NNSP_GEN_TABLES_H\n#define NNSP_GEN_TABLES_H\n#include <stdint.h>\n",
         f"#define NNSP_TBL_MEL_LEN {len(mel)}\n",
         _c_array("int16_t", "nnsp_tbl_window", stft_window()),

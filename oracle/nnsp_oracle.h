@@ -7,8 +7,9 @@
  * bench.py's cpu_baseline leg may load it; the product library never does.
  *
  * Parity status (details in DESIGN.md "Oracle"):
- *   - constant tables: pinned byte-exact against the reference source tables
- *     and the CMSIS-DSP data sections (tests/test_tables.py);
+ *   - constant tables: window, Mel, log and tanh pinned byte-exact against the
+ *     reference source tables (tests/test_tables.py); those of the FFT are the
+ *     nearest q31 values of their cos and sin, parity unpinned;
  *   - post-FFT front end, activations, post-processing, reset logic: pinned
  *     against reference C files compiled here from their own sources
  *     (oracle/_ref -> tests/golden/ref_stages.npz, tests/test_oracle_pinned.py);
@@ -20,8 +21,8 @@
  *     differs from the shipped one only in the byte walk (pinned by
  *     layout.npz) and the live align shift (or_net.portable = 1 reproduces
  *     it; the shipped build's dead shift is trap T1);
- *   - CMSIS arm_rfft_q31 (binary-only third-party code): restated, "parity
- *     unpinned" beyond its tables and a float-DFT check.
+ *   - CMSIS arm_rfft_q31 (third-party code without source in the reference):
+ *     restated, tables included; "parity unpinned" beyond a float-DFT check.
  */
 #ifndef NNSP_ORACLE_H
 #define NNSP_ORACLE_H

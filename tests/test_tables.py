@@ -74,6 +74,44 @@ def test_portable_fft_tables_exact():
     np.testing.assert_array_equal(tables.bitrev8().astype(np.int64), words("br_coeff"))
 
 
+def test_fft_tables_are_the_nearest_q31_values():
+    """Twiddles and split coefficients are cos and sin to the nearest q31
+    value, half a step off at most (1 itself, which q31 has not, saturates);
+    cos and sin here from their series in exact fractions."""
+    from fractions import Fraction
+
+    pi = Fraction(31415926535897932384626433832795028841971693993751, 10 ** 49)
+
+    def sin(n, d):  # of 2 pi n / d
+        x, t, out = 2 * pi * n / d, Fraction(1), Fraction(0)
+        if 4 * n > d:  # to the first quadrant
+            return sin(d - n, d) * -1 if 2 * n > d else sin(d - 2 * n, 2 * d)
+        t = x = Fraction(x).limit_denominator(10 ** 30)
+        for k in range(1, 16):
+            out += t
+            t = Fraction(-t * x * x / ((2 * k) * (2 * k + 1))).limit_denominator(10 ** 30)
+        return out
+
+    def cos(n, d):
+        return sin((4 * n + d) % (4 * d), 4 * d)
+
+    def check(got, value):
+        # cos and sin of the generator are doubles: 2^31 times half a unit in their last place beyond the half step
+        exact = min(value * 2 ** 31, 2 ** 31 - 1)
+        assert abs(int(got) - exact) <= Fraction(1, 2) + Fraction(1, 10 ** 6)
+
+    tw = tables.cfft256_twiddles().reshape(-1, 2)
+    for i in range(192):
+        check(tw[i, 0], 1 if i == 0 else cos(i, 256))
+        check(tw[i, 1], sin(i, 256))
+    split = tables.rfft512_split_coefs().reshape(-1, 3)
+    for k in range(256):
+        s, c = sin(k, 512), 1 if k == 0 else cos(k, 512)
+        check(split[k, 0], (1 - s) / 2)
+        check(split[k, 1], -Fraction(c) / 2)
+        check(split[k, 2], (1 + s) / 2)
+
+
 def test_split_coefficients_are_symmetric():
     """fe_kernel splits bins k and 256 - k together (nnsp_dev.h split_pair),
     which relies on realCoefA/B at 16k being symmetric: A1[256-k] = A1[k],
