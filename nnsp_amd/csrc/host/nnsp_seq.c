@@ -231,7 +231,7 @@ int nnsp_delta_exec_device(const nnsp_delta_args *a, void *stream)
                            {"out", a->out, el},
                            {"beta", a->beta, f},
                            {"g", a->g, a->g ? f : 0},
-                           {"lens", a->lens, a->lens ? f : 0},
+                           {"lens", a->lens, a->lens ? 4 : 0}, /* read without frames too */
                            {"state_in", a->state_in, a->state_in ? 4 : 0},
                            {"state_out", a->state_out, a->state_out ? 4 : 0},
                            {"workspace", a->workspace, need ? 16 : 0}};

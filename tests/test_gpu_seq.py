@@ -225,6 +225,19 @@ def test_delta_no_frames_copies_the_state():
     assert not bool(so.any())
 
 
+def test_delta_no_frames_with_lens():
+    """Lengths are cut to the call's no frames; lengths in host memory are refused, not read."""
+    d = make(2, 0, 1, 1, 16, 16, "bf16")
+    _, so = run_delta(d, 1, "bf16", lens=[5, -1])
+    assert torch.equal(so, d["state"])
+    host, so = np.zeros(2, np.int32), torch.zeros_like(so)
+    with pytest.raises(RuntimeError, match="lens is not memory of device"):
+        gated_delta()(2, 0, 1, 1, 16, 16).exec_device(None, None, None, None, None, None, state_in=ptr(d["state"]),
+                                                      state_out=ptr(so), lens=host.ctypes.data)
+    torch.cuda.synchronize()
+    assert not bool(so.any())
+
+
 def test_delta_chunks_then_frames():
     """A stream taken in pieces of any length ends where one call ends."""
     T, cuts = 210, [0, 100, 101, 102, 166, 170, 210]

@@ -138,6 +138,11 @@ def test_delta_nothing_to_do():
     delta({"q": None, "k": None, "v": None, "beta": None, "out": None}, sizes=(2, 0, 1, 2, 8, 8))()
 
 
+def test_delta_lens_are_checked_without_frames_too():
+    """The copy of the state still reads every stream's length."""
+    refused(delta({"lens": BAD + 2, "state_in": BAD, "state_out": BAD + 4096}, sizes=(2, 0, 1, 2, 8, 8)), "lens is not aligned")
+
+
 def test_null_arguments():
     L = _lib.lib()
     n = C.c_size_t()
