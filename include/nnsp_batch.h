@@ -111,6 +111,8 @@ int nnsp_device_info(int *compute_units, int *clock_khz, char *arch, int arch_le
 #define NNSP_EINVAL (-1)
 #define NNSP_EUNSUPPORTED (-2)
 #define NNSP_ENOMEM (-3)
+/* What a code means; of a negative one, what the calling thread's last refused
+ * call was refused for (another thread's calls do not change it). */
 const char *nnsp_strerror(int code);
 
 #ifdef __cplusplus

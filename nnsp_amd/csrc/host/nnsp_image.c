@@ -18,7 +18,7 @@
 
 #include "nnsp_host.h"
 
-static char g_err[256];
+static _Thread_local char g_err[256]; /* of the thread's last refusal */
 
 void nnsp_set_error(const char *fmt, ...)
 {

@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import re
 import subprocess
+import threading
 
 import pytest
 
@@ -141,6 +142,27 @@ def test_delta_nothing_to_do():
 def test_delta_lens_are_checked_without_frames_too():
     """The copy of the state still reads every stream's length."""
     refused(delta({"lens": BAD + 2, "state_in": BAD, "state_out": BAD + 4096}, sizes=(2, 0, 1, 2, 8, 8)), "lens is not aligned")
+
+
+def test_refusals_keep_to_their_thread():
+    """What one thread's call was refused for is not overwritten by another thread's refusal."""
+    L = _lib.lib()
+    plans = [GatedDelta(1, 1, 1, 1, 8, 8) for _ in range(2)]
+    plans[0].args.out, plans[1].args.dtype = BAD, 7
+    assert L.nnsp_delta_exec_device(plans[0]._ref, None) == _lib.NNSP_EINVAL
+    mine = L.nnsp_strerror(_lib.NNSP_EINVAL)
+    seen = []
+
+    def other():
+        seen.append(L.nnsp_strerror(_lib.NNSP_EINVAL))
+        assert L.nnsp_delta_exec_device(plans[1]._ref, None) == _lib.NNSP_EINVAL
+        seen.append(L.nnsp_strerror(_lib.NNSP_EINVAL))
+
+    t = threading.Thread(target=other)
+    t.start()
+    t.join()
+    assert b"q is NULL" in mine and L.nnsp_strerror(_lib.NNSP_EINVAL) == mine
+    assert seen[0] == b"invalid argument" and b"unknown dtype" in seen[1]
 
 
 def test_null_arguments():
