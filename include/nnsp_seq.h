@@ -63,14 +63,18 @@ extern "C" {
  * state is dropped; it may be state_in itself (not a part of it).  out must
  * not overlap an input, nor any state.
  * g is a logarithm of the decay, normally <= 0; -infinity clears the state.
- * The state, sums and exponentials are held in 32 bits or more.
+ * The state, sums and exponentials are held in 32 bits or more.  Calls of more
+ * than NNSP_DELTA_STEP_FRAMES frames may run in chunks of up to 64 on the matrix
+ * cores, whose products take the state, what is made of it and fp32 q and k in 22
+ * bits, each column of the state and of v under scales of its own; where the
+ * output is bf16, what only the output takes (the state for S^T q^, and the
+ * products of a chunk's frames among each other) goes in with 11 bits.  Decays
+ * above 1 (g > 0) cost such calls precision by their product over 64 frames.
  *
  * A value that is not finite in frame t spreads, as the recurrence has it, to
- * the later frames of its stream and head; where a call has more than
- * NNSP_DELTA_STEP_FRAMES frames it may reach the other frames of the same 64
- * (64 n .. 64 n + 63), earlier ones too.  In such calls a column of v or of the
- * state is as exact as 2^-38 of the largest among the 16 or 32 columns beside
- * it, and decays above 1 (g > 0) cost precision by their product over 64 frames.
+ * the later frames of its stream and head, from v and the state to their own
+ * column only; in chunks it may reach the other frames of the same 64
+ * (64 n .. 64 n + 63), earlier ones too.
  *
  * workspace: nnsp_delta_workspace() bytes of device memory, 16-byte aligned,
  * used by this call only while its kernels run (one workspace per call in

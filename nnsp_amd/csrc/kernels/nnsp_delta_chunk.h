@@ -14,10 +14,14 @@
 // Numbers.  The state, T and U are 32-bit values, and the matrix cores take 16
 // bits: each is scaled by a power of two and split into an fp16 high and low
 // part, 22 bits in all, and products keep hi hi + hi lo + lo hi, accumulated in
-// 32 bits.  The powers come from the largest magnitude among a wave's columns
-// or from a bound; an fp16 pair under a bound of 2^14 is good to 2^-24 in
-// absolute terms, 2^-38 of the bound, so neither a loose bound nor a column much
-// smaller than its neighbours costs precision.  q and k go in with their rows
+// 32 bits.  A column has powers of its own, as it is a recurrence of its own:
+// neither its precision nor its range depends on the columns beside it, and what
+// is not finite stays in it.  They come from the column's largest magnitude or
+// from a bound.  An fp16 pair is good to 2^-23 of its value, or to 2^-25, which is
+// 2^-39 of what is scaled to 2^14; a bound is at most 64 times the largest term of
+// the sum it is of (and 2^5 more where R's own was a bound), so that this stays
+// below 2^-28 of that term, and adding the sum up in 32 bits loses 2^-24 of it.
+// T has a power a row tile, shared by all columns.  q and k go in with their rows
 // scaled too: fp16 and bf16 in one part (exact down to 2^-19 and 2^-28 of a row's
 // largest, to 2^-30 and 2^-39 of it below), fp32 in two.  All other factors
 // (norms, decays, beta) multiply in 32 bits outside the products.  For bf16
@@ -201,6 +205,8 @@ struct Geo {
 template <class T, int NKT, int C>
 struct KQ {
     static constexpr int KP = std::is_same<T, float>::value ? 2 : 1, KS = NKT * 32 + 8;
+    // 64 elements of K at most: rows are scaled to a length below 2^6 in fp16, to a largest element below 2^15 else
+    static constexpr float BOUND64 = std::is_same<T, _Float16>::value ? 0x1p12f : 0x1p21f;
     alignas(16) _Float16 K[KP][C][KS], Q[KP][C][KS];
 };
 // what else a chunk's products take; e() is a decay, G the sum of g
@@ -570,34 +576,33 @@ __device__ __forceinline__ f32x4 tile_of(const T (*V)[VS], int n, int l15, int g
 
 // K S0 and R of a chunk of 32 with nt live tiles of 16 frames, for this wave's
 // columns; with LOW outputs also Q S0, whose high part outlasts R otherwise (in
-// fewer registers).  S holds the state times 1 / sinv, a power of two.
+// fewer registers).  S holds the state times 1 / sinv, powers of two; a lane's
+// scales are those of its column.
 template <class T, int NKT, int NB>
 struct Chunk {
     using G = Geo<T, NKT, NB>;
     static constexpr bool LOW = G::OP == 2;
     f32x4 R[2][NB], O[LOW ? 2 : 1][NB];
     h8 shi[NKT][NB];
-    float smax, rmax, sout;
+    float smax[NB], rmax[NB], sout[NB];
 
     __device__ __forceinline__ void first(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], const f32x4 (&S)[2 * NKT][NB],
-                                          float sinv, int lane, int nt) {
+                                          const float (&sinv)[NB], int lane, int nt) {
         const int l15 = lane & 15, g = lane >> 4;
         const f32x4 zero = {0, 0, 0, 0};
         h8 lo[NKT][NB];
-        smax = rmax = 0.0f;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < NB; ++n) {
+            float m = 0.0f, inv;
 #pragma unroll
-            for (int t = 0; t < 2 * NKT; ++t) smax = amax4(smax, S[t][n]);
-        smax = wave_max(smax);
-        float inv;
-        const float sc = scale_of(smax, inv);
-        inv = fmaf(inv, sinv, poison(smax));
-        sout = inv;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
+            for (int t = 0; t < 2 * NKT; ++t) m = amax4(m, S[t][n]);
+            smax[n] = max_xor16_32(m);
+            rmax[n] = 0.0f;
+            const float sc = scale_of(smax[n], inv);
+            sout[n] = fmaf(inv, sinv[n], poison(smax[n]));
 #pragma unroll
             for (int t = 0; t < NKT; ++t) split<true>(S[2 * t][n], S[2 * t + 1][n], all4(sc), all4(sc), shi[t][n], lo[t][n]);
+        }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             if (m >= nt) {
@@ -626,14 +631,14 @@ struct Chunk {
                     }
                 }
             }
-            const f32x4 b = ld4(&Y.beta[16 * m + 4 * g]), fx = ld4(&Y.fx[16 * m + 4 * g]) * -inv;
+            const f32x4 b = ld4(&Y.beta[16 * m + 4 * g]), f = ld4(&Y.fx[16 * m + 4 * g]);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                const f32x4 v = tile_of<T>(V + 16 * m, n, l15, g) * b;
+                const f32x4 v = tile_of<T>(V + 16 * m, n, l15, g) * b, fx = f * -sout[n];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) R[m][n][r] = fmaf(fx[r], x[n][r], v[r]);
-                if (LOW) O[LOW ? m : 0][n] = o[n] * (ld4(&Y.fq[16 * m + 4 * g]) * inv);
-                rmax = amax4(rmax, R[m][n]);
+                if (LOW) O[LOW ? m : 0][n] = o[n] * (ld4(&Y.fq[16 * m + 4 * g]) * sout[n]);
+                rmax[n] = amax4(rmax[n], R[m][n]);
             }
         }
     }
@@ -641,24 +646,28 @@ struct Chunk {
     // U, the output (into V) and the state after the chunk; mid() is called once on the way
     template <class F>
     __device__ __forceinline__ void second(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], f32x4 (&S)[2 * NKT][NB],
-                                           float& sinv, int lane, int nt, const F& mid) {
+                                           float (&sinv)[NB], int lane, int nt, const F& mid) {
         const int l15 = lane & 15, g = lane >> 4;
         const f32x4 zero = {0, 0, 0, 0};
         f32x4 u[2][NB];  // U = u ti rinv, where |u| is at most 32 products of 2^30
-        float rinv;
+        float rs[NB], ti[NB];
         h8 hi[NB], lo[NB];
-        rmax = wave_max(rmax);
-        const float rs = scale_of(rmax, rinv);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) split<true>(R[0][n], R[1][n], all4(rs), all4(rs), hi[n], lo[n]);
+        for (int n = 0; n < NB; ++n) {
+            float inv;
+            rmax[n] = max_xor16_32(rmax[n]);
+            rs[n] = scale_of(rmax[n], inv);
+            ti[n] = fmaf(Y.ti[0], inv, poison(rmax[n]));
+            split<true>(R[0][n], R[1][n], all4(rs[n]), all4(rs[n]), hi[n], lo[n]);
+        }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             const h8 th = Y.T_[0].operand(m, l15, 0, g), tl = Y.T_[1].operand(m, l15, 0, g);
 #pragma unroll
             for (int n = 0; n < NB; ++n) u[m][n] = mma(tl, hi[n], mma(th, lo[n], mma(th, hi[n], zero)));
         }
-        const float ti = fmaf(Y.ti[0], rinv, poison(rmax));  // u to below 2^14: times 2^-22
 #pragma unroll
+        // u to below 2^14: times 2^-22
         for (int n = 0; n < NB; ++n) split<LOW>(u[0][n], u[1][n], all4(0x1p-22f), all4(0x1p-22f), hi[n], lo[n]);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -677,24 +686,29 @@ struct Chunk {
 #pragma unroll
                     for (int n = 0; n < NB; ++n) qs[n] = mma(q, shi[s][n], s ? qs[n] : zero);
                 }
-            const f32x4 pi = ld4(&Y.pi[16 * m + 4 * g]) * (ti * 0x1p22f), fq = ld4(&Y.fq[16 * m + 4 * g]) * sout;
+            const f32x4 p = ld4(&Y.pi[16 * m + 4 * g]), f = ld4(&Y.fq[16 * m + 4 * g]);
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int n = 0; n < NB; ++n) {
+                const f32x4 pi = p * (ti[n] * 0x1p22f), fq = f * sout[n];
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     V[16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], LOW ? O[LOW ? m : 0][n][r] : fq[r] * qs[n][r]);
+            }
         }
         mid();
         // S1, accumulated onto the decayed state in the scale s of U fk; where U is next to nothing, in 2^13 of the
         // decayed state's own, so that neither leaves its range (2^100 at most: the state's factor stays finite)
         const float all = Y.all;
-        float zi, li;
-        const float z = scale_of(Y.fkmax, zi) * 0x1p-36f, low = scale_of(fmaxf(smax * sinv * (all * 0x1p-13f), 0x1p-86f), li);
-        const float s = fminf(z * inverse2(Y.ti[0]) * rs, low), d = all * s * sinv;  // true U fk times s = u fk (ti s)
-        sinv = inverse2(s);
-        const f32x4 f0 = ld4(&Y.fk[4 * g]) * (ti * s), f1 = ld4(&Y.fk[16 + 4 * g]) * (ti * s);
+        float zi;
+        const float z = scale_of(Y.fkmax, zi) * 0x1p-36f * inverse2(Y.ti[0]);
+        const f32x4 fk0 = ld4(&Y.fk[4 * g]), fk1 = ld4(&Y.fk[16 + 4 * g]);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
+            float li;
+            const float low = scale_of(fmaxf(smax[n] * sinv[n] * (all * 0x1p-13f), 0x1p-86f), li);
+            const float s = fminf(z * rs[n], low), d = all * s * sinv[n];  // true U fk times s = u fk (ti s)
+            sinv[n] = inverse2(s);
+            const f32x4 f0 = fk0 * (ti[n] * s), f1 = fk1 * (ti[n] * s);
             split<true>(u[0][n], u[1][n], f0, f1, hi[n], lo[n]);
 #pragma unroll
             for (int t = 0; t < 2 * NKT; ++t) S[t][n] *= d;
@@ -865,14 +879,6 @@ struct Cols {
         }
         vp += vc;
     }
-    __device__ __forceinline__ float largest() const {
-        float m = 0.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf((float)x[i][j]));
-        return m;
-    }
     __device__ __forceinline__ void stage(T (*V)[VS]) const {
         if (row < ROWS)
 #pragma unroll
@@ -970,11 +976,13 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
     const int role = (wave + (spare ? 1 : blockIdx.x)) & (NW - 1);
 
     f32x4 S[2 * NKT][NB];
-    float sinv = 1.0f;
+    float sinv[NB];
 #pragma unroll
-    for (int t = 0; t < 2 * NKT; ++t)
+    for (int j = 0; j < NB; ++j) {
+        sinv[j] = 1.0f;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) S[t][j] = f32x4{0, 0, 0, 0};
+        for (int t = 0; t < 2 * NKT; ++t) S[t][j] = f32x4{0, 0, 0, 0};
+    }
     if (a.state_in && live) {
         const float* sp = a.state_in + so;
         each_state<NKT, NB, FAST>(a, c0, lane, [&](int t, int j, int r, int base, unsigned at, bool in) {
@@ -1016,7 +1024,7 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
     if (a.state_out && live) {
         float* sq = a.state_out + so;
         each_state<NKT, NB, FAST>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
-            if (in) (sq + base)[at] = S[t][j][r] * sinv;
+            if (in) (sq + base)[at] = S[t][j][r] * sinv[j];
         });
     }
 }
@@ -1081,7 +1089,7 @@ __global__ __launch_bounds__(576) void delta_pipe_kernel(const nnsp_delta_args a
     const int c0 = (cb * 4 + wave) * 16;
     const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
     f32x4 S[2 * NKT][1];
-    float sinv = 1.0f;
+    float sinv[1] = {1.0f};
 #pragma unroll
     for (int t = 0; t < 2 * NKT; ++t) S[t][0] = f32x4{0, 0, 0, 0};
     Cols<T, NKT, 1, FAST, CF, CF> cols(a, s, h, 0, c0, lane);
@@ -1112,7 +1120,7 @@ __global__ __launch_bounds__(576) void delta_pipe_kernel(const nnsp_delta_args a
     if (a.state_out) {
         float* sq = a.state_out + so;
         each_state<NKT, 1, FAST>(a, c0, here(lane), [&](int t, int j, int r, int base, unsigned at, bool in) {
-            if (in) (sq + base)[at] = S[t][j][r] * sinv;
+            if (in) (sq + base)[at] = S[t][j][r] * sinv[j];
         });
     }
 }
@@ -1208,11 +1216,12 @@ __device__ __forceinline__ void put_part(h8 (*dst)[64], int lane, int half, cons
 }
 
 // What the four waves of a scan hand each other: B operands of 32 rows x 16
-// columns, high and low, and the largest magnitudes that set their scales.
+// columns, high and low, and each column's largest magnitudes of a wave, which
+// set its scales.
 template <int NKT, int NB>
 struct Exchange {
     h8 S[NKT][NB][2][64], R[2][NB][2][64], U[2][NB][2][64], F[2][NB][2][64];  // S0, R, U for the output, U fk for the state
-    float smax[4], vmax[4], fmax[4];
+    float smax[NB][16][4], vmax[NB][16][4], fmax[NB][16][4];
 };
 
 // XB, YB: buffers of the two images
@@ -1233,10 +1242,10 @@ struct ScanLds {
 // the products' own reads of LDS (64 chunks of 128 x 128 bf16: 127 us, all after
 // the first barrier 148, none 121).  Where LDS has no room for two of an image, it
 // comes after the third barrier, when the one before has been read.
-// Scales have to be the same for all four before anybody has seen all values:
-// they come from bounds (|R| <= bmax |v| + xmax |S|, |u| <= 64 2^30,
-// |S1| <= all |S0| + 64 2^15 |U fk|) over the magnitudes exchanged at the
-// barriers, looser than the largest value by 2^4 to 2^8.
+// A column's scales have to be the same for all four before anybody has seen all
+// its values: they come from bounds (|R| <= bmax |v| + xmax |S|, |u| <= 64 2^30,
+// |S1| <= all |S0| + BOUND64 |U fk|) over the column's magnitudes exchanged at the
+// barriers, sums of their largest terms.
 template <class T, int NKT, int NB, bool FAST, int XB, int YB>
 __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a, const Slab b) {
     using G = Geo<T, NKT, NB>;
@@ -1280,7 +1289,19 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
     const long long so = ((long long)s * a.value_heads + h) * a.dk * a.dv;
     const f32x4 zero = {0, 0, 0, 0};
     f32x4 S[TPW][NB];
-    float sinv = 1.0f, m = 0.0f;
+    float sinv[NB], sbound[NB], m[NB];  // of this lane's columns; sbound: of |S|, the registers' values
+    // of all four waves, from what each has put where this lane's columns are
+    const auto put_max = [&](float (*p)[16][4], int lane) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const float x = max_xor16_32(m[n]);
+            if (lane < 16) p[n][lane][wave] = x;
+        }
+    };
+    const auto max4 = [](const float* p) {
+        const f32x4 x = ld4(p);
+        return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+    };
     // f(i, j, r, place, in) for element r of this wave's tile (i, j), as each_state
     const auto own_state = [&](int lane, const auto& f) {
 #pragma unroll
@@ -1296,23 +1317,22 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
             }
     };
 #pragma unroll
-    for (int i = 0; i < TPW; ++i)
+    for (int j = 0; j < NB; ++j) {
+        sinv[j] = 1.0f;
+        m[j] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) S[i][j] = zero;
+        for (int i = 0; i < TPW; ++i) S[i][j] = zero;
+    }
     if (b.state_in)
         own_state(lane_, [&](int i, int j, int r, long long at, bool in) {
             const float x = b.state_in[at];
             S[i][j][r] = in ? x : 0.0f;
-            m = fmaxf(m, fabsf(S[i][j][r]));
+            m[j] = fmaxf(m[j], fabsf(S[i][j][r]));
         });
-    m = wave_max(m);
-    if (lane_ == 0) L.E.smax[wave] = m;
+    put_max(L.E.smax, lane_);
     __syncthreads();
-    const auto max4 = [](const float* p) {
-        const f32x4 x = ld4(p);
-        return fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-    };
-    float sbound = max4(L.E.smax);  // of |S|, the registers' values
+#pragma unroll
+    for (int n = 0; n < NB; ++n) sbound[n] = max4(L.E.smax[n][lane_ & 15]);
 
     Cols<T, NKT, NB, FAST, 16, C> cols(a, s, h, (long long)b.first * C + 16 * wave, c0, lane_);
     if (n > 0) cols.fetch(n - 16 * wave);
@@ -1323,34 +1343,40 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
         const TP<T, C>& Y = L.Y[i & (YB - 1)];
         Exchange<NKT, NB>& E = L.E;
         // 1: the state's parts, and what bounds R
-        float inv;
-        {
-            const float sc = scale_of(sbound, inv);
-            inv *= sinv;
-            m = 0.0f;
+        float inv[NB];
+        f32x4 vt[NB];
+        cols.stage(L.V[wave]);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) vt[n] = tile_of<T>(L.V[wave], n, l15, g);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            const float sc = scale_of(sbound[n], inv[n]);
+            inv[n] *= sinv[n];
+            m[n] = 0.0f;
 #pragma unroll
             for (int j = 0; j < TPW; ++j) {
                 const int t = wave * TPW + j;
                 if (t >= 2 * NKT) continue;  // not a tile of the state; its registers are never handed on
-#pragma unroll
-                for (int k = 0; k < NB; ++k) {
-                    put_part<true>(E.S[t >> 1][k], lane, t & 1, S[j][k], all4(sc));
-                    m = amax4(m, S[j][k]);
-                }
+                put_part<true>(E.S[t >> 1][n], lane, t & 1, S[j][n], all4(sc));
+                m[n] = amax4(m[n], S[j][n]);
             }
-            m = wave_max(m);
-            const float v = wave_max(cols.largest());
-            cols.stage(L.V[wave]);
-            if (lane == 0) E.smax[wave] = m, E.vmax[wave] = v;
         }
+        put_max(E.smax, lane);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) m[n] = amax4(0.0f, vt[n]);
+        put_max(E.vmax, lane);
         __syncthreads();
         // 2: R and Q S0 of this wave's frames
-        const float sreg = max4(E.smax), smax = sreg * sinv;  // the registers' values, the true ones
-        const float vmax = max4(E.vmax), bad = poison(sreg) + poison(vmax);
-        float rinv;
-        const float sc = scale_of(Y.bmax * vmax + Y.xmax * smax, rinv);
-        rinv += bad;
-        inv += bad;
+        float sreg[NB], smax[NB], sc[NB], rinv[NB];  // the registers' values, the true ones; the scale of R and its inverse
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            sreg[n] = max4(E.smax[n][l15]);
+            smax[n] = sreg[n] * sinv[n];
+            const float vmax = max4(E.vmax[n][l15]), bad = poison(sreg[n]) + poison(vmax);
+            sc[n] = scale_of(Y.bmax * vmax + Y.xmax * smax[n], rinv[n]);
+            rinv[n] += bad;
+            inv[n] += bad;
+        }
         f32x4 O[NB];
         {
             f32x4 x[NB];
@@ -1371,24 +1397,35 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
                     }
                 }
             }
-            const f32x4 bt = ld4(&Y.beta[16 * wave + 4 * g]), fx = ld4(&Y.fx[16 * wave + 4 * g]) * -inv;
-            const f32x4 fq = ld4(&Y.fq[16 * wave + 4 * g]) * inv;
+            const f32x4 bt = ld4(&Y.beta[16 * wave + 4 * g]), fx = ld4(&Y.fx[16 * wave + 4 * g]);
+            const f32x4 fq = ld4(&Y.fq[16 * wave + 4 * g]);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                f32x4 r = tile_of<T>(L.V[wave], n, l15, g) * bt;
+                const f32x4 f = fx * -inv[n];
+                f32x4 r = vt[n] * bt;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) r[e] = fmaf(fx[e], x[n][e], r[e]);
-                put_part<true>(E.R[wave >> 1][n], lane, wave & 1, r, all4(sc));
-                O[n] *= fq;
+                for (int e = 0; e < 4; ++e) r[e] = fmaf(f[e], x[n][e], r[e]);
+                put_part<true>(E.R[wave >> 1][n], lane, wave & 1, r, all4(sc[n]));
+                O[n] *= fq * inv[n];
             }
         }
         if (left > C) cols.fetch(left - C - 16 * wave);
         // what the next steps take of the images and know of the scales (see advance()), before the waits
         const float tmax = max4(Y.ti), cinv = tmax * 0x1p22f, c = inverse2(cinv), all = Y.all, ti = Y.ti[wave];
-        float zi, li;
-        const float z = scale_of(Y.fkmax, zi) * 0x1p-14f, low = scale_of(fmaxf(smax * (all * 0x1p-13f), 0x1p-86f), li);
-        const float s1 = fminf(c * z * sc, low), d = all * s1 * sinv;
-        const f32x4 f = ld4(&Y.fk[16 * wave + 4 * g]) * (ti * (s1 * rinv));
+        float zi, s1[NB], d[NB];
+        const float z = scale_of(Y.fkmax, zi) * 0x1p-14f;
+        f32x4 f[NB];
+        {
+            const f32x4 fk = ld4(&Y.fk[16 * wave + 4 * g]);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                float li;
+                const float low = scale_of(fmaxf(smax[n] * (all * 0x1p-13f), 0x1p-86f), li);
+                s1[n] = fminf(c * z * sc[n], low);
+                d[n] = all * s1[n] * sinv[n];
+                f[n] = fk * (ti * (s1[n] * rinv[n]));
+            }
+        }
         h8 th[2], tl[2];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -1408,15 +1445,13 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
                     u[n] = mma(tl[s], hi, mma(th[s], lo, mma(th[s], hi, s ? u[n] : zero)));
                 }
             }
-            m = 0.0f;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                put_part<true>(E.F[wave >> 1][n], lane, wave & 1, u[n], f);
+                put_part<true>(E.F[wave >> 1][n], lane, wave & 1, u[n], f[n]);
                 put_part<LOW>(E.U[wave >> 1][n], lane, wave & 1, u[n], all4(ti * c));
-                m = amax4(m, u[n] * f);
+                m[n] = amax4(0.0f, u[n] * f[n]);
             }
-            m = wave_max(m);
-            if (lane == 0) E.fmax[wave] = m;
+            put_max(E.fmax, lane);
 #pragma unroll
             for (int j = 0; j < TPW; ++j) {
                 const int t = min(wave * TPW + j, 2 * NKT - 1);
@@ -1430,7 +1465,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
                         kt[j][s][part] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
                     }
 #pragma unroll
-                for (int n = 0; n < NB; ++n) S[j][n] *= d;
+                for (int n = 0; n < NB; ++n) S[j][n] *= d[n];
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s)
@@ -1438,12 +1473,15 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
                     ph[s] = Y.P_[0].operand(wave, l15, s, g);
                     if (LOW) pl[s] = Y.P_[G::OP - 1].operand(wave, l15, s, g);
                 }
-            pi = ld4(&Y.pi[16 * wave + 4 * g]) * (rinv * cinv);
+            pi = ld4(&Y.pi[16 * wave + 4 * g]);
         }
         __syncthreads();
         // 4: this wave's rows of the state, its frames of the output
-        sbound = fmaf(d, sreg, 0x1p21f * max4(E.fmax));
-        sinv = inverse2(s1);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            sbound[n] = fmaf(d[n], sreg[n], KQ<T, NKT, C>::BOUND64 * max4(E.fmax[n][l15]));
+            sinv[n] = inverse2(s1[n]);
+        }
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -1468,16 +1506,18 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
                 }
             }
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+            for (int n = 0; n < NB; ++n) {
+                const f32x4 p = pi * (rinv[n] * cinv);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) L.V[wave][4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], O[n][r]);
+                for (int r = 0; r < 4; ++r) L.V[wave][4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], p[r], O[n][r]);
+            }
         }
         wait_loads();
         cols.store(L.V[wave], left - 16 * wave);
     }
     if (b.state_out)
         own_state(here(lane_), [&](int i, int j, int r, long long at, bool in) {
-            if (in) b.state_out[at] = S[i][j][r] * sinv;
+            if (in) b.state_out[at] = S[i][j][r] * sinv[j];
         });
 }
 

@@ -1,0 +1,119 @@
+"""Delta rule on the GPU: every stream, head and column of the state by itself,
+against the rule in 64 bits.
+
+A column of the state, with its column of v and out, is a recurrence of its
+own: S'^T k, u, S and the output's column take nothing from the columns beside
+it.  So each is bounded by its own size, with big = the largest length of the
+state's column over the frames (its start too) plus the largest |v| of it:
+
+  * Within a chunk seven roundings of an operand or a sum stand between S0 and
+    S1 (q or k and S0 in K S0; R, T in T R; U fk and K in K^T U; each an fp16
+    pair of 22 bits, off by 2^-23 of its value, lo * lo of two pairs left out,
+    2^-24; and sums in 32 bits, 2^-24 a step of a few).  By Cauchy-Schwarz each
+    is off by its part of |k| |S|, whatever dk is, so all of them by less than
+    8 * 2^-23 of big, and by twice that where the inverse's rows add up what
+    cancels.  |beta k k^T| <= 1 lets no error grow, and errors of the frames
+    have random signs: part = 16 * 2^-23 * sqrt(frames).
+  * out = scale q . S: scale * part * big, and one rounding to its type (half a
+    step of the value, or of the smallest subnormal).  For bf16 three operands
+    of what only the output takes have 11 bits, 2^-12 each: 2^-10 of big.
+"""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_seq import DT, HALF, make, run_delta
+
+pytestmark = pytest.mark.gpu
+
+
+def rule(d, scale, lens=None, eps=1e-6):
+    """out, the final state, and big [S][hv][dv], in 64 bits on the GPU."""
+    q, k, v, g, beta, st = (d[n].double() for n in ("q", "k", "v", "g", "beta", "state"))
+    S, T, hv = v.shape[:3]
+    rep = hv // q.shape[2]
+    q = q / (q.square().sum(-1, keepdim=True) + eps).sqrt()
+    k = k / (k.square().sum(-1, keepdim=True) + eps).sqrt()
+    out, big = torch.zeros_like(v), st.square().sum(2)
+    for t in range(T):
+        kt, qt = k[:, t].repeat_interleave(rep, 1), q[:, t].repeat_interleave(rep, 1)
+        new = st * torch.exp(g[:, t])[..., None, None]
+        u = beta[:, t][..., None] * (v[:, t] - (new * kt[..., None]).sum(2))
+        new = new + kt[..., None] * u[..., None, :]
+        if lens is not None:
+            new = torch.where((t < lens)[:, None, None, None], new, st)
+        st = new
+        out[:, t] = scale * (st * qt[..., None]).sum(2)
+        big = torch.maximum(big, st.square().sum(2))
+    return out, st, big.sqrt() + v.abs().amax(1)
+
+
+def check(got, ref, scale, dtype, T):
+    (out, so), (ro, rs, big) = got, ref
+    part = 16 * 2.0 ** -23 * np.sqrt(T)
+    least = 2.0 ** -25 if dtype == "f16" else 2.0 ** -134 if dtype == "bf16" else 2.0 ** -150
+    bound = HALF[dtype] * ro.abs() + least + (scale * big * (part + (2.0 ** -10 if dtype == "bf16" else 0)))[:, None]
+    for what, off, most in (("out", (out.double() - ro).abs(), bound), ("state", (so.double() - rs).abs(), (part * big)[:, :, None])):
+        at = torch.nonzero(~(off <= most))
+        assert len(at) == 0, f"{what}: {len(at)} of {off.numel()} beyond the bound, at {at[0].tolist()} by {float((off / most).max()):.3g}"
+
+
+# one for each way that a call runs: frame by frame, three chunks at once, many rows (by 64 and 128 columns a workgroup, with
+# waves to spare and without), wide keys, two passes by 16 and by 32 columns, and by several slabs
+WAYS = [(2, 2, 1, 2, 64, 72), (2, 100, 1, 2, 64, 72), (1, 40, 2, 2, 128, 128), (2, 70, 1, 2, 61, 47), (300, 40, 1, 2, 64, 48),
+        (200, 70, 1, 2, 64, 128), (140, 40, 1, 2, 128, 136), (260, 33, 1, 1, 96, 24), (3, 45, 1, 2, 200, 72), (200, 40, 1, 2, 160, 128),
+        (1, 300, 1, 2, 64, 64), (2, 333, 1, 2, 128, 40), (10, 420, 2, 4, 64, 128), (9, 420, 2, 4, 128, 128), (1, 200, 1, 2, 192, 64),
+        (1, 420, 1, 2, 61, 47), (1, 1900, 32, 32, 128, 128)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("S,T,hk,hv,dk,dv", WAYS)
+def test_delta_every_column_by_its_own_size(S, T, hk, hv, dk, dv, dtype):
+    """Columns of all sizes side by side, fast and slow heads, loud and quiet streams."""
+    d = make(S, T, hk, hv, dk, dv, dtype, seed=S + T + dv)
+    low = [0, -5, -20, 3, -12] if dtype == "f16" else [0, -12, -24, 3, -40]
+    col = 2.0 ** torch.tensor([low[(i * 3 + i // 16) % 5] for i in range(dv)], dtype=torch.float32).cuda()
+    # fp16's own range is not as wide: nothing is written to the faintest columns there
+    d["v"] = (d["v"].float() * (col * (col > 2.0 ** -10) if dtype == "f16" else col)).to(DT[dtype])
+    d["state"] = d["state"] * col
+    d["g"] = d["g"] * torch.tensor([4.0 ** -(h % 4) for h in range(hv)]).cuda()
+    got = run_delta(d, hk, dtype)
+    check(got, rule(d, dk ** -0.5), dk ** -0.5, dtype, T)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("S,T,hk,hv,dk,dv", [w for w in WAYS if w[1] < 1000])
+def test_delta_columns_do_not_touch_each_other(S, T, hk, hv, dk, dv, dtype):
+    """What stands in one column, be it an infinity or a NaN, changes no bit of the others."""
+    d = make(S, T, hk, hv, dk, dv, dtype, seed=S + T)
+    out, so = run_delta(d, hk, dtype)
+    hit = [2, 17, 18, dv - 1]
+    keep = [c for c in range(dv) if c not in hit]
+    d["state"][:, :, 3, 2] = float("inf")
+    d["v"][:, T // 2:, :, 17] = float("-inf")
+    d["v"][:, T - 1, :, 18] = float("nan")
+    d["v"][..., dv - 1] *= 1024
+    out2, so2 = run_delta(d, hk, dtype)
+    assert torch.equal(out[..., keep], out2[..., keep]) and torch.equal(so[..., keep], so2[..., keep])
+    for c in (2, 17, 18):
+        assert not bool(torch.isfinite(out2[:, T - 1, :, c]).any())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("S,T,hk,hv,dk,dv", WAYS[:-1])
+def test_delta_a_stream_by_itself_and_among_others(S, T, hk, hv, dk, dv, dtype):
+    """A stream's results do not depend on what the call's other streams hold (how many they are may choose another
+    kernel, whose results are as exact)."""
+    d = make(S, T, hk, hv, dk, dv, dtype, seed=S + dk)
+    d["g"] = d["g"] * torch.tensor([4.0 ** -(h % 4) for h in range(hv)]).cuda()
+    out, so = run_delta(d, hk, dtype)
+    one = {n: x[-1:].contiguous() for n, x in d.items()}
+    ref = rule(one, dk ** -0.5)
+    check((out[-1:], so[-1:]), ref, dk ** -0.5, dtype, T)
+    check(run_delta(one, hk, dtype), ref, dk ** -0.5, dtype, T)
+    if S > 1:
+        for x in d.values():
+            x[:-1] = x[:-1].flip(0) * 3
+        d["v"][0], d["k"][0] = float("nan"), float("inf")
+        out2, so2 = run_delta(d, hk, dtype)
+        assert torch.equal(out[-1], out2[-1]) and torch.equal(so[-1], so2[-1])
