@@ -365,7 +365,7 @@ __device__ __forceinline__ void make_factors(const KQ<T, NKT, C>&, TP<T, C>& Y, 
         const float lo = scan_min<C>(h, lane), kn = wave_max(M.kn[i]);
         float inv;
         const float qx = M.qx[i], sc = scale_of(M.qn[i] * kn * exp2_fast(fminf(h - lo, 120.0f)), inv);
-        Y.pi[i] = inv;
+        Y.pi[i] = inv + poison(kn);
         M.pb[i] = qx * sc;
         M.pr[i] = qx * sc * exp2_fast((h - M.gh[s]) + (l - M.gl[s]));
     } else {
@@ -524,8 +524,9 @@ __device__ __forceinline__ void make_tp(const KQ<T, NKT, 64>& X, TP<T, 64>& Y, M
     __syncthreads();
     {
         float inv;
-        const float s = scale_of(wave_max(m), inv);
-        if (lane == 0) Y.ti[wave] = inv;
+        m = wave_max(m);
+        const float s = scale_of(m, inv);
+        if (lane == 0) Y.ti[wave] = inv + poison(m);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j <= (wave | 1)) put_t(Y, t[j], s, wave, j, l15, g);
@@ -551,8 +552,8 @@ __device__ __forceinline__ void make_t(TP<T, 32>& Y, const TriA<32>& A, int lane
 #pragma unroll
     for (int r = 0; r < 4; ++r) t = __builtin_amdgcn_mfma_f32_16x16x4f32(-d[r], y[r], t, 0, 0, 0);
     float inv;
-    const float s = scale_of(wave_max(amax4(amax4(amax4(0.0f, t0), t1), t)), inv);
-    if (lane == 0) Y.ti[0] = inv;
+    const float m = wave_max(amax4(amax4(amax4(0.0f, t0), t1), t)), s = scale_of(m, inv);
+    if (lane == 0) Y.ti[0] = inv + poison(m);
     put_t(Y, t0, s, 0, 0, l15, g);
     put_t(Y, f32x4{0, 0, 0, 0}, s, 0, 1, l15, g);
     put_t(Y, t, s, 1, 0, l15, g);
@@ -1368,11 +1369,12 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
         __syncthreads();
         // 2: R and Q S0 of this wave's frames
         float sreg[NB], smax[NB], sc[NB], rinv[NB];  // the registers' values, the true ones; the scale of R and its inverse
+        const float shared = poison(Y.bmax) + poison(Y.xmax);
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             sreg[n] = max4(E.smax[n][l15]);
             smax[n] = sreg[n] * sinv[n];
-            const float vmax = max4(E.vmax[n][l15]), bad = poison(sreg[n]) + poison(vmax);
+            const float vmax = max4(E.vmax[n][l15]), bad = shared + poison(sreg[n]) + poison(vmax);
             sc[n] = scale_of(Y.bmax * vmax + Y.xmax * smax[n], rinv[n]);
             rinv[n] += bad;
             inv[n] += bad;

@@ -27,21 +27,23 @@ from test_gpu_seq import DT, HALF, make, run_delta
 pytestmark = pytest.mark.gpu
 
 
-def rule(d, scale, lens=None, eps=1e-6):
+def rule(d, scale, eps=1e-6):
     """out, the final state, and big [S][hv][dv], in 64 bits on the GPU."""
+    unit = {n: d[n].double() / (d[n].double().square().sum(-1, keepdim=True) + eps).sqrt() for n in ("q", "k")}
+    return rule_given(dict(d, **unit), scale)
+
+
+def rule_given(d, scale):
+    """The same with q and k as they are."""
     q, k, v, g, beta, st = (d[n].double() for n in ("q", "k", "v", "g", "beta", "state"))
-    S, T, hv = v.shape[:3]
+    T, hv = v.shape[1:3]
     rep = hv // q.shape[2]
-    q = q / (q.square().sum(-1, keepdim=True) + eps).sqrt()
-    k = k / (k.square().sum(-1, keepdim=True) + eps).sqrt()
     out, big = torch.zeros_like(v), st.square().sum(2)
     for t in range(T):
         kt, qt = k[:, t].repeat_interleave(rep, 1), q[:, t].repeat_interleave(rep, 1)
         new = st * torch.exp(g[:, t])[..., None, None]
         u = beta[:, t][..., None] * (v[:, t] - (new * kt[..., None]).sum(2))
         new = new + kt[..., None] * u[..., None, :]
-        if lens is not None:
-            new = torch.where((t < lens)[:, None, None, None], new, st)
         st = new
         out[:, t] = scale * (st * qt[..., None]).sum(2)
         big = torch.maximum(big, st.square().sum(2))
@@ -117,3 +119,43 @@ def test_delta_a_stream_by_itself_and_among_others(S, T, hk, hv, dk, dv, dtype):
         d["v"][0], d["k"][0] = float("nan"), float("inf")
         out2, so2 = run_delta(d, hk, dtype)
         assert torch.equal(out[-1], out2[-1]) and torch.equal(so[-1], so2[-1])
+
+
+@pytest.mark.parametrize("what", ["beta", "g", "k", "q", "nan beta", "nan g", "nan k"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("S,T,t", [(1, 60, 25), (1, 60, 45), (1, 300, 168), (1, 300, 250), (300, 60, 45), (6, 420, 240)])
+def test_delta_what_is_not_finite_leaves_no_wrong_frame(S, T, t, dtype, what):
+    """Frames before it come out right or, in its chunk, not finite; never finite and wrong.  Keys as given."""
+    hk, hv, dk, dv = 1, 2, 64, 72 if S < 6 else 128
+    d = make(S, T, hk, hv, dk, dv, dtype, seed=T + t, l2norm=False)
+    ro, rs, big = rule_given(d, dk ** -0.5)
+    x = float("nan") if what.startswith("nan") else float("inf")
+    name = what.split()[-1]
+    if name in ("k", "q"):
+        d[name][-1, t, 0, 3] = x
+    else:
+        d[name][-1, t, 1] = x
+    out, so = run_delta(d, hk, dtype, l2norm=False)
+    part = 16 * 2.0 ** -23 * np.sqrt(T)
+    bound = HALF[dtype] * ro.abs() + (dk ** -0.5 * big * (part + (2.0 ** -10 if dtype == "bf16" else 0)))[:, None] + 2.0 ** -25
+    fine = (out.double() - ro).abs() <= bound
+    heads = [0, 1] if name in ("k", "q") else [1]
+    start = t // 64 * 64 if name != "q" else t
+    assert bool(fine[:-1].all()) and bool(fine[-1, :start].all()) and bool(fine[-1, :, [h for h in (0, 1) if h not in heads]].all())
+    assert bool((fine | ~torch.isfinite(out))[-1, :t].all())
+    if name == "q":  # only its own frame takes it
+        assert bool(fine[-1, t + 1:].all()) and bool(((so.double() - rs).abs() <= (part * big)[:, :, None]).all())
+        assert not bool(torch.isfinite(out[-1, t]).any())
+    else:
+        assert not bool(torch.isfinite(out[-1, t:, heads]).any()) and not bool(torch.isfinite(so[-1, heads]).any())
+
+
+@pytest.mark.parametrize("T", [3, 40, 300])
+@pytest.mark.parametrize("exponent", [-14, -17, -20])
+def test_delta_faintest_keys_of_fp16(T, exponent):
+    """Rows of fp16's subnormal numbers have their length too, beside eps (1e-6 is above it from 2^-14 on) and without."""
+    for eps in (1e-6, 0.0):
+        d = make(2, T, 1, 2, 64, 48, "f16", seed=T)
+        d["q"], d["k"] = (d["q"].float() * 2.0 ** exponent).half(), (d["k"].float() * 2.0 ** exponent).half()
+        got = run_delta(d, 1, "f16", eps=eps)
+        check(got, rule(d, 64 ** -0.5, eps=eps or 1e-60), 64 ** -0.5, "f16", T)
