@@ -352,14 +352,30 @@ __device__ __forceinline__ void norm_row(float (&h)[NCH][8], int kind, float eps
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[i][j] -= m;
     }
-    float v = 0.0f;
+    const auto square = [&] {
+        float v = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NCH; ++i)
+        for (int i = 0; i < NCH; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v = at[i].counts(j) ? fmaf(h[i][j], h[i][j], v) : v;
+            for (int j = 0; j < 8; ++j) v = at[i].counts(j) ? fmaf(h[i][j], h[i][j], v) : v;
+        return fmaf(sum(v), inv_n, eps);
+    };
+    float v = square();
+    // squares that left 32 bits: such rows of the wave (a longer row is the same in all its waves) at another scale, which
+    // the norm takes out again
+    const bool outside = !(v > 0x1p-100f && v < INFINITY);
+    if (__any(outside)) {
+        const float f = !outside ? 1.0f : v > 1.0f ? 0x1p-80f : 0x1p90f;
+#pragma unroll
+        for (int i = 0; i < NCH; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[i][j] *= f;
+        eps = eps * f * f;
+        v = square();
+    }
     // v_rsq_f32 is good to one unit in the last place; a row whose variance and eps are both 0 is infinite times 0, as
     // its definition is
-    const float r = __builtin_amdgcn_rsqf(fmaf(sum(v), inv_n, eps));
+    const float r = __builtin_amdgcn_rsqf(v);
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
 #pragma unroll
@@ -387,7 +403,7 @@ __device__ __forceinline__ float sigmoid(float z) {
 template <class T, class R, int TPR, int NCH, int MODE>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void norm_kernel(const nnsp_norm_args a) {
     constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;  // rows of a workgroup at a time
-    __shared__ float red[4 * (TPR > 64 ? TPR / 64 : 1)];
+    __shared__ float red[6 * (TPR > 64 ? TPR / 64 : 1)];  // of two norms: the mean, the squares, at most once more
     RowSum<TPR> sum{red};
     const int tid = threadIdx.x % TPR, n = a.dim;
     const unsigned rows = (unsigned)a.rows * (unsigned)a.groups;
