@@ -66,10 +66,8 @@ extern "C" {
  * The state, sums and exponentials are held in 32 bits or more.  Calls of more
  * than NNSP_DELTA_STEP_FRAMES frames may run in chunks of up to 64 on the matrix
  * cores, whose products take the state, what is made of it and fp32 q and k in 22
- * bits, each column of the state and of v under scales of its own; where the
- * output is bf16, what only the output takes (the state for S^T q^, and the
- * products of a chunk's frames among each other) goes in with 11 bits.  Decays
- * above 1 (g > 0) cost such calls precision by their product over 64 frames.
+ * bits, each column of the state and of v under scales of its own.  Decays above
+ * 1 (g > 0) cost such calls precision by their product over 64 frames.
  *
  * A value that is not finite in frame t spreads, as the recurrence has it, to
  * the later frames of its stream and head, from v and the state to their own

@@ -24,9 +24,7 @@
 // T has a power a row tile, shared by all columns.  q and k go in with their rows
 // scaled too: fp16 and bf16 in one part (exact down to 2^-19 and 2^-28 of a row's
 // largest, to 2^-30 and 2^-39 of it below), fp32 in two.  All other factors
-// (norms, decays, beta) multiply in 32 bits outside the products.  For bf16
-// outputs the products that reach only the output (Q S0, P U) use one part of
-// S0, P and U, 11 bits, below the output's own 8.
+// (norms, decays, beta) multiply in 32 bits outside the products.
 //
 // Layout.  A wave owns 16 NB columns of the state and keeps them in registers
 // in the 16x16 accumulator layout (lane: column lane % 16, rows 4 (lane / 16)
@@ -158,14 +156,12 @@ __device__ __forceinline__ _Float16 half_of(float x, float s) {
 }
 // two accumulator tiles times their rows' factors s as the high and low B
 // operand of a 32-deep product
-template <bool LOW>
 __device__ __forceinline__ void split(const f32x4& a, const f32x4& b, const f32x4& sa, const f32x4& sb, h8& hi, h8& lo) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) hi[i] = half_of(i < 4 ? a[i & 3] : b[i & 3], i < 4 ? sa[i & 3] : sb[i & 3]);
-    if (LOW)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            lo[i] = (_Float16)fmaf(i < 4 ? a[i & 3] : b[i & 3], i < 4 ? sa[i & 3] : sb[i & 3], -(float)hi[i]);
+    for (int i = 0; i < 8; ++i)
+        lo[i] = (_Float16)fmaf(i < 4 ? a[i & 3] : b[i & 3], i < 4 ? sa[i & 3] : sb[i & 3], -(float)hi[i]);
 }
 __device__ __forceinline__ f32x4 all4(float x) { return f32x4{x, x, x, x}; }
 
@@ -197,7 +193,6 @@ template <class T, int NKT, int NB>
 struct Geo {
     static constexpr bool WIDE = std::is_same<T, float>::value;       // 32-bit input
     static constexpr int KP = WIDE ? 2 : 1;                           // parts of q and k
-    static constexpr int OP = std::is_same<T, __bf16>::value ? 1 : 2; // parts of what only the output takes
     static constexpr int VS = 16 * NB + 4;                            // row of a wave's V, elements
 };
 
@@ -212,8 +207,7 @@ struct KQ {
 // what else a chunk's products take; e() is a decay, G the sum of g
 template <class T, int C>
 struct TP {
-    static constexpr int OP = std::is_same<T, __bf16>::value ? 1 : 2;
-    Tri<C> P_[OP];
+    Tri<C> P_[2];
     alignas(16) float beta[C], fx[C], fk[C], fq[C];  // factors of v, K S0, U into the state, Q S0
     alignas(16) float pi[C];                         // 2^-scale of P's rows
     float ti[4];                                     // 2^-scale of T's row tiles
@@ -425,7 +419,7 @@ __device__ __forceinline__ void put_p(TP<T, C>& Y, const Make<C>& M, const f32x4
         }
     }
     Y.P_[0].put(mi, l15, j, g, a);
-    if (TP<T, C>::OP == 2) Y.P_[TP<T, C>::OP - 1].put(mi, l15, j, g, b);
+    Y.P_[1].put(mi, l15, j, g, b);
 }
 
 // block (mi, j) of T, transposed, times s
@@ -575,23 +569,21 @@ __device__ __forceinline__ f32x4 tile_of(const T (*V)[VS], int n, int l15, int g
     return v;
 }
 
-// K S0 and R of a chunk of 32 with nt live tiles of 16 frames, for this wave's
-// columns; with LOW outputs also Q S0, whose high part outlasts R otherwise (in
-// fewer registers).  S holds the state times 1 / sinv, powers of two; a lane's
+// K S0, R and Q S0 of a chunk of 32 with nt live tiles of 16 frames, for this
+// wave's columns.  S holds the state times 1 / sinv, powers of two; a lane's
 // scales are those of its column.
 template <class T, int NKT, int NB>
 struct Chunk {
     using G = Geo<T, NKT, NB>;
-    static constexpr bool LOW = G::OP == 2;
-    f32x4 R[2][NB], O[LOW ? 2 : 1][NB];
-    h8 shi[NKT][NB];
-    float smax[NB], rmax[NB], sout[NB];
+    f32x4 R[2][NB], O[2][NB];
+    float smax[NB], rmax[NB];
 
     __device__ __forceinline__ void first(const KQ<T, NKT, 32>& X, const TP<T, 32>& Y, T (*V)[G::VS], const f32x4 (&S)[2 * NKT][NB],
                                           const float (&sinv)[NB], int lane, int nt) {
         const int l15 = lane & 15, g = lane >> 4;
         const f32x4 zero = {0, 0, 0, 0};
-        h8 lo[NKT][NB];
+        h8 hi[NKT][NB], lo[NKT][NB];
+        float sout[NB];
 #pragma unroll
         for (int n = 0; n < NB; ++n) {
             float m = 0.0f, inv;
@@ -602,7 +594,7 @@ struct Chunk {
             const float sc = scale_of(smax[n], inv);
             sout[n] = fmaf(inv, sinv[n], poison(smax[n]));
 #pragma unroll
-            for (int t = 0; t < NKT; ++t) split<true>(S[2 * t][n], S[2 * t + 1][n], all4(sc), all4(sc), shi[t][n], lo[t][n]);
+            for (int t = 0; t < NKT; ++t) split(S[2 * t][n], S[2 * t + 1][n], all4(sc), all4(sc), hi[t][n], lo[t][n]);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -616,19 +608,19 @@ struct Chunk {
             for (int s = 0; s < NKT; ++s) {
                 const int c = 32 * s + 8 * g;
                 const h8 k = *reinterpret_cast<const h8*>(&X.K[0][16 * m + l15][c]);
-                h8 q, kl, ql;
-                if (LOW) q = *reinterpret_cast<const h8*>(&X.Q[0][16 * m + l15][c]);
+                const h8 q = *reinterpret_cast<const h8*>(&X.Q[0][16 * m + l15][c]);
+                h8 kl, ql;
                 if (G::KP == 2) {
                     kl = *reinterpret_cast<const h8*>(&X.K[G::KP - 1][16 * m + l15][c]);
                     ql = *reinterpret_cast<const h8*>(&X.Q[G::KP - 1][16 * m + l15][c]);
                 }
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
-                    x[n] = mma(k, lo[s][n], mma(k, shi[s][n], s ? x[n] : zero));
-                    if (LOW) o[n] = mma(q, lo[s][n], mma(q, shi[s][n], s ? o[n] : zero));
+                    x[n] = mma(k, lo[s][n], mma(k, hi[s][n], s ? x[n] : zero));
+                    o[n] = mma(q, lo[s][n], mma(q, hi[s][n], s ? o[n] : zero));
                     if (G::KP == 2) {
-                        x[n] = mma(kl, shi[s][n], x[n]);
-                        o[n] = mma(ql, shi[s][n], o[n]);
+                        x[n] = mma(kl, hi[s][n], x[n]);
+                        o[n] = mma(ql, hi[s][n], o[n]);
                     }
                 }
             }
@@ -638,7 +630,7 @@ struct Chunk {
                 const f32x4 v = tile_of<T>(V + 16 * m, n, l15, g) * b, fx = f * -sout[n];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) R[m][n][r] = fmaf(fx[r], x[n][r], v[r]);
-                if (LOW) O[LOW ? m : 0][n] = o[n] * (ld4(&Y.fq[16 * m + 4 * g]) * sout[n]);
+                O[m][n] = o[n] * (ld4(&Y.fq[16 * m + 4 * g]) * sout[n]);
                 rmax[n] = amax4(rmax[n], R[m][n]);
             }
         }
@@ -659,7 +651,7 @@ struct Chunk {
             rmax[n] = max_xor16_32(rmax[n]);
             rs[n] = scale_of(rmax[n], inv);
             ti[n] = fmaf(Y.ti[0], inv, poison(rmax[n]));
-            split<true>(R[0][n], R[1][n], all4(rs[n]), all4(rs[n]), hi[n], lo[n]);
+            split(R[0][n], R[1][n], all4(rs[n]), all4(rs[n]), hi[n], lo[n]);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
@@ -669,31 +661,24 @@ struct Chunk {
         }
 #pragma unroll
         // u to below 2^14: times 2^-22
-        for (int n = 0; n < NB; ++n) split<LOW>(u[0][n], u[1][n], all4(0x1p-22f), all4(0x1p-22f), hi[n], lo[n]);
+        for (int n = 0; n < NB; ++n) split(u[0][n], u[1][n], all4(0x1p-22f), all4(0x1p-22f), hi[n], lo[n]);
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
             if (m >= nt) continue;
-            const h8 ph = Y.P_[0].operand(m, l15, 0, g);
-            f32x4 o[NB], qs[NB];
+            const h8 ph = Y.P_[0].operand(m, l15, 0, g), pl = Y.P_[1].operand(m, l15, 0, g);
+            f32x4 o[NB];
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 o[n] = mma(ph, hi[n], zero);
-                if (LOW) o[n] = mma(Y.P_[G::OP - 1].operand(m, l15, 0, g), hi[n], mma(ph, lo[n], o[n]));
+                o[n] = mma(pl, hi[n], mma(ph, lo[n], o[n]));
             }
-            if (!LOW)
-#pragma unroll
-                for (int s = 0; s < NKT; ++s) {
-                    const h8 q = *reinterpret_cast<const h8*>(&X.Q[0][16 * m + l15][32 * s + 8 * g]);
-#pragma unroll
-                    for (int n = 0; n < NB; ++n) qs[n] = mma(q, shi[s][n], s ? qs[n] : zero);
-                }
-            const f32x4 p = ld4(&Y.pi[16 * m + 4 * g]), f = ld4(&Y.fq[16 * m + 4 * g]);
+            const f32x4 p = ld4(&Y.pi[16 * m + 4 * g]);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                const f32x4 pi = p * (ti[n] * 0x1p22f), fq = f * sout[n];
+                const f32x4 pi = p * (ti[n] * 0x1p22f);
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    V[16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], LOW ? O[LOW ? m : 0][n][r] : fq[r] * qs[n][r]);
+                    V[16 * m + 4 * g + r][16 * n + l15] = (T)fmaf(o[n][r], pi[r], O[m][n][r]);
             }
         }
         mid();
@@ -710,7 +695,7 @@ struct Chunk {
             const float s = fminf(z * rs[n], low), d = all * s * sinv[n];  // true U fk times s = u fk (ti s)
             sinv[n] = inverse2(s);
             const f32x4 f0 = fk0 * (ti[n] * s), f1 = fk1 * (ti[n] * s);
-            split<true>(u[0][n], u[1][n], f0, f1, hi[n], lo[n]);
+            split(u[0][n], u[1][n], f0, f1, hi[n], lo[n]);
 #pragma unroll
             for (int t = 0; t < 2 * NKT; ++t) S[t][n] *= d;
         }
@@ -937,7 +922,11 @@ struct Tiles {
     }
 };
 
-// waves per SIMD that the state and the operands leave registers and LDS for
+// Waves per SIMD that the state and the operands leave registers and LDS for.  Keys
+// of 97 to 128 in 16 bits by 16 columns spill 7 to 39 registers at three, which
+// two would not; 512 streams of 100 frames, 4 heads, at three and two, us, bf16
+// and fp16: 128 x 64 111 and 112, 107 and 106; 128 x 48 103 and 100, 100 and 94;
+// 100 x 64 (keys read by elements) 189 and 206, 191 and 203.
 template <class T, int NKT, int NB, int NW>
 constexpr int fused_waves() {
     return Geo<T, NKT, NB>::WIDE && NKT > 4 && NW == 4 ? 1 : Geo<T, NKT, NB>::WIDE || NB == 2 || NKT > 4 ? 2 : 3;
@@ -1202,18 +1191,14 @@ __device__ __forceinline__ void copy_in(X& x, const char* sx, Y& y, const char* 
 }
 
 // a tile times its rows' factors, as half of the high and low B operand that it is part of
-template <bool LOW>
 __device__ __forceinline__ void put_part(h8 (*dst)[64], int lane, int half, const f32x4& x, const f32x4& s) {
-    h4 hi;
+    h4 hi, lo;
 #pragma unroll
     for (int i = 0; i < 4; ++i) hi[i] = half_of(x[i], s[i]);
     reinterpret_cast<h4*>(&dst[0][lane])[half] = hi;
-    if (LOW) {
-        h4 lo;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) lo[i] = (_Float16)fmaf(x[i], s[i], -(float)hi[i]);
-        reinterpret_cast<h4*>(&dst[1][lane])[half] = lo;
-    }
+    for (int i = 0; i < 4; ++i) lo[i] = (_Float16)fmaf(x[i], s[i], -(float)hi[i]);
+    reinterpret_cast<h4*>(&dst[1][lane])[half] = lo;
 }
 
 // What the four waves of a scan hand each other: B operands of 32 rows x 16
@@ -1250,7 +1235,6 @@ struct ScanLds {
 template <class T, int NKT, int NB, bool FAST, int XB, int YB>
 __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a, const Slab b) {
     using G = Geo<T, NKT, NB>;
-    constexpr bool LOW = G::OP == 2;
     constexpr int TPW = (2 * NKT + 3) / 4;  // state tiles of a wave
     __shared__ ScanLds<T, NKT, NB, XB, YB> L;
     const int lane_ = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -1358,7 +1342,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
             for (int j = 0; j < TPW; ++j) {
                 const int t = wave * TPW + j;
                 if (t >= 2 * NKT) continue;  // not a tile of the state; its registers are never handed on
-                put_part<true>(E.S[t >> 1][n], lane, t & 1, S[j][n], all4(sc));
+                put_part(E.S[t >> 1][n], lane, t & 1, S[j][n], all4(sc));
                 m[n] = amax4(m[n], S[j][n]);
             }
         }
@@ -1391,8 +1375,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
                 for (int n = 0; n < NB; ++n) {
                     const h8 hi = E.S[s][n][0][lane], lo = E.S[s][n][1][lane];
                     x[n] = mma(k, lo, mma(k, hi, s ? x[n] : zero));
-                    O[n] = mma(q, hi, s ? O[n] : zero);
-                    if (LOW) O[n] = mma(q, lo, O[n]);
+                    O[n] = mma(q, lo, mma(q, hi, s ? O[n] : zero));
                     if (G::KP == 2) {
                         x[n] = mma(*reinterpret_cast<const h8*>(&X.K[G::KP - 1][16 * wave + l15][c]), hi, x[n]);
                         O[n] = mma(*reinterpret_cast<const h8*>(&X.Q[G::KP - 1][16 * wave + l15][c]), hi, O[n]);
@@ -1407,7 +1390,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
                 f32x4 r = vt[n] * bt;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) r[e] = fmaf(f[e], x[n][e], r[e]);
-                put_part<true>(E.R[wave >> 1][n], lane, wave & 1, r, all4(sc[n]));
+                put_part(E.R[wave >> 1][n], lane, wave & 1, r, all4(sc[n]));
                 O[n] *= fq * inv[n];
             }
         }
@@ -1449,8 +1432,8 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
             }
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
-                put_part<true>(E.F[wave >> 1][n], lane, wave & 1, u[n], f[n]);
-                put_part<LOW>(E.U[wave >> 1][n], lane, wave & 1, u[n], all4(ti * c));
+                put_part(E.F[wave >> 1][n], lane, wave & 1, u[n], f[n]);
+                put_part(E.U[wave >> 1][n], lane, wave & 1, u[n], all4(ti * c));
                 m[n] = amax4(0.0f, u[n] * f[n]);
             }
             put_max(E.fmax, lane);
@@ -1473,7 +1456,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
             for (int s = 0; s < 2; ++s)
                 if (2 * s <= wave) {
                     ph[s] = Y.P_[0].operand(wave, l15, s, g);
-                    if (LOW) pl[s] = Y.P_[G::OP - 1].operand(wave, l15, s, g);
+                    pl[s] = Y.P_[1].operand(wave, l15, s, g);
                 }
             pi = ld4(&Y.pi[16 * wave + 4 * g]);
         }
@@ -1503,8 +1486,7 @@ __global__ __launch_bounds__(512) void delta_scan_kernel(const nnsp_delta_args a
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     const h8 hi = E.U[s][n][0][lane];
-                    o[n] = mma(ph[s], hi, s ? o[n] : zero);
-                    if (LOW) o[n] = mma(pl[s], hi, mma(ph[s], E.U[s][n][1][lane], o[n]));
+                    o[n] = mma(pl[s], hi, mma(ph[s], E.U[s][n][1][lane], mma(ph[s], hi, s ? o[n] : zero)));
                 }
             }
 #pragma unroll

@@ -15,8 +15,7 @@ state's column over the frames (its start too) plus the largest |v| of it:
     cancels.  |beta k k^T| <= 1 lets no error grow, and errors of the frames
     have random signs: part = 16 * 2^-23 * sqrt(frames).
   * out = scale q . S: scale * part * big, and one rounding to its type (half a
-    step of the value, or of the smallest subnormal).  For bf16 three operands
-    of what only the output takes have 11 bits, 2^-12 each: 2^-10 of big.
+    step of the value, or of the smallest subnormal).
 """
 import numpy as np
 import pytest
@@ -54,7 +53,7 @@ def check(got, ref, scale, dtype, T):
     (out, so), (ro, rs, big) = got, ref
     part = 16 * 2.0 ** -23 * np.sqrt(T)
     least = 2.0 ** -25 if dtype == "f16" else 2.0 ** -134 if dtype == "bf16" else 2.0 ** -150
-    bound = HALF[dtype] * ro.abs() + least + (scale * big * (part + (2.0 ** -10 if dtype == "bf16" else 0)))[:, None]
+    bound = HALF[dtype] * ro.abs() + least + (scale * big * part)[:, None]
     for what, off, most in (("out", (out.double() - ro).abs(), bound), ("state", (so.double() - rs).abs(), (part * big)[:, :, None])):
         at = torch.nonzero(~(off <= most))
         assert len(at) == 0, f"{what}: {len(at)} of {off.numel()} beyond the bound, at {at[0].tolist()} by {float((off / most).max()):.3g}"
@@ -137,7 +136,7 @@ def test_delta_what_is_not_finite_leaves_no_wrong_frame(S, T, t, dtype, what):
         d[name][-1, t, 1] = x
     out, so = run_delta(d, hk, dtype, l2norm=False)
     part = 16 * 2.0 ** -23 * np.sqrt(T)
-    bound = HALF[dtype] * ro.abs() + (dk ** -0.5 * big * (part + (2.0 ** -10 if dtype == "bf16" else 0)))[:, None] + 2.0 ** -25
+    bound = HALF[dtype] * ro.abs() + (dk ** -0.5 * big * part)[:, None] + 2.0 ** -25
     fine = (out.double() - ro).abs() <= bound
     heads = [0, 1] if name in ("k", "q") else [1]
     start = t // 64 * 64 if name != "q" else t
