@@ -67,7 +67,10 @@ extern "C" {
  * than NNSP_DELTA_STEP_FRAMES frames may run in chunks of up to 64 on the matrix
  * cores, whose products take the state, what is made of it and fp32 q and k in 22
  * bits, each column of the state and of v under scales of its own.  Decays above
- * 1 (g > 0) cost such calls precision by their product over 64 frames.
+ * 1 (g > 0) cost such calls precision by their product over 64 frames (beyond
+ * 2^20 none is left: take such frames in calls of NNSP_DELTA_STEP_FRAMES).
+ * How many streams, heads and frames a call has decides which of its forms runs;
+ * what the other streams and heads hold changes no bit of a result.
  *
  * A value that is not finite in frame t spreads, as the recurrence has it, to
  * the later frames of its stream and head, from v and the state to their own

@@ -158,3 +158,29 @@ def test_delta_faintest_keys_of_fp16(T, exponent):
         d["q"], d["k"] = (d["q"].float() * 2.0 ** exponent).half(), (d["k"].float() * 2.0 ** exponent).half()
         got = run_delta(d, 1, "f16", eps=eps)
         check(got, rule(d, 64 ** -0.5, eps=eps or 1e-60), 64 ** -0.5, "f16", T)
+
+
+@pytest.mark.parametrize("T", [1, 12])
+@pytest.mark.parametrize("dk,dv,streams", [(1, 1, (1 << 24) - 1), (33, 80, ((1 << 24) - 1) // 5)])
+def test_delta_as_many_streams_as_there_may_be(dk, dv, streams, T):
+    """The largest grids, frame by frame and in chunks, on inputs that all streams share; the first, the last and some
+    between against the rule."""
+    if T > 1 and dk > 1:
+        streams //= 8  # its states alone would be 35 GB
+    d = make(1, T, 1, 1, dk, dv, "f32", seed=dk)
+    from nnsp_amd.seq import GatedDelta
+    zero = {n: (0, h * w, w) for n, h, w in (("q", 1, dk), ("k", 1, dk), ("g", 1, 1), ("beta", 1, 1))}
+    p = GatedDelta(streams, T, 1, 1, dk, dv, dtype="f32", strides=dict(zero, v=(1, dv, dv)))
+    v = torch.randn(streams + T * dv, generator=torch.Generator().manual_seed(1)).cuda()  # stream s: from element s on
+    out = torch.full((streams, T, dv), 7.0, device="cuda")
+    so = torch.full((streams, dk, dv), 7.0, device="cuda")
+    assert p.workspace_bytes == 0
+    p.exec_device(d["q"].data_ptr(), d["k"].data_ptr(), v.data_ptr(), d["g"].data_ptr(), d["beta"].data_ptr(), out.data_ptr(),
+                  state_out=so.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    at = [0, 1, streams // 3, streams // 2 + 1, streams - 2, streams - 1]
+    some = {n: d[n].expand(len(at), *d[n].shape[1:]) for n in ("q", "k", "g", "beta")}
+    some["v"] = torch.stack([v[s:s + T * dv].view(T, 1, dv) for s in at])
+    some["state"] = torch.zeros(len(at), 1, dk, dv, device="cuda")
+    check((out[at][:, :, None], so[at][:, None]), rule(some, dk ** -0.5), dk ** -0.5, "f32", T)
+    assert bool((so != 7).any(-1).any(-1).all())
