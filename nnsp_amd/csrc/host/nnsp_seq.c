@@ -161,24 +161,24 @@ enum { DELTA_STEP, DELTA_CHUNK, DELTA_SPLIT };
 static int delta_way(const nnsp_delta_args *a)
 {
     /* A frame by itself costs 0.9 to 2 us after the first, a chunk of up to 32
-     * about 7 to 13 us whatever it holds; rows of dk = 32 cost little more frame
+     * about 6 to 10 us whatever it holds; rows of dk = 32 cost little more frame
      * by frame.  Frames against a chunk, bf16, us, 4096 rows: dk = dv = 32, 8
-     * frames 27 against 39; 64, 4 frames 42 against 45, 6 frames 50 against 45;
-     * 96, 4 frames 82 against 87, 6 frames 102 against 87; 128, 2 frames 121
-     * against 118, 4 frames 156 against 120.  One row, 4 frames: 32 8.4 against
-     * 6.9, 64 8.5 against 7.2, 128 10.9 against 8.6. */
+     * frames 26 against 36; 64, 4 frames 39 against 43, 6 frames 47 against 43;
+     * 96, 4 frames 81 against 78, 6 frames 98 against 80; 128, 2 frames 119
+     * against 127, 4 frames 154 against 128.  One row, 4 frames: 32 6.2 against
+     * 6.2, 64 8.6 against 6.5, 128 9.4 against 7.6. */
     if (a->n_frames <= (a->dk <= 32 ? 8 : a->dk <= 96 ? 4 : NNSP_DELTA_STEP_FRAMES)) return DELTA_STEP;
     /* Two passes shorten the chain of a call whose few rows leave CUs idle, and
      * move twice the bytes.  What counts is how many workgroups of 16 columns
      * the second pass has for 256 CUs.  Chunks against two passes, us.  bf16, dk =
-     * dv = 64: 256 workgroups, 260 frames 28 against 28, 500 frames 45 against 36;
-     * 512: 260 frames 29 against 35, 500 frames 46 against 42; 768: 1000 frames 84
-     * against 107.  128: 256, 130 frames 21 against 24, 260 frames 33 against 29;
-     * 512: 260 frames 34 against 37, 500 frames 55 against 46, 1000 frames 103
-     * against 67; 1024: 1000 frames 109 against 126.  fp32, 128: 256, 260 frames
-     * 40 against 41, 500 frames 65 against 56; 512: 500 frames 70 against 60.
+     * dv = 64: 256 workgroups, 260 frames 28 against 25, 500 frames 45 against 33;
+     * 512: 260 frames 28 against 38, 500 frames 46 against 46; 768: 1000 frames 86
+     * against 147.  128: 256, 130 frames 20 against 20, 260 frames 33 against 25;
+     * 512: 260 frames 33 against 36, 500 frames 55 against 43, 1000 frames 104
+     * against 74; 1024: 1000 frames 106 against 156.  fp32, 128: 256, 260 frames
+     * 38 against 38, 500 frames 64 against 49; 512: 500 frames 65 against 63.
      * Wider keys, whose chunks go one after the other, 160 x 128, bf16: 256, 130
-     * frames 32 against 27; 512, 260 frames 56 against 44.  LDS has no room for 64
+     * frames 31 against 23; 512, 260 frames 54 against 49.  LDS has no room for 64
      * frames of fp32 wider than 128. */
     const long long groups = (long long)a->n_streams * a->value_heads * ((a->dv + 15) / 16);
     if (a->dtype == NNSP_F32 && a->dk > 128) return DELTA_CHUNK;

@@ -50,7 +50,7 @@ typedef short s4 __attribute__((ext_vector_type(4)));
 // of 8192 streams, 2 heads of 64 x 64: chunks of 64 667 us, of 32 607 us then)
 constexpr int C = 64, CF = 32;
 // images of a slab, inside the 256 MB cache behind the L2s (16384 frames of 32
-// heads of 128 x 128, us: 32 MB 703, 96 MB 633, 200 MB 619; fp32 932, 870, 892)
+// heads of 128 x 128, us: 32 MB 737, 96 MB 607, 200 MB 625; fp32 1295, 1250, 1290)
 constexpr long long DELTA_SLAB_BYTES = 96ll << 20;
 
 // sizes of a call in two passes
@@ -936,14 +936,14 @@ constexpr int fused_waves() {
 // chunks of 32 alone, and the workgroups of a CU fill each other's waits.
 // FAST: dk and dv are multiples of 8.  SPARE: dv leaves the last of them waves
 // without columns, which only help with the tiles and the inverse (512 streams of
-// 100 frames, 4 heads of 72 x 72, bf16: 134 -> 118 us; asking costs registers: 128
-// x 128, which has none, 168 -> 176).
+// 100 frames, 4 heads of 72 x 72, bf16: 139 -> 121 us; where all have some, asking
+// costs registers: 8192 streams of 64 x 64 518 -> 528, fp32 of 128 x 128 252 ->
+// 255, bf16 of 96 x 128 147 -> 149, of 128 x 128 171 -> 169).
 //
-// 100 frames of 8192 streams, 2 heads of 64 x 64, fp16: 505 us, of which the bytes
-// alone would take 280; the vector units issue 68 % of the time (splits, factors,
-// addresses: some 680 instructions a wave and chunk, 38 of them matrix ones), at
-// three waves a SIMD.  512 streams of 4 heads of 128 x 128, bf16: 159 us, bytes
-// 98.
+// 100 frames of 8192 streams, 2 heads of 64 x 64, fp16: 500 us, of which the bytes
+// alone would take 257; the vector units issue 67 % of the time (splits, factors,
+// addresses: some 660 instructions a wave and chunk, and 38 matrix ones), at three
+// waves a SIMD.  512 streams of 4 heads of 128 x 128, bf16: 169 us, bytes 98.
 template <class T, int NKT, int NB, int NW, bool FAST, bool SPARE>
 __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delta_chunk_kernel(const nnsp_delta_args a) {
     using G = Geo<T, NKT, NB>;
@@ -1022,9 +1022,9 @@ __global__ __launch_bounds__(64 * NW, (fused_waves<T, NKT, NB, NW>())) void delt
 // Few rows, some chunks: the same with the parts of a chunk's work beside each
 // other.  While waves 0 .. 3, 16 columns each, take chunk c through the state,
 // wave 8 inverts chunk c + 1 and waves 4 .. 7 stage chunk c + 2 and make its
-// tiles.  All meet three times a period; only 4 .. 7 need that.  A chunk takes
-// the 6000 cycles of 4 .. 7 (the others' parts 4900 and 3200), one after the
-// other 13000.
+// tiles.  All meet three times a period; only 4 .. 7 need that.  A chunk of 128
+// rows of 128 x 128, bf16, takes 3.1 us, where one part after the other takes
+// about 5.
 template <class T, int NKT>
 struct PipeLds {
     KQ<T, NKT, CF> X[3];
@@ -1134,8 +1134,8 @@ __device__ __forceinline__ void copy_out(char* dst, const X& src, int tid) {
 }
 
 // One workgroup per stream, key head and chunk, for all the key head's value heads.
-// 64 chunks of 16 key heads and 32 value heads, 128 wide, bf16: 40 us for 34 MB in
-// and 83 MB out, that is 2.1 TB/s of stores, where a large copy's are 2.5 (workgroups
+// 64 chunks of 16 key heads and 32 value heads, 128 wide, bf16: 41 us for 34 MB in
+// and 97 MB out, that is 2.4 TB/s of stores, where a large copy's are 2.5 (workgroups
 // that stay and fetch their next chunk beside the work on one took as long).
 template <class T, int NKT, bool FAST>
 __global__ __launch_bounds__(256, (sizeof(KQ<T, NKT, C>) > 48 * 1024 ? 1 : 2)) void delta_prepare_kernel(const nnsp_delta_args a, const Slab b) {
@@ -1225,7 +1225,7 @@ struct ScanLds {
 // K S0, T R, Q S0 and P U, a quarter of the state's rows in K^T U, handing its
 // results on through LDS (three barriers a chunk).  Waves 4 .. 7 bring the next
 // chunk's images meanwhile, a third after each barrier: all at once they hold up
-// the products' own reads of LDS (64 chunks of 128 x 128 bf16: 127 us, all after
+// the products' own reads of LDS (64 chunks of 128 x 128 bf16: 126 us, all after
 // the first barrier 148, none 121).  Where LDS has no room for two of an image, it
 // comes after the third barrier, when the one before has been read.
 // A column's scales have to be the same for all four before anybody has seen all
@@ -1565,7 +1565,7 @@ void launch_split(const nnsp_delta_args& a, hipStream_t st) {
         delta_prepare_kernel<T, NKT, FAST>
             <<<dim3((unsigned)((long long)a.n_streams * a.key_heads * b.chunks)), dim3(256), 0, st>>>(a, b);
         // 16 columns a workgroup while each still has a CU to itself, else 32 (LDS has room for one workgroup): 1000
-        // frames of 128 x 128, bf16, us, 32 rows 55 and 65, 40 rows 83 and 66
+        // frames of 128 x 128, bf16, us, 32 rows 49 and 61, 40 rows 81 and 68
         if (rows * ((a.dv + 15) / 16) <= 256) launch_scan<T, NKT, 1, FAST>(a, b, st);
         else launch_scan<T, NKT, 2, FAST>(a, b, st);
     }
@@ -1573,8 +1573,8 @@ void launch_split(const nnsp_delta_args& a, hipStream_t st) {
 
 // f<NKT, FAST>() of this call's sizes: keys go in by 32 columns, padded to one of
 // a few widths (512 streams of 100 frames, 4 heads of 192 x 128, bf16: padded to
-// 192 310 us, to 256 355; one stream of 4000 frames, 8 heads of 160 x 128, in two
-// passes 146 and 226)
+// 192 256 us, to 256 307; one stream of 4000 frames, 8 heads of 160 x 128, in two
+// passes 158 and 245)
 template <class F>
 auto with_sizes(const nnsp_delta_args& a, const F& f) {
     typedef std::integral_constant<int, 1> I1;
@@ -1613,9 +1613,9 @@ int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
         }
         // Workgroups of 64 columns that work on three chunks at once (pipe, keys up to 128 wide) while each has a CU to
         // itself, else such as share a CU, of 128 columns where there are so many (fused).  260 frames, dk = dv, us, pipe
-        // against fused, bf16: 64, 32 rows 28 and 41, 256 rows 30 and 42, 384 rows 53 and 51; 128, 32 rows 33 and 47 (by 64
-        // columns), 128 rows 37 and 50, 192 rows 66 and 59; fp32: 64, 256 rows 35 and 46, 384 rows 62 and 57; 128, 128
-        // rows 45 and 58, 192 rows 80 and 66.  20 frames, 64: 9 and 9; 128, 128 rows 11 and 12.
+        // against fused, bf16: 64, 32 rows 27 and 39, 256 rows 31 and 40, 384 rows 54 and 50; 128, 32 rows 33 and 51 (by 64
+        // columns), 128 rows 38 and 54, 192 rows 66 and 61; fp32: 64, 256 rows 33 and 44, 384 rows 60 and 56; 128, 128
+        // rows 42 and 61, 192 rows 77 and 63.  20 frames, 64: 7 and 7; 128, 128 rows 10 and 11.
         const long long groups = (long long)a.n_streams * a.value_heads * ((a.dv + 63) / 64);
         if constexpr (NKT <= 4) {
             if (groups <= 256) {
@@ -1623,9 +1623,9 @@ int launch_chunk(const nnsp_delta_args& a, int split, hipStream_t st) {
                 return 0;
             }
         }
-        // Keys over 128 leave registers for 64 columns in 16 bits (512 rows of 256 x 256, 200 frames: 258 us, 128 columns
+        // Keys over 128 leave registers for 64 columns in 16 bits (512 rows of 256 x 256, 200 frames: 256 us, 128 columns
         // by 8 waves 276), and fp32 is faster by 64 while CUs are left over (64 streams of 8 frames, 8
-        // heads of 256 x 256: 114 us by 64, by 128 85; one stream, 2000 frames 521 and 624)
+        // heads of 256 x 256: 112 us by 64, by 128 80; one stream, 2000 frames 529 and 617)
         const bool narrow = a.dv <= 64 || (NKT > 4 && groups <= 256);
         if constexpr (WIDE) narrow ? launch_fused<T, NKT, 1, 4, FAST>(a, st) : launch_fused<T, NKT, 1, 8, FAST>(a, st);
         else if constexpr (NKT > 4) launch_fused<T, NKT, 1, 4, FAST>(a, st);
